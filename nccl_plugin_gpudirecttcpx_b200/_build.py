@@ -7,6 +7,7 @@ entry file and the test-suite can produce the libraries with nothing but nvcc
 and g++.  Outputs land in `nccl_plugin_gpudirecttcpx_b200/_lib/`:
 
   libtcpxb_kernels.so   device kernels behind a C ABI (needs nvcc)
+  libtcpxb_train.so     the training step's operators behind a C ABI (needs nvcc)
   libnccl-net.so        the NCCL net plugin: host core + kernels + engine (needs nvcc)
   libtcpxb_host.so      host core + engine with no CUDA: device calls go to a stand-in
                         device in host memory (g++ only; used by CPU tests)
@@ -122,7 +123,12 @@ def build_cuda(verbose: bool = False) -> list[Path]:
     klib = OUT / "libtcpxb_kernels.so"
     if _stale(klib, kobjs, 0.0):
         _run([nvcc, "-shared", "-o", str(klib)] + [str(o) for o in kobjs] + ["-cudart", "static"])
-    outs = [klib]
+    tobjs = _compile(_sources("train", ".cu"), "cu", nv, NVCC_FLAGS, hdr, verbose)
+    tobjs += _compile(_sources("train", ".cc"), "full", ["g++"], CXX_FLAGS + ["-I", _cuda_include(nvcc)], hdr, verbose)
+    tlib = OUT / "libtcpxb_train.so"
+    if _stale(tlib, tobjs, 0.0):
+        _run([nvcc, "-shared", "-o", str(tlib)] + [str(o) for o in tobjs] + ["-cudart", "static"])
+    outs = [klib, tlib]
     core = _sources("core", ".cc") + _sources("plugin", ".cc") + _sources("engine", ".cc")
     if core:
         cobjs = _compile(core, "full", ["g++"], CXX_FLAGS + ["-I", _cuda_include(nvcc)], hdr, verbose)

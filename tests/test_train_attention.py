@@ -1,0 +1,279 @@
+"""Attention forward and backward against the definition in 64 bits, at the sizes and masks where tiles end."""
+import math
+
+import pytest
+import torch
+
+import train_oracle as oracle
+from nccl_plugin_gpudirecttcpx_b200 import ops
+
+gpu = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def inputs(b, sq, sk, h, hk, d, dtype, seed=0, device="cuda"):
+    g = torch.Generator(device=device).manual_seed(seed)
+    return [torch.randn(s, device=device, generator=g).to(dtype) for s in ((b, sq, h, d), (b, sk, hk, d), (b, sk, hk, d), (b, sq, h, d))]
+
+
+def check(q, k, v, dout, causal=False, lengths=None, scale=None):
+    how = {"causal": causal, "key_lengths": lengths, "scale": scale}
+    out, lse = ops.attention_forward(q, k, v, **how)
+    dq, dk, dv = ops.attention_backward(dout, q, k, v, out, lse, **how)
+    want = oracle.attention(q, k, v, dout, causal, lengths, scale)
+    for name, got in (("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
+        oracle.close(got, want[name], name)
+    return out, lse, dq, dk, dv
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d", [
+    (1, 1, 1, 1, 1, 8), (2, 1, 17, 4, 2, 64), (1, 17, 1, 2, 1, 64), (3, 64, 64, 4, 2, 16), (1, 127, 127, 2, 1, 64), (1, 128, 128, 2, 1, 128),
+    (1, 129, 129, 2, 2, 64), (1, 129, 127, 2, 2, 128), (1, 200, 72, 3, 1, 40), (2, 257, 513, 6, 3, 96), (1, 300, 641, 4, 4, 64),
+    (2, 255, 256, 8, 1, 72), (1, 1000, 1000, 2, 1, 128), (1, 385, 385, 5, 5, 24), (1, 2, 1500, 4, 2, 64), (1, 1500, 3, 4, 2, 120)])
+def test_against_the_definition(b, sq, sk, h, hk, d, causal, dtype):
+    check(*inputs(b, sq, sk, h, hk, d, dtype, seed=sq * 7 + sk), causal=causal)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("s,lengths", [(130, [130, 0, 1, 129]), (513, [512, 128, 127, 300]), (64, [64, 63, 100, -5])])
+def test_key_lengths(s, lengths, causal):
+    """Lengths that end inside and at tiles; none; values beyond the ends count as the nearer end."""
+    q, k, v, dout = inputs(4, s, s, 4, 2, 64, BF16, seed=s)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    got = check(q, k, v, dout, causal, lens)
+    for i, n in enumerate(lengths):
+        n = min(max(n, 0), s)
+        assert not got[3][i, n:].any() and not got[4][i, n:].any()
+        if n == 0:
+            assert not got[0][i].any() and not got[2][i].any() and (got[1][i] == -math.inf).all()
+
+
+@gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("d", [64, 128])
+def test_what_lies_behind_a_length_has_no_influence(bad, d):
+    q, k, v, dout = inputs(3, 200, 300, 4, 2, d, BF16, seed=3)
+    lens = torch.tensor([300, 150, 0], dtype=torch.int32, device="cuda")
+    clean = [t.clone() for t in check(q, k, v, dout, False, lens)]
+    for i, n in enumerate(lens.tolist()):
+        k[i, n:], v[i, n:] = bad, bad
+    for a, b in zip(clean, check(q, k, v, dout, False, lens)):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_nan_of_a_query_stays_in_its_row():
+    q, k, v, dout = inputs(1, 200, 200, 2, 2, 64, BF16, seed=4)
+    want = ops.attention_forward(q, k, v)[0]
+    q[0, 77, 1] = math.nan
+    got = ops.attention_forward(q, k, v)[0]
+    assert got[0, 77, 1].isnan().all()
+    got[0, 77, 1] = want[0, 77, 1]
+    assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("factor", [1e-3, 30.0])
+def test_flat_and_peaked_rows(factor):
+    """Scores of almost one size, and scores of hundreds whose exponentials span the range."""
+    q, k, v, dout = inputs(1, 300, 300, 2, 1, 64, BF16, seed=5)
+    check((q * factor).to(BF16), k, v, dout, True)
+
+
+@gpu
+def test_scores_that_fall_and_rise_along_the_keys():
+    """The running maximum changes in every tile, or never after the first."""
+    q, k, v, dout = inputs(1, 64, 1024, 1, 1, 64, BF16, seed=6)
+    q[..., 0] = 8.0
+    ramp = torch.linspace(-16, 16, 1024, device="cuda")
+    for sign in (1, -1):
+        k[0, :, 0, 0] = (sign * ramp).to(BF16)
+        check(q, k, v, dout)
+
+
+@gpu
+def test_scale():
+    q, k, v, dout = inputs(1, 150, 150, 2, 1, 64, F16, seed=7)
+    check(q, k, v, dout, True, scale=0.31)
+
+
+@gpu
+def test_views_and_copies():
+    """Heads first, a fused projection, odd offsets that have to be copied, a broadcast batch: the same bits."""
+    q, k, v, dout = inputs(2, 150, 150, 4, 2, 64, BF16, seed=8)
+    want = check(q, k, v, dout, True)
+    fused = torch.cat((q, k, v), 2)
+    odd = torch.empty(q.numel() + 1, dtype=BF16, device="cuda")[1:].view(q.shape).copy_(q)
+    wide = torch.empty(2, 150, 4, 65, dtype=BF16, device="cuda")[..., :64].copy_(q)
+    every_second = torch.empty(2, 150, 4, 128, dtype=BF16, device="cuda")[..., ::2].copy_(q)
+    first = q.transpose(1, 2).contiguous().transpose(1, 2)
+    for q2, (k2, v2) in [(x, (k, v)) for x in (odd, wide, every_second, first)] + [(fused[:, :, :4], (fused[:, :, 4:6], fused[:, :, 6:]))]:
+        out, lse = ops.attention_forward(q2, k2, v2, causal=True)
+        grads = ops.attention_backward(dout.transpose(1, 2).contiguous().transpose(1, 2), q2, k2, v2, out, lse, causal=True)
+        assert all(torch.equal(a, b) for a, b in zip(want, (out, lse, *grads)))
+    one = k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1)
+    check(q, *one, dout, True)
+
+
+@gpu
+def test_same_bits_every_time():
+    q, k, v, dout = inputs(2, 700, 700, 8, 2, 64, BF16, seed=9)
+    first = check(q, k, v, dout, True)
+    out, lse = ops.attention_forward(q, k, v, causal=True)
+    for _ in range(5):
+        again = (*ops.attention_forward(q, k, v, causal=True), *ops.attention_backward(dout, q, k, v, out, lse, causal=True))
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@gpu
+def test_autograd_and_differences():
+    """Gradients through autograd are the backward call's, and agree with central differences of the definition."""
+    q, k, v, dout = inputs(1, 70, 70, 4, 2, 64, BF16, seed=10)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*leaves, causal=True)
+    got = torch.autograd.grad(out, leaves, dout)
+    raw = ops.attention_forward(q, k, v, causal=True)
+    assert torch.equal(out, raw[0])
+    assert all(torch.equal(a, b) for a, b in zip(got, ops.attention_backward(dout, q, k, v, *raw, causal=True)))
+    want = oracle.attention(q, k, v, dout, True)
+    step = 2.0 ** -12
+    for n, (name, grad) in enumerate(zip(("dq", "dk", "dv"), got)):
+        way = torch.randn(grad.shape, device="cuda", dtype=torch.float64, generator=torch.Generator("cuda").manual_seed(n))
+
+        def value(t):
+            x = [q.double(), k.double(), v.double()]
+            x[n] = x[n] + t * way
+            x = [y.transpose(1, 2) for y in x]
+            x[1:] = [y.repeat_interleave(2, 1) for y in x[1:]]
+            s = (x[0] @ x[1].mT * 64 ** -0.5).masked_fill(~oracle.visible(1, 70, 70, True, None).cuda(), -torch.inf)
+            return ((s.softmax(-1) @ x[2]).transpose(1, 2) * dout.double()).sum()
+
+        diff = (value(step) - value(-step)) / (2 * step)
+        # the difference's own error: a third derivative times step^2 / 6, below 2^-24 of the sum of magnitudes times a hundred
+        room = (want[name][1] * way.abs()).sum() + 100 * step ** 2 * (grad.double() * way).abs().sum()
+        assert abs((grad.double() * way).sum() - diff) <= room
+    with torch.no_grad():
+        assert not ops.attention(*leaves, causal=True).requires_grad
+
+
+@gpu
+def test_gradients_where_only_some_are_wanted():
+    q, k, v, dout = inputs(1, 33, 33, 2, 2, 64, BF16, seed=11)
+    v2 = v.clone().requires_grad_()
+    ops.attention(q, k, v2).backward(dout)
+    out, lse = ops.attention_forward(q, k, v)
+    assert torch.equal(v2.grad, ops.attention_backward(dout, q, k, v, out, lse)[2])
+
+
+@gpu
+@pytest.mark.parametrize("b,sq,sk", [(0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 0)])
+def test_nothing_to_do(b, sq, sk):
+    q, k, v, dout = inputs(b, sq, sk, 4, 2, 64, BF16)
+    out, lse = ops.attention_forward(q, k, v)
+    grads = ops.attention_backward(dout, q, k, v, out, lse)
+    assert not out.any() and (lse == -math.inf).all() and not any(g.any() for g in grads)
+    assert [g.shape for g in grads] == [q.shape, k.shape, v.shape]
+
+
+@gpu
+def test_on_another_stream_and_in_two_graphs():
+    """Captured calls replay on new contents of their inputs; two graphs replay at the same time."""
+    sets = [inputs(1, 260, 260, 4, 2, 64, BF16, seed=20 + i) for i in range(2)]
+    runs = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for s in sets:
+        with torch.cuda.stream(side):
+            ops.attention_backward(s[3], *s[:3], *ops.attention_forward(*s[:3], causal=True), causal=True)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out, lse = ops.attention_forward(*s[:3], causal=True)
+            runs.append((g, (out, lse, *ops.attention_backward(s[3], *s[:3], out, lse, causal=True))))
+    for s, fresh in zip(sets, [inputs(1, 260, 260, 4, 2, 64, BF16, seed=30 + i) for i in range(2)]):
+        for a, b in zip(s, fresh):
+            a.copy_(b)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(3):
+        for (g, _), st in zip(runs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for s, (_, got) in zip(sets, runs):
+        want = check(*s, causal=True)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Batches 2^31 elements and heads 2^30 elements apart in one buffer."""
+    buf = torch.empty((1 << 32) + (1 << 20), dtype=BF16, device="cuda")
+    q, k, v, dout = inputs(2, 150, 150, 2, 2, 64, BF16, seed=12)
+    far = buf.as_strided((2, 150, 2, 64), (1 << 31, 64, 1 << 30, 1))
+    want = check(q, k, v, dout, True)
+    for n in range(3):
+        far.copy_((q, k, v)[n])
+        x = [q, k, v]
+        x[n] = far
+        out, lse = ops.attention_forward(*x, causal=True)
+        assert all(torch.equal(a, b) for a, b in zip(want, (out, lse, *ops.attention_backward(dout, *x, out, lse, causal=True))))
+
+
+def test_refusals():
+    q, k, v, dout = inputs(2, 5, 7, 4, 2, 64, BF16, device="cpu")
+    bad = [
+        (ValueError, lambda: ops.attention(q[0], k, v)),
+        (TypeError, lambda: ops.attention(q.float(), k, v)),
+        (TypeError, lambda: ops.attention(q, k.half(), v)),
+        (TypeError, lambda: ops.attention(q.float(), k.float(), v.float())),
+        (ValueError, lambda: ops.attention(q, k, v[:, :6])),
+        (ValueError, lambda: ops.attention(q, k[:1], v[:1])),
+        (ValueError, lambda: ops.attention(q[:, :, :3], k, v)),
+        (ValueError, lambda: ops.attention(q, k[:, :, :0], v[:, :, :0])),
+        (ValueError, lambda: ops.attention(q[..., :60], k[..., :60], v[..., :60])),
+        (ValueError, lambda: ops.attention(*(torch.zeros(1, 2, 2, 136, dtype=BF16),) * 3)),
+        (ValueError, lambda: ops.attention(q, k, v, scale=0.0)),
+        (ValueError, lambda: ops.attention(q, k, v, scale=math.nan)),
+        (ValueError, lambda: ops.attention(q, k, v, scale=-1.0)),
+        (TypeError, lambda: ops.attention(q, k, v, key_lengths=torch.ones(2, dtype=torch.int64))),
+        (ValueError, lambda: ops.attention(q, k, v, key_lengths=torch.ones(3, dtype=torch.int32))),
+        (ValueError, lambda: ops.attention(q, k, v)),  # not on a GPU
+    ]
+    lse = torch.zeros(2, 4, 5)
+    bad += [
+        (ValueError, lambda: ops.attention_backward(dout[:, :4], q, k, v, q, lse)),
+        (TypeError, lambda: ops.attention_backward(dout.float(), q, k, v, q, lse)),
+        (ValueError, lambda: ops.attention_backward(dout, q, k, v, q, lse[:, :2])),
+        (TypeError, lambda: ops.attention_backward(dout, q, k, v, q, lse.double())),
+        (ValueError, lambda: ops.attention_backward(dout, q, k, v, q, lse)),
+    ]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
+
+
+def test_the_c_entry_refuses():
+    """What the Python checks keep out is an error code of the C entry too, before it touches the device."""
+    import ctypes
+    from nccl_plugin_gpudirecttcpx_b200.ops import train as T
+    lib = T._t()
+    assert lib.tcpxb_attention_forward(None, None) == -1
+
+    def args(**kw):
+        a = T._Attention(b=1, sq=4, sk=4, heads=4, kv_heads=2, d=64, scale=0.1, dtype=1, out=4096, lse=4096)
+        for n in ("q", "k", "v"):
+            setattr(a, n, T._Heads(4096, 1024, 256, 64))
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return ctypes.byref(a)
+
+    for kw in ({"b": -1}, {"kv_heads": 3}, {"kv_heads": 0}, {"d": 60}, {"d": 136}, {"d": 0}, {"dtype": 2}, {"scale": 0.0}, {"scale": math.nan},
+               {"out": 0}, {"q": T._Heads(4098, 1024, 256, 64)}, {"k": T._Heads(4096, 1024, 257, 64)}, {"v": T._Heads(0, 0, 0, 0)}):
+        assert lib.tcpxb_attention_forward(args(**kw), None) == -1, kw
+        assert lib.tcpxb_train_last_error()
+    assert lib.tcpxb_attention_backward(args(), None) == -1
