@@ -29,7 +29,7 @@ typedef enum tcpxbTrainError {
 const char* tcpxb_train_last_error(void);
 
 // A [batch, tokens, heads, head size] tensor: head elements contiguous, the other strides in
-// elements and multiples of 16 bytes, base on a 16-byte boundary.
+// elements and multiples of 16 bytes (for attention above zero), base on a 16-byte boundary.
 typedef struct tcpxbHeads {
   void* ptr;
   int64_t stride_b, stride_s, stride_h;
@@ -51,6 +51,7 @@ typedef struct tcpxbAttention {
   int32_t b, sq, sk, heads, kv_heads, d;  // d: a multiple of 8, at most 128
   float scale;            // above zero
   int32_t causal, dtype;
+  int32_t* status;        // a word on the device, or null: 3 (TCPXB_ST_TIMEOUT) where a bounded wait ran out
 } tcpxbAttention;
 
 int tcpxb_attention_forward(const tcpxbAttention* a, void* stream);

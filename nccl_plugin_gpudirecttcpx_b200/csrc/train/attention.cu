@@ -5,154 +5,731 @@
 //   D_i = dout_i . out_i          dS_ij = P_ij (dout_i . v_j - D_i)
 //   dq_i = scale sum_j dS_ij k_j  dk_j = scale sum_i dS_ij q_i   dv_j = sum_i P_ij dout_i
 //
-// The backward pass keeps no probabilities: it takes them from the scores and lse again.
-// One warp per row: lanes hold the head's elements, the softmax runs over the keys in one pass
-// with a running maximum and sum.  Every sum is taken by one warp in a fixed order.
-#include "common.h"
+// The backward pass keeps no probabilities: it takes them from the scores and lse again.  It runs
+// as two kernels, one that owns rows of dq and one that owns rows of dk and dv.  That costs seven
+// matrix products where one kernel would need five, and in return no sum is ever taken by
+// atomics: a gradient does not depend on the order in which blocks run, and no 32-bit copy of dq
+// goes through memory.
+//
+// All three kernels work on tiles of 128 x 128 scores.  One warp loads tiles with TMA, one thread
+// issues the matrix instructions, and the other eight warps turn scores into the operand of the
+// next product, in tensor memory: the score tile is read into registers (a thread has one row, or
+// half of one) and P or dS is written back over it in 16 bits.  A head size under 64 or between
+// 64 and 128 fills its panel with zeros from the load.
+//
+// Probabilities and score gradients are rounded to the inputs' type because the matrix units take
+// operands of one type; sums, statistics and everything else are 32-bit.
+#include <cstring>
+
+#include "tc.h"
 
 namespace tcpxb_train {
 namespace {
 
 constexpr int kMaxD = 128;
-constexpr int kPer = kMaxD / 32;
-constexpr int kWarps = 4;
+constexpr int kTile = 128;
+constexpr int kComputeWarps = 8, kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 320;
+constexpr int kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float warpSum(float x) {
+struct Args {
+  CUtensorMap q, k, v, dout;
+  const void* out;
+  const void* doutPtr;
+  int64_t doutB, doutS, doutH;
+  void *o, *dq, *dk, *dv;
+  float *lse, *delta;
+  const int32_t* keyLengths;
+  int32_t* status;
+  int b, sq, sk, heads, kvHeads, d, causal;
+  float scale;
+};
+
+__device__ __forceinline__ int keysOf(const Args& a, int b) { return a.keyLengths ? min(max(a.keyLengths[b], 0), a.sk) : a.sk; }
+
+// Keys that query i sees, of `keys`.
+__device__ __forceinline__ int seenBy(const Args& a, int i, int keys) { return a.causal ? min(keys, max(0, i + a.sk - a.sq + 1)) : keys; }
+
+__device__ __forceinline__ int tiles(int n) { return (n + kTile - 1) / kTile; }
+
+template <int P> __device__ __forceinline__ void loadTile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int batch) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+  for (int p = 0; p < P; p++) tmaLoad(dst + p * kPanelBytes, map, bar, p * 64, row, head, batch);
 }
 
-template <class T> __device__ __forceinline__ void loadRow(const T* p, int d, float (&f)[kPer]) {
+// Rows from `first` on become zero: what lies behind a key length may hold anything, and zero
+// times NaN would reach the sums.  A warp does it between the load and the product that reads it.
+template <int P> __device__ __forceinline__ void clearRows(uint32_t tile, int first) {
+  for (int r = first * 8 + int(threadIdx.x % 32); r < kTile * 8; r += 32) {
 #pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    const int c = i * 32 + (threadIdx.x & 31);
-    f[i] = c < d ? toFloat(p[c]) : 0.f;
+    for (int p = 0; p < P; p++)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + p * kPanelBytes + r * 16), "r"(0) : "memory");
   }
+  fenceAsyncShared();
+  __syncwarp();
 }
-template <class T> __device__ __forceinline__ void storeRow(T* p, int d, const float (&f)[kPer], float by) {
-#pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    const int c = i * 32 + (threadIdx.x & 31);
-    if (c < d) p[c] = fromFloat<T>(f[i] * by);
+
+struct Shared {
+  uint64_t bars[32];
+  uint32_t tmem;
+  int dead;
+  float stats[4][2][kTile];  // lse and D of a stage's queries
+};
+constexpr int kSharedBytes = 6144;
+static_assert(sizeof(Shared) <= kSharedBytes, "barriers and statistics");
+
+__device__ __forceinline__ void finish(const Args& a, uint32_t tmem, volatile int* dead) {
+  tcBefore();
+  __syncthreads();
+  if (*dead) {
+    // copies and products that nobody waited for may still be under way
+    const uint64_t began = nowNs();
+    while (nowNs() - began < 1000000) __nanosleep(1000);
+    if (threadIdx.x == 0 && a.status) atomicMax(a.status, kStatusTimeout);
   }
-}
-__device__ __forceinline__ float dot(const float (&a)[kPer], const float (&b)[kPer]) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; i++) s += a[i] * b[i];
-  return warpSum(s);
+  if (threadIdx.x / 32 == kMmaWarp) tmemFree(tmem, kTmemCols);
 }
 
-template <class T> __device__ __forceinline__ const T* row(const tcpxbHeads& x, int b, int s, int h) {
-  return static_cast<const T*>(x.ptr) + b * x.stride_b + s * x.stride_s + h * x.stride_h;
-}
-__device__ __forceinline__ int keysOf(const tcpxbAttention& a, int b) {
-  return a.key_lengths ? min(max(a.key_lengths[b], 0), a.sk) : a.sk;
-}
-
-template <class T> __global__ void forwardKernel(const tcpxbAttention a) {
-  const long long r = (long long)blockIdx.x * kWarps + threadIdx.x / 32;
-  if (r >= (long long)a.b * a.heads * a.sq) return;
-  const int i = int(r % a.sq), h = int(r / a.sq % a.heads), b = int(r / a.sq / a.heads), kv = h / (a.heads / a.kv_heads);
-  int keys = keysOf(a, b);
-  if (a.causal) keys = min(keys, i + a.sk - a.sq + 1);
-  float q[kPer], o[kPer] = {}, x[kPer];
-  loadRow(row<T>(a.q, b, i, h), a.d, q);
-  float top = -INFINITY, sum = 0.f;
-  for (int j = 0; j < keys; j++) {
-    loadRow(row<T>(a.k, b, j, kv), a.d, x);
-    const float s = dot(q, x) * a.scale;
-    const float next = fmaxf(top, s), keep = expf(top - next), p = expf(s - next);
-    top = next;
-    sum = sum * keep + p;
-    loadRow(row<T>(a.v, b, j, kv), a.d, x);
-#pragma unroll
-    for (int c = 0; c < kPer; c++) o[c] = o[c] * keep + p * x[c];
+// Eight 32-bit values as one 16-byte store; by zero they are zeros, whatever they were.
+template <class T> __device__ __forceinline__ void storeRow8(T* p, const uint32_t* r, float by) {
+  uint4 x = {};
+  if (by != 0.f) {
+    x.x = pack2<T>(__uint_as_float(r[0]) * by, __uint_as_float(r[1]) * by);
+    x.y = pack2<T>(__uint_as_float(r[2]) * by, __uint_as_float(r[3]) * by);
+    x.z = pack2<T>(__uint_as_float(r[4]) * by, __uint_as_float(r[5]) * by);
+    x.w = pack2<T>(__uint_as_float(r[6]) * by, __uint_as_float(r[7]) * by);
   }
-  storeRow(static_cast<T*>(a.out) + (((long long)b * a.sq + i) * a.heads + h) * a.d, a.d, o, keys > 0 ? 1.f / sum : 0.f);
-  if ((threadIdx.x & 31) == 0) a.lse[((long long)b * a.heads + h) * a.sq + i] = keys > 0 ? top + logf(sum) : -INFINITY;
+  *reinterpret_cast<uint4*>(p) = x;
 }
-
-// dq of one row, and D for the other kernel.
-template <class T> __global__ void backwardQueryKernel(const tcpxbAttention a) {
-  const long long r = (long long)blockIdx.x * kWarps + threadIdx.x / 32;
-  if (r >= (long long)a.b * a.heads * a.sq) return;
-  const int i = int(r % a.sq), h = int(r / a.sq % a.heads), b = int(r / a.sq / a.heads), kv = h / (a.heads / a.kv_heads);
-  int keys = keysOf(a, b);
-  if (a.causal) keys = min(keys, i + a.sk - a.sq + 1);
-  const long long at = (((long long)b * a.sq + i) * a.heads + h) * a.d;
-  float q[kPer], go[kPer], dq[kPer] = {}, x[kPer];
-  loadRow(row<T>(a.q, b, i, h), a.d, q);
-  loadRow(row<T>(a.dout, b, i, h), a.d, go);
-  loadRow(static_cast<const T*>(a.out) + at, a.d, x);
-  const long long stat = ((long long)b * a.heads + h) * a.sq + i;
-  const float lse = a.lse[stat], delta = dot(go, x);
-  if ((threadIdx.x & 31) == 0) a.delta[stat] = delta;
-  for (int j = 0; j < keys; j++) {
-    loadRow(row<T>(a.v, b, j, kv), a.d, x);
-    const float dp = dot(go, x);
-    loadRow(row<T>(a.k, b, j, kv), a.d, x);
-    const float ds = expf(dot(q, x) * a.scale - lse) * (dp - delta);
-#pragma unroll
-    for (int c = 0; c < kPer; c++) dq[c] += ds * x[c];
-  }
-  storeRow(static_cast<T*>(a.dq) + at, a.d, dq, a.scale);
-}
-
-// dk and dv of one key, over all query heads of its group.
-template <class T> __global__ void backwardKeyKernel(const tcpxbAttention a) {
-  const long long r = (long long)blockIdx.x * kWarps + threadIdx.x / 32;
-  if (r >= (long long)a.b * a.kv_heads * a.sk) return;
-  const int j = int(r % a.sk), kv = int(r / a.sk % a.kv_heads), b = int(r / a.sk / a.kv_heads), group = a.heads / a.kv_heads;
-  float k[kPer], v[kPer], dk[kPer] = {}, dv[kPer] = {}, x[kPer], go[kPer];
-  loadRow(row<T>(a.k, b, j, kv), a.d, k);
-  loadRow(row<T>(a.v, b, j, kv), a.d, v);
-  const int first = a.causal ? max(0, j - (a.sk - a.sq)) : 0;
-  for (int h = kv * group; h < (kv + 1) * group && j < keysOf(a, b); h++) {
-    for (int i = first; i < a.sq; i++) {
-      loadRow(row<T>(a.q, b, i, h), a.d, x);
-      loadRow(row<T>(a.dout, b, i, h), a.d, go);
-      const long long stat = ((long long)b * a.heads + h) * a.sq + i;
-      const float p = expf(dot(x, k) * a.scale - a.lse[stat]), ds = p * (dot(go, v) - a.delta[stat]);
-#pragma unroll
-      for (int c = 0; c < kPer; c++) dk[c] += ds * x[c], dv[c] += p * go[c];
+// Columns [begin, end) of the thread's accumulator row, times `by`; all threads of the warp come here.
+template <class T> __device__ __forceinline__ void storeRow(T* row, bool live, uint32_t tmem, int begin, int end, int d, float by, bool any) {
+  for (int c = begin; c < end && c < d; c += 32) {
+    uint32_t r[32] = {};
+    if (any) {
+      tmemLoad32(tmem + c, r);
+      tmemWaitLoad();
     }
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+      if (live && c + i < d) storeRow8(row + c + i, r + i, by);
   }
-  const long long at = (((long long)b * a.sk + j) * a.kv_heads + kv) * a.d;
-  storeRow(static_cast<T*>(a.dk) + at, a.d, dk, a.scale);
-  storeRow(static_cast<T*>(a.dv) + at, a.d, dv, 1.f);
+}
+
+// ------------------------------------------------------------------ forward
+// A block owns two tiles of queries; four warps do the softmax of each.  While one tile's scores
+// are turned into probabilities, the matrix units work for the other one: out += P V of the
+// last key tile, then the scores of the next.  A thread holds a whole row, so maximum and sum
+// need no exchange.  The accumulator is rescaled only where a row's maximum has grown by more
+// than 2^8 since its last rescaling: probabilities then reach 2^8, which costs no precision.
+template <class T, int P> struct Forward {
+  static constexpr int kSlots = P == 2 ? 4 : 8;  // tiles of keys and values in turn
+  static constexpr uint32_t kTileBytes = P * kPanelBytes;
+  static constexpr size_t kShared = kSharedBytes + 1024 + (2 + kSlots) * kTileBytes;
+  enum { kQFull = 0, kFull = 2, kEmpty = kFull + kSlots, kSFull = kEmpty + kSlots, kPFull = kSFull + 2, kOFull = kPFull + 2, kBars = kOFull + 2 };
+};
+
+template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forwardKernel(const __grid_constant__ Args a) {
+  using F = Forward<T, P>;
+  static_assert(F::kBars <= 32, "barriers");
+  extern __shared__ char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  const uint32_t tile0 = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, ring = tile0 + 2 * F::kTileBytes;
+  const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
+  volatile int* dead = &sh.dead;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // long rows first: with a causal mask the last queries see the most keys
+  const int q0 = (int(gridDim.x) - 1 - int(blockIdx.x)) * 2 * kTile, h = blockIdx.y, b = blockIdx.z, kv = h / (a.heads / a.kvHeads);
+  const int keys = keysOf(a, b);
+  int n[2];
+#pragma unroll
+  for (int t = 0; t < 2; t++) n[t] = q0 + t * kTile < a.sq ? tiles(seenBy(a, min(q0 + t * kTile + kTile, a.sq) - 1, keys)) : 0;
+  const int most = max(n[0], n[1]);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < F::kBars; i++) barInit(bar(i), i >= F::kPFull && i < F::kOFull ? 4 : 1);
+    sh.dead = 0;
+    fenceBarInit();
+  }
+  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), kTmemCols);
+  tcBefore();
+  __syncthreads();
+  tcAfter();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      for (int t = 0; t < 2; t++)
+        if (n[t]) {
+          barExpect(bar(F::kQFull + t), F::kTileBytes);
+          loadTile<P>(tile0 + t * F::kTileBytes, &a.q, bar(F::kQFull + t), q0 + t * kTile, h, b);
+        }
+      for (int i = 0; i < 2 * most; i++) {
+        const int slot = i % F::kSlots, turn = i / F::kSlots;
+        if (turn) barWait(bar(F::kEmpty + slot), (turn - 1) & 1, dead);
+        barExpect(bar(F::kFull + slot), F::kTileBytes);
+        loadTile<P>(ring + slot * F::kTileBytes, i & 1 ? &a.v : &a.k, bar(F::kFull + slot), i / 2 * kTile, kv, b);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    const int steps = (a.d + 15) / 16;
+    const uint32_t scores = mmaShape<T>(kTile, false), values = mmaShape<T>(steps * 16, true);
+    for (int j = 0; j <= most; j++) {
+      const int ik = 2 * j, iv = 2 * j - 1;  // numbers of K_j and V_j-1
+      const uint32_t kTileAt = ring + ik % F::kSlots * F::kTileBytes, vTileAt = ring + (iv + F::kSlots) % F::kSlots * F::kTileBytes;
+      if (j < most) barWait(bar(F::kFull + ik % F::kSlots), ik / F::kSlots & 1, dead);
+      if (j) {
+        barWait(bar(F::kFull + iv % F::kSlots), iv / F::kSlots & 1, dead);
+        if (j * kTile > keys && keys < a.sk) clearRows<P>(vTileAt, keys - (j - 1) * kTile);
+      }
+      for (int t = 0; t < 2; t++) {
+        const uint32_t s = tmem + t * kTile, o = tmem + 2 * kTile + t * kMaxD;
+        if (j && j <= n[t]) {
+          barWait(bar(F::kPFull + t), (j - 1) & 1, dead);
+          tcAfter();
+          if (lane == 0) {
+            for (int k = 0; k < kTile / 16; k++) mmaFromTmem(o, s + k * 8, acrossRows(vTileAt, k), values, j > 1 || k);
+            if (j == n[t]) mmaCommit(bar(F::kOFull + t));
+          }
+        }
+        if (j < n[t]) {
+          if (j == 0) barWait(bar(F::kQFull + t), 0, dead);
+          if (lane == 0) {
+            // in issue order behind the product that reads P out of the same columns
+            for (int k = 0; k < steps; k++) mma(s, alongRow(tile0 + t * F::kTileBytes, k), alongRow(kTileAt, k), scores, k);
+            mmaCommit(bar(F::kSFull + t));
+          }
+        }
+      }
+      if (lane == 0) {
+        // only where a load waits for it: no arrival may come after the block has gone
+        if (ik + F::kSlots < 2 * most) mmaCommit(bar(F::kEmpty + ik % F::kSlots));
+        if (j && iv + F::kSlots < 2 * most) mmaCommit(bar(F::kEmpty + iv % F::kSlots));
+      }
+      __syncwarp();
+    }
+  } else {
+    const int t = warp / 4, row = warp % 4 * 32 + lane, i = q0 + t * kTile + row;
+    const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
+    const uint32_t s = tmem + t * kTile + lanes, o = tmem + 2 * kTile + t * kMaxD + lanes;
+    const float c = a.scale * kLog2e;
+    const int seen = seenBy(a, i, keys);                       // of this row
+    const int whole = seenBy(a, q0 + t * kTile, keys) / kTile;  // tiles that every row sees whole
+    float top = -INFINITY;
+    float2 sum2 = {0.f, 0.f};
+    for (int j = 0; j < n[t]; j++) {
+      barWait(bar(F::kSFull + t), j & 1, dead);
+      tcAfter();
+      uint32_t x[kTile];
+#pragma unroll
+      for (int k = 0; k < kTile; k += 32) tmemLoad32(s + k, x + k);
+      tmemWaitLoad();
+      if (j >= whole) {
+        const int left = seen - j * kTile;
+#pragma unroll
+        for (int k = 0; k < kTile; k++) x[k] = k < left ? x[k] : 0xff800000u;
+      }
+      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int k = 0; k < kTile; k += 8)
+#pragma unroll
+        for (int u = 0; u < 4; u++) m[u] = fmaxf(m[u], fmaxf(__uint_as_float(x[k + u]), __uint_as_float(x[k + 4 + u])));
+      const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      const bool grown = (now - top) * c > 8.f || (top == -INFINITY && now > -INFINITY);
+      if (__any_sync(0xffffffffu, grown)) {
+        const float keep = grown ? exp2Fast((top - now) * c) : 1.f;
+        if (grown) top = now;
+        sum2 = mul2(sum2, {keep, keep});
+        if (j) {
+          for (int k = 0; k < (a.d + 31) / 32 * 32; k += 32) {
+            uint32_t r[32];
+            tmemLoad32(o + k, r);
+            tmemWaitLoad();
+#pragma unroll
+            for (int u = 0; u < 32; u++) r[u] = __float_as_uint(__uint_as_float(r[u]) * keep);
+            tmemStore32(o + k, r);
+          }
+        }
+      }
+      const float base = top == -INFINITY ? 0.f : -top * c;
+#pragma unroll
+      for (int k = 0; k < kTile; k += 64) {
+        uint32_t p[32];
+#pragma unroll
+        for (int u = 0; u < 64; u += 2) {
+          float2 e = fma2({__uint_as_float(x[k + u]), __uint_as_float(x[k + u + 1])}, {c, c}, {base, base});
+          e.x = exp2Fast(e.x), e.y = exp2Fast(e.y);
+          sum2 = add2(sum2, e);
+          p[u / 2] = pack2<T>(e.x, e.y);
+        }
+        tmemStore32(s + k / 2, p);
+      }
+      tmemWaitStore();
+      tcBefore();
+      __syncwarp();
+      if (lane == 0) barArrive(bar(F::kPFull + t));
+    }
+    if (n[t]) {
+      barWait(bar(F::kOFull + t), 0, dead);
+      tcAfter();
+    }
+    const float sum = sum2.x + sum2.y;
+    const bool live = i < a.sq;
+    const long long at = (((long long)b * a.sq + i) * a.heads + h) * a.d;
+    // a row that sees nothing is zero, whatever its tile holds
+    const float by = seen > 0 ? 1.f / sum : 0.f;
+    if (q0 + t * kTile < a.sq) storeRow(static_cast<T*>(a.o) + at, live, o, 0, kMaxD, a.d, by, n[t] > 0);
+    if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
+  }
+  finish(a, tmem, dead);
+}
+
+// ------------------------------------------------------------------ backward, queries
+// A block owns 128 queries and goes through the key tiles:  S = Q K^T, dP = dout V^T, then
+// dq += dS K.  Two buffers of scores: the next tile's exponentials start while the matrix units
+// still work on dP and dq of this one.  Both halves of the warps hold all rows, 64 keys each.
+// D_i is computed here, on the way in, and left for the other kernel.
+template <class T, int P> struct Queries {
+  static constexpr int kKSlots = 3, kVSlots = 2;
+  static constexpr uint32_t kTileBytes = P * kPanelBytes;
+  static constexpr size_t kShared = 1024 + 1024 + (2 + kKSlots + kVSlots) * kTileBytes;
+  enum { kQFull = 0, kKFull = 1, kVFull = kKFull + kKSlots, kKEmpty = kVFull + kVSlots, kVEmpty = kKEmpty + kKSlots, kSFull = kVEmpty + kVSlots,
+         kDpFull = kSFull + 2, kDsFull, kDone, kBars };
+};
+
+// A score that the row or key does not count for leaves exactly zero.
+template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKernel(const __grid_constant__ Args a) {
+  using F = Queries<T, P>;
+  static_assert(F::kBars <= 32, "barriers");
+  extern __shared__ char raw[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(raw);
+  uint32_t* tmemAt = reinterpret_cast<uint32_t*>(raw + 256);
+  volatile int* dead = reinterpret_cast<int*>(raw + 264);
+  float* deltas = reinterpret_cast<float*>(raw + 512);
+  const uint32_t tile0 = (smemAddr(raw) + 1024 + 1023) / 1024 * 1024, qTile = tile0, doTile = tile0 + F::kTileBytes, kRing = tile0 + 2 * F::kTileBytes,
+                 vRing = kRing + F::kKSlots * F::kTileBytes;
+  const auto bar = [&](int i) { return smemAddr(bars) + 8 * i; };
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int q0 = (int(gridDim.x) - 1 - int(blockIdx.x)) * kTile, h = blockIdx.y, b = blockIdx.z, kv = h / (a.heads / a.kvHeads);
+  const int keys = keysOf(a, b), n = tiles(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < F::kBars; i++) barInit(bar(i), i == F::kDsFull ? kComputeWarps : 1);
+    *dead = 0;
+    fenceBarInit();
+  }
+  if (warp == kMmaWarp) tmemAlloc(smemAddr(tmemAt), kTmemCols);
+  tcBefore();
+  __syncthreads();
+  tcAfter();
+  const uint32_t tmem = *tmemAt, dp = tmem + 2 * kTile, dq = tmem + 3 * kTile;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0 && n) {
+      barExpect(bar(F::kQFull), 2 * F::kTileBytes);
+      loadTile<P>(qTile, &a.q, bar(F::kQFull), q0, h, b);
+      loadTile<P>(doTile, &a.dout, bar(F::kQFull), q0, h, b);
+      for (int j = 0; j < n; j++) {
+        const int ks = j % F::kKSlots, vs = j % F::kVSlots;
+        if (j >= F::kKSlots) barWait(bar(F::kKEmpty + ks), (j / F::kKSlots - 1) & 1, dead);
+        barExpect(bar(F::kKFull + ks), F::kTileBytes);
+        loadTile<P>(kRing + ks * F::kTileBytes, &a.k, bar(F::kKFull + ks), j * kTile, kv, b);
+        if (j >= F::kVSlots) barWait(bar(F::kVEmpty + vs), (j / F::kVSlots - 1) & 1, dead);
+        barExpect(bar(F::kVFull + vs), F::kTileBytes);
+        loadTile<P>(vRing + vs * F::kTileBytes, &a.v, bar(F::kVFull + vs), j * kTile, kv, b);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    const int steps = (a.d + 15) / 16;
+    const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
+    const auto score = [&](int j) {  // S of key tile j
+      const int ks = j % F::kKSlots;
+      const uint32_t kTileAt = kRing + ks * F::kTileBytes;
+      barWait(bar(F::kKFull + ks), j / F::kKSlots & 1, dead);
+      if ((j + 1) * kTile > keys && keys < a.sk) clearRows<P>(kTileAt, keys - j * kTile);
+      if (lane == 0) {
+        for (int k = 0; k < steps; k++) mma(tmem + (j & 1) * kTile, alongRow(qTile, k), alongRow(kTileAt, k), scores, k);
+        mmaCommit(bar(F::kSFull + (j & 1)));
+      }
+    };
+    const auto gradient = [&](int j) {  // dP of key tile j
+      const int vs = j % F::kVSlots;
+      barWait(bar(F::kVFull + vs), j / F::kVSlots & 1, dead);
+      if (lane == 0) {
+        for (int k = 0; k < steps; k++) mma(dp, alongRow(doTile, k), alongRow(vRing + vs * F::kTileBytes, k), scores, k);
+        mmaCommit(bar(F::kDpFull));
+        if (j + F::kVSlots < n) mmaCommit(bar(F::kVEmpty + vs));
+      }
+    };
+    if (n) {
+      barWait(bar(F::kQFull), 0, dead);
+      score(0);
+      gradient(0);
+      if (n > 1) score(1);
+      for (int j = 0; j < n; j++) {
+        barWait(bar(F::kDsFull), j & 1, dead);
+        tcAfter();
+        if (j + 1 < n) gradient(j + 1);
+        if (lane == 0) {
+          const int ks = j % F::kKSlots;
+          const uint32_t ds = tmem + (j & 1) * kTile;
+          for (int k = 0; k < kTile / 16; k++)
+            mmaFromTmem(dq, ds + k / 4 * 64 + k % 4 * 8, acrossRows(kRing + ks * F::kTileBytes, k), back, j || k);
+          if (j + F::kKSlots < n) mmaCommit(bar(F::kKEmpty + ks));
+          if (j == n - 1) mmaCommit(bar(F::kDone));
+        }
+        if (j + 2 < n) score(j + 2);
+        __syncwarp();
+      }
+    }
+  } else {
+    const int half = warp / 4, row = warp % 4 * 32 + lane, i = q0 + row;
+    const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
+    const bool live = i < a.sq;
+    const long long at = (((long long)b * a.sq + i) * a.heads + h) * a.d, stat = ((long long)b * a.heads + h) * a.sq + i;
+    const float c = a.scale * kLog2e;
+    if (half == 0) {
+      float sum = 0.f;
+      if (live) {
+        const T *o = static_cast<const T*>(a.out) + at, *g = static_cast<const T*>(a.doutPtr) + b * a.doutB + i * a.doutS + h * a.doutH;
+        for (int k = 0; k < a.d; k += 8) {
+          float x[8], y[8];
+          load8(o + k, x);
+          load8(g + k, y);
+#pragma unroll
+          for (int u = 0; u < 8; u++) sum += x[u] * y[u];
+        }
+        a.delta[stat] = sum;
+      }
+      deltas[row] = sum;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float delta = deltas[row];
+    // a row that sees nothing, or lies behind the last query, has no probabilities
+    float l = live ? a.lse[stat] * -kLog2e : -INFINITY;
+    if (l == INFINITY) l = -INFINITY;
+    const int seen = live ? seenBy(a, i, keys) : 0, whole = seenBy(a, q0, keys) / kTile;
+    for (int j = 0; j < n; j++) {
+      const uint32_t s = tmem + (j & 1) * kTile + half * 64 + lanes;
+      barWait(bar(F::kSFull + (j & 1)), j / 2 & 1, dead);
+      tcAfter();
+      uint32_t x[64];
+      tmemLoad32(s, x);
+      tmemLoad32(s + 32, x + 32);
+      tmemWaitLoad();
+#pragma unroll
+      for (int k = 0; k < 64; k += 2) {
+        const float2 e = fma2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, {c, c}, {l, l});
+        x[k] = __float_as_uint(exp2Fast(e.x)), x[k + 1] = __float_as_uint(exp2Fast(e.y));
+      }
+      barWait(bar(F::kDpFull), j & 1, dead);
+      tcAfter();
+      uint32_t y[64], ds[32];
+      tmemLoad32(dp + half * 64 + lanes, y);
+      tmemLoad32(dp + half * 64 + lanes + 32, y + 32);
+      tmemWaitLoad();
+      const bool some = j >= whole;
+      const int left = seen - j * kTile - half * 64;
+#pragma unroll
+      for (int k = 0; k < 64; k += 2) {
+        float2 g = add2({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, {-delta, -delta});
+        g = mul2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, g);
+        if (some) {
+          g.x = k < left ? g.x : 0.f;
+          g.y = k + 1 < left ? g.y : 0.f;
+        }
+        ds[k / 2] = pack2<T>(g.x, g.y);
+      }
+      tmemStore32(s, ds);
+      tmemWaitStore();
+      tcBefore();
+      __syncwarp();
+      if (lane == 0) barArrive(bar(F::kDsFull));
+    }
+    if (n) {
+      barWait(bar(F::kDone), 0, dead);
+      tcAfter();
+    }
+    storeRow(static_cast<T*>(a.dq) + at, live, dq + lanes, half * 64, half * 64 + 64, a.d, seen > 0 ? a.scale : 0.f, n > 0);
+  }
+  finish(a, tmem, dead);
+}
+
+// ------------------------------------------------------------------ backward, keys
+// A block owns 128 keys of one key head and goes through the query tiles of all query heads of
+// its group:  S^T = K Q^T, dP^T = V dout^T, then dv += P^T dout and dk += dS^T Q.  While the warps
+// make P, the matrix units do the last tile's dk and this one's dP; while they make dS, dv and
+// the next scores.
+template <class T, int P> struct Keys {
+  static constexpr int kStages = P == 2 ? 2 : 4;
+  static constexpr uint32_t kTileBytes = P * kPanelBytes;
+  static constexpr size_t kShared = kSharedBytes + 1024 + (2 + 2 * kStages) * kTileBytes;
+  enum { kKvFull = 0, kFull = 1, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kDpFull, kPFull, kDsFull, kDone, kBars };
+};
+
+template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKernel(const __grid_constant__ Args a) {
+  using F = Keys<T, P>;
+  static_assert(F::kBars <= 32 && F::kStages <= 4, "barriers");
+  extern __shared__ char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  const uint32_t kTileAt = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, vTileAt = kTileAt + F::kTileBytes, ring = vTileAt + F::kTileBytes;
+  const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
+  volatile int* dead = &sh.dead;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int j0 = blockIdx.x * kTile, kv = blockIdx.y, b = blockIdx.z, group = a.heads / a.kvHeads;
+  const int keys = keysOf(a, b);
+  const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kTile : 0;  // first query tile that sees a key of this one
+  const int each = j0 < keys ? max(0, tiles(a.sq) - first) : 0, n = each * group;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < F::kBars; i++)
+      barInit(bar(i), i == F::kPFull || i == F::kDsFull ? kComputeWarps : i >= F::kFull && i < F::kEmpty ? 33 : 1);
+    sh.dead = 0;
+    fenceBarInit();
+  }
+  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), kTmemCols);
+  tcBefore();
+  __syncthreads();
+  tcAfter();
+  const uint32_t tmem = sh.tmem, s = tmem, dp = tmem + kTile, dv = tmem + 2 * kTile, dk = tmem + 3 * kTile;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0 && n) {
+      barExpect(bar(F::kKvFull), 2 * F::kTileBytes);
+      loadTile<P>(kTileAt, &a.k, bar(F::kKvFull), j0, kv, b);
+      loadTile<P>(vTileAt, &a.v, bar(F::kKvFull), j0, kv, b);
+    }
+    for (int it = 0; it < n; it++) {
+      const int st = it % F::kStages, turn = it / F::kStages, h = kv * group + it / each, q0 = (first + it % each) * kTile;
+      const long long stat = ((long long)b * a.heads + h) * a.sq;
+      float l[4], d[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int i = q0 + u * 32 + lane;
+        l[u] = i < a.sq ? a.lse[stat + i] * -kLog2e : -INFINITY;
+        if (l[u] == INFINITY) l[u] = -INFINITY;
+        d[u] = i < a.sq ? -a.delta[stat + i] : 0.f;
+      }
+      if (turn) barWait(bar(F::kEmpty + st), (turn - 1) & 1, dead);
+      if (lane == 0) {
+        const uint32_t q = ring + 2 * st * F::kTileBytes;
+        barExpect(bar(F::kFull + st), 2 * F::kTileBytes);
+        loadTile<P>(q, &a.q, bar(F::kFull + st), q0, h, b);
+        loadTile<P>(q + F::kTileBytes, &a.dout, bar(F::kFull + st), q0, h, b);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) sh.stats[st][0][u * 32 + lane] = l[u], sh.stats[st][1][u * 32 + lane] = d[u];
+      barArrive(bar(F::kFull + st));
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    const int steps = (a.d + 15) / 16;
+    const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
+    if (n) {
+      barWait(bar(F::kKvFull), 0, dead);
+      for (int it = -1; it < n; it++) {
+        const int st = (it + F::kStages) % F::kStages, next = (it + 1) % F::kStages;
+        const uint32_t q = ring + 2 * st * F::kTileBytes, qn = ring + 2 * next * F::kTileBytes;
+        if (it >= 0) {
+          barWait(bar(F::kPFull), it & 1, dead);
+          tcAfter();
+          if (lane == 0)
+            for (int k = 0; k < kTile / 16; k++)
+              mmaFromTmem(dv, s + k / 4 * 64 + k % 4 * 8, acrossRows(q + F::kTileBytes, k), back, it || k);
+        }
+        if (it + 1 < n) {
+          barWait(bar(F::kFull + next), (it + 1) / F::kStages & 1, dead);
+          if (lane == 0) {
+            for (int k = 0; k < steps; k++) mma(s, alongRow(kTileAt, k), alongRow(qn, k), scores, k);
+            mmaCommit(bar(F::kSFull));
+          }
+        }
+        if (it >= 0) {
+          barWait(bar(F::kDsFull), it & 1, dead);
+          tcAfter();
+          if (lane == 0) {
+            for (int k = 0; k < kTile / 16; k++) mmaFromTmem(dk, dp + k / 4 * 64 + k % 4 * 8, acrossRows(q, k), back, it || k);
+            if (it + F::kStages < n) mmaCommit(bar(F::kEmpty + st));
+            if (it == n - 1) mmaCommit(bar(F::kDone));
+          }
+        }
+        if (it + 1 < n && lane == 0) {
+          for (int k = 0; k < steps; k++) mma(dp, alongRow(vTileAt, k), alongRow(qn + F::kTileBytes, k), scores, k);
+          mmaCommit(bar(F::kDpFull));
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int half = warp / 4, row = warp % 4 * 32 + lane, j = j0 + row;
+    const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
+    const bool counts = j < keys;
+    const float c = a.scale * kLog2e;
+    for (int it = 0; it < n; it++) {
+      const int st = it % F::kStages, q0 = (first + it % each) * kTile;
+      const float2* l = reinterpret_cast<const float2*>(sh.stats[st][0] + half * 64);
+      const float2* d = reinterpret_cast<const float2*>(sh.stats[st][1] + half * 64);
+      // first query of this half that sees the row's key
+      const int from = !counts ? 64 : a.causal ? j - (a.sk - a.sq) - q0 - half * 64 : 0;
+      const bool some = j0 + kTile > keys || (a.causal && j0 + kTile - 1 > q0 + a.sk - a.sq);
+      barWait(bar(F::kFull + st), it / F::kStages & 1, dead);
+      barWait(bar(F::kSFull), it & 1, dead);
+      tcAfter();
+      uint32_t x[64], o[32];
+      tmemLoad32(s + half * 64 + lanes, x);
+      tmemLoad32(s + half * 64 + lanes + 32, x + 32);
+      tmemWaitLoad();
+#pragma unroll
+      for (int k = 0; k < 64; k += 2) {
+        float2 e = fma2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, {c, c}, l[k / 2]);
+        e.x = exp2Fast(e.x), e.y = exp2Fast(e.y);
+        if (some) {
+          e.x = k >= from ? e.x : 0.f;
+          e.y = k + 1 >= from ? e.y : 0.f;
+        }
+        x[k] = __float_as_uint(e.x), x[k + 1] = __float_as_uint(e.y);
+        o[k / 2] = pack2<T>(e.x, e.y);
+      }
+      tmemStore32(s + half * 64 + lanes, o);
+      tmemWaitStore();
+      tcBefore();
+      __syncwarp();
+      if (lane == 0) barArrive(bar(F::kPFull));
+
+      barWait(bar(F::kDpFull), it & 1, dead);
+      tcAfter();
+      uint32_t y[64];
+      tmemLoad32(dp + half * 64 + lanes, y);
+      tmemLoad32(dp + half * 64 + lanes + 32, y + 32);
+      tmemWaitLoad();
+#pragma unroll
+      for (int k = 0; k < 64; k += 2) {
+        float2 g = add2({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, d[k / 2]);
+        g = mul2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, g);
+        if (some) {
+          g.x = k >= from ? g.x : 0.f;
+          g.y = k + 1 >= from ? g.y : 0.f;
+        }
+        o[k / 2] = pack2<T>(g.x, g.y);
+      }
+      tmemStore32(dp + half * 64 + lanes, o);
+      tmemWaitStore();
+      tcBefore();
+      __syncwarp();
+      if (lane == 0) barArrive(bar(F::kDsFull));
+    }
+    if (n) {
+      barWait(bar(F::kDone), 0, dead);
+      tcAfter();
+    }
+    const bool live = j < a.sk;
+    const long long at = (((long long)b * a.sk + j) * a.kvHeads + kv) * a.d;
+    storeRow(static_cast<T*>(a.dv) + at, live, dv + lanes, half * 64, half * 64 + 64, a.d, counts ? 1.f : 0.f, n > 0);
+    storeRow(static_cast<T*>(a.dk) + at, live, dk + lanes, half * 64, half * 64 + 64, a.d, counts ? a.scale : 0.f, n > 0);
+  }
+  finish(a, tmem, dead);
+}
+
+// ------------------------------------------------------------------ host
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                            const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+  static const Encode f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<Encode>(p);
+  }();
+  return f;
+}
+
+int makeMap(CUtensorMap* map, const char* name, const tcpxbHeads& x, int b, int s, int heads, int d, int dtype) {
+  std::memset(map, 0, sizeof(*map));
+  if ((long long)b * s == 0) return TCPXB_T_OK;  // nothing is loaded
+  const Encode encode = encoder();
+  if (!encode) return fail(TCPXB_T_CUDA, "the driver has no tensor maps");
+  const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(s), cuuint64_t(heads), cuuint64_t(b)};
+  cuuint64_t strides[3] = {cuuint64_t(x.stride_s) * 2, cuuint64_t(x.stride_h) * 2, cuuint64_t(x.stride_b) * 2};
+  for (int i = 0; i < 3; i++)
+    if (dims[i + 1] == 1) strides[i] = 256;  // of no influence
+  const cuuint32_t box[4] = {64, kTile, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, dtype == TCPXB_T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, x.ptr, dims, strides, box,
+                            ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TCPXB_T_OK : fail(TCPXB_T_INVALID, "%s cannot be loaded in tiles (driver error %d): its strides are out of range", name, int(r));
+}
+
+bool stridesOk(const tcpxbHeads& x, int b, int s, int heads) {
+  return headsOk(x, 2) && (b == 1 || x.stride_b > 0) && (s == 1 || x.stride_s > 0) && (heads == 1 || x.stride_h > 0);
 }
 
 int check(const tcpxbAttention* a, bool backward) {
   if (!a) return fail(TCPXB_T_INVALID, "null argument");
   if (a->b < 0 || a->sq < 0 || a->sk < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->d < 8 || a->d > kMaxD || a->d % 8)
     return fail(TCPXB_T_INVALID, "bad shape: b %d sq %d sk %d heads %d/%d d %d", a->b, a->sq, a->sk, a->heads, a->kv_heads, a->d);
+  if (a->b > 65535 || a->heads > 65535 || a->sq > 1 << 30 || a->sk > 1 << 30)
+    return fail(TCPXB_T_INVALID, "at most 65535 batches and heads and 2^30 tokens: b %d heads %d sq %d sk %d", a->b, a->heads, a->sq, a->sk);
   if (a->dtype != TCPXB_T_BF16 && a->dtype != TCPXB_T_F16) return fail(TCPXB_T_INVALID, "attention takes bf16 and fp16, not type %d", a->dtype);
   if (!(a->scale > 0.f) || a->scale > 1e30f) return fail(TCPXB_T_INVALID, "scale has to be finite and above zero");
   const bool queries = (long long)a->b * a->sq > 0, keys = (long long)a->b * a->sk > 0;
-  if (queries && (!headsOk(a->q, 2) || !a->out || !a->lse)) return fail(TCPXB_T_INVALID, "q, out or lse is null or off the 16-byte boundary");
-  if (keys && (!headsOk(a->k, 2) || !headsOk(a->v, 2))) return fail(TCPXB_T_INVALID, "k or v is null or off the 16-byte boundary");
-  if (backward && ((queries && (!headsOk(a->dout, 2) || !a->dq || !a->delta)) || (keys && (!a->dk || !a->dv))))
-    return fail(TCPXB_T_INVALID, "dout, dq, dk, dv or delta is null or off the 16-byte boundary");
+  if (queries && (!stridesOk(a->q, a->b, a->sq, a->heads) || !a->out || !a->lse))
+    return fail(TCPXB_T_INVALID, "q, out or lse is null, off the 16-byte boundary or broadcast");
+  if (keys && (!stridesOk(a->k, a->b, a->sk, a->kv_heads) || !stridesOk(a->v, a->b, a->sk, a->kv_heads)))
+    return fail(TCPXB_T_INVALID, "k or v is null, off the 16-byte boundary or broadcast");
+  if (backward && ((queries && (!stridesOk(a->dout, a->b, a->sq, a->heads) || !a->dq || !a->delta)) || (keys && (!a->dk || !a->dv))))
+    return fail(TCPXB_T_INVALID, "dout, dq, dk, dv or delta is null, off the 16-byte boundary or broadcast");
   return TCPXB_T_OK;
 }
 
-template <class T> int forward(const tcpxbAttention& a, cudaStream_t s) {
-  const long long rows = (long long)a.b * a.heads * a.sq;
-  if (rows == 0) return TCPXB_T_OK;
-  forwardKernel<T><<<unsigned((rows + kWarps - 1) / kWarps), kWarps * 32, 0, s>>>(a);
-  return launched("attention forward");
+int makeArgs(const tcpxbAttention& a, bool backward, Args* x) {
+  // a thread that only autograd has used so far knows its device but has no context yet, which the driver's call needs
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaSetDevice(device);
+  if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "attention: %s", cudaGetErrorString(e));
+  int rc = makeMap(&x->q, "q", a.q, a.b, a.sq, a.heads, a.d, a.dtype);
+  if (!rc) rc = makeMap(&x->k, "k", a.k, a.b, a.sk, a.kv_heads, a.d, a.dtype);
+  if (!rc) rc = makeMap(&x->v, "v", a.v, a.b, a.sk, a.kv_heads, a.d, a.dtype);
+  if (!rc && backward) rc = makeMap(&x->dout, "dout", a.dout, a.b, a.sq, a.heads, a.d, a.dtype);
+  if (rc) return rc;
+  x->out = x->o = a.out;
+  x->doutPtr = a.dout.ptr;
+  x->doutB = a.dout.stride_b, x->doutS = a.dout.stride_s, x->doutH = a.dout.stride_h;
+  x->dq = a.dq, x->dk = a.dk, x->dv = a.dv, x->lse = a.lse, x->delta = a.delta;
+  x->keyLengths = a.key_lengths, x->status = a.status;
+  x->b = a.b, x->sq = a.sq, x->sk = a.sk, x->heads = a.heads, x->kvHeads = a.kv_heads, x->d = a.d, x->causal = a.causal, x->scale = a.scale;
+  return TCPXB_T_OK;
 }
 
-template <class T> int backward(const tcpxbAttention& a, cudaStream_t s) {
-  const long long rows = (long long)a.b * a.heads * a.sq, keys = (long long)a.b * a.kv_heads * a.sk;
-  if (rows) {
-    backwardQueryKernel<T><<<unsigned((rows + kWarps - 1) / kWarps), kWarps * 32, 0, s>>>(a);
-    if (const int rc = launched("attention backward, queries")) return rc;
+int launch(void (*kernel)(Args), dim3 grid, size_t shared, const Args& a, cudaStream_t s, const char* what) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+  if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  kernel<<<grid, kThreads, shared, s>>>(a);
+  return launched(what);
+}
+
+template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaStream_t s) {
+  Args x;
+  if (const int rc = makeArgs(a, backward, &x)) return rc;
+  if (!backward) {
+    if (!a.b || !a.sq) return TCPXB_T_OK;
+    return launch(forwardKernel<T, P>, dim3((a.sq + 2 * kTile - 1) / (2 * kTile), a.heads, a.b), Forward<T, P>::kShared, x, s, "attention forward");
   }
-  if (keys) backwardKeyKernel<T><<<unsigned((keys + kWarps - 1) / kWarps), kWarps * 32, 0, s>>>(a);
-  return launched("attention backward, keys");
+  if (a.b && a.sq)
+    if (const int rc = launch(queryKernel<T, P>, dim3((a.sq + kTile - 1) / kTile, a.heads, a.b), Queries<T, P>::kShared, x, s, "attention backward, queries"))
+      return rc;
+  if (!a.b || !a.sk) return TCPXB_T_OK;
+  return launch(keyKernel<T, P>, dim3((a.sk + kTile - 1) / kTile, a.kv_heads, a.b), Keys<T, P>::kShared, x, s, "attention backward, keys");
+}
+
+int dispatch(const tcpxbAttention* a, bool backward, void* stream) {
+  if (const int rc = check(a, backward)) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == TCPXB_T_BF16) return a->d <= 64 ? run<__nv_bfloat16, 1>(*a, backward, s) : run<__nv_bfloat16, 2>(*a, backward, s);
+  return a->d <= 64 ? run<__half, 1>(*a, backward, s) : run<__half, 2>(*a, backward, s);
 }
 
 }  // namespace
@@ -160,14 +737,5 @@ template <class T> int backward(const tcpxbAttention& a, cudaStream_t s) {
 
 using namespace tcpxb_train;
 
-extern "C" int tcpxb_attention_forward(const tcpxbAttention* a, void* stream) {
-  if (const int rc = check(a, false)) return rc;
-  auto s = static_cast<cudaStream_t>(stream);
-  return a->dtype == TCPXB_T_BF16 ? forward<__nv_bfloat16>(*a, s) : forward<__half>(*a, s);
-}
-
-extern "C" int tcpxb_attention_backward(const tcpxbAttention* a, void* stream) {
-  if (const int rc = check(a, true)) return rc;
-  auto s = static_cast<cudaStream_t>(stream);
-  return a->dtype == TCPXB_T_BF16 ? backward<__nv_bfloat16>(*a, s) : backward<__half>(*a, s);
-}
+extern "C" int tcpxb_attention_forward(const tcpxbAttention* a, void* stream) { return dispatch(a, false, stream); }
+extern "C" int tcpxb_attention_backward(const tcpxbAttention* a, void* stream) { return dispatch(a, true, stream); }

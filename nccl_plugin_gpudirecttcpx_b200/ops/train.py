@@ -32,7 +32,7 @@ class _Heads(ctypes.Structure):
 class _Attention(ctypes.Structure):
     _fields_ = [("q", _Heads), ("k", _Heads), ("v", _Heads), ("out", _vp), ("lse", _vp), ("dout", _Heads), ("dq", _vp), ("dk", _vp),
                 ("dv", _vp), ("delta", _vp), ("key_lengths", _vp), ("b", _i32), ("sq", _i32), ("sk", _i32), ("heads", _i32),
-                ("kv_heads", _i32), ("d", _i32), ("scale", _f32), ("causal", _i32), ("dtype", _i32)]
+                ("kv_heads", _i32), ("d", _i32), ("scale", _f32), ("causal", _i32), ("dtype", _i32), ("status", _vp)]
 
 
 class _NormRope(ctypes.Structure):
@@ -93,10 +93,10 @@ def _on_one_device(*ts: Optional[torch.Tensor]) -> torch.device:
 
 def _heads(t: torch.Tensor) -> tuple:
     """(descriptor, tensor that it points into): the tensor itself where its head rows start on 16-byte
-    boundaries, else a contiguous copy."""
+    boundaries and are not broadcast, else a contiguous copy."""
     size = t.element_size()
-    strides = [st if n > 1 else 0 for n, st in zip(t.shape, t.stride())]
-    if (t.shape[3] > 1 and t.stride(3) != 1) or t.data_ptr() % 16 or any(st * size % 16 for st in strides[:3]):
+    strides = [st if n > 1 else 16 for n, st in zip(t.shape, t.stride())]
+    if (t.shape[3] > 1 and t.stride(3) != 1) or t.data_ptr() % 16 or any(st * size % 16 or st == 0 for st in strides[:3]):
         t = t.clone(memory_format=torch.contiguous_format)
         strides = list(t.stride())
     return _Heads(t.data_ptr(), *strides[:3]), t
