@@ -20,6 +20,7 @@
 // Probabilities and score gradients are rounded to the inputs' type because the matrix units take
 // operands of one type; sums, statistics and everything else are 32-bit.
 #include <cstring>
+#include <type_traits>
 
 #include "tc.h"
 
@@ -74,7 +75,7 @@ struct Shared {
   uint64_t bars[32];
   uint32_t tmem;
   int dead;
-  float stats[4][2][kTile];  // lse and D of a stage's queries
+  alignas(16) float stats[4][2][kTile];  // lse and D of a stage's queries
 };
 constexpr int kSharedBytes = 6144;
 static_assert(sizeof(Shared) <= kSharedBytes, "barriers and statistics");
@@ -138,8 +139,8 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  // long rows first: with a causal mask the last queries see the most keys
-  const int q0 = (int(gridDim.x) - 1 - int(blockIdx.x)) * 2 * kTile, h = blockIdx.y, b = blockIdx.z, kv = h / (a.heads / a.kvHeads);
+  // the longest blocks first, over all heads and batches: with a causal mask the last queries see the most keys
+  const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * 2 * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
   const int keys = keysOf(a, b);
   int n[2];
 #pragma unroll
@@ -234,7 +235,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
 #pragma unroll
       for (int k = 0; k < kTile; k += 8)
 #pragma unroll
-        for (int u = 0; u < 4; u++) m[u] = fmaxf(m[u], fmaxf(__uint_as_float(x[k + u]), __uint_as_float(x[k + 4 + u])));
+        for (int u = 0; u < 4; u++) m[u] = max3(m[u], __uint_as_float(x[k + u]), __uint_as_float(x[k + 4 + u]));
       const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
       const bool grown = (now - top) * c > 8.f || (top == -INFINITY && now > -INFINITY);
       if (__any_sync(0xffffffffu, grown)) {
@@ -311,7 +312,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
                  vRing = kRing + F::kKSlots * F::kTileBytes;
   const auto bar = [&](int i) { return smemAddr(bars) + 8 * i; };
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int q0 = (int(gridDim.x) - 1 - int(blockIdx.x)) * kTile, h = blockIdx.y, b = blockIdx.z, kv = h / (a.heads / a.kvHeads);
+  const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
   const int keys = keysOf(a, b), n = tiles(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
 
   if (threadIdx.x == 0) {
@@ -430,18 +431,21 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       tmemLoad32(dp + half * 64 + lanes, y);
       tmemLoad32(dp + half * 64 + lanes + 32, y + 32);
       tmemWaitLoad();
-      const bool some = j >= whole;
       const int left = seen - j * kTile - half * 64;
+      const auto gradients = [&](auto masked) {
 #pragma unroll
-      for (int k = 0; k < 64; k += 2) {
-        float2 g = add2({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, {-delta, -delta});
-        g = mul2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, g);
-        if (some) {
-          g.x = k < left ? g.x : 0.f;
-          g.y = k + 1 < left ? g.y : 0.f;
+        for (int k = 0; k < 64; k += 2) {
+          float2 g = add2({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, {-delta, -delta});
+          g = mul2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, g);
+          if (decltype(masked)::value) {
+            g.x = k < left ? g.x : 0.f;
+            g.y = k + 1 < left ? g.y : 0.f;
+          }
+          ds[k / 2] = pack2<T>(g.x, g.y);
         }
-        ds[k / 2] = pack2<T>(g.x, g.y);
-      }
+      };
+      if (j < whole) gradients(std::false_type());
+      else gradients(std::true_type());
       tmemStore32(s, ds);
       tmemWaitStore();
       tcBefore();
@@ -478,7 +482,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int j0 = blockIdx.x * kTile, kv = blockIdx.y, b = blockIdx.z, group = a.heads / a.kvHeads;
+  const int j0 = blockIdx.z * kTile, kv = blockIdx.x, b = blockIdx.y, group = a.heads / a.kvHeads;
   const int keys = keysOf(a, b);
   const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kTile : 0;  // first query tile that sees a key of this one
   const int each = j0 < keys ? max(0, tiles(a.sq) - first) : 0, n = each * group;
@@ -569,8 +573,8 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
     const float c = a.scale * kLog2e;
     for (int it = 0; it < n; it++) {
       const int st = it % F::kStages, q0 = (first + it % each) * kTile;
-      const float2* l = reinterpret_cast<const float2*>(sh.stats[st][0] + half * 64);
-      const float2* d = reinterpret_cast<const float2*>(sh.stats[st][1] + half * 64);
+      const float4* l = reinterpret_cast<const float4*>(sh.stats[st][0] + half * 64);
+      const float4* d = reinterpret_cast<const float4*>(sh.stats[st][1] + half * 64);
       // first query of this half that sees the row's key
       const int from = !counts ? 64 : a.causal ? j - (a.sk - a.sq) - q0 - half * 64 : 0;
       const bool some = j0 + kTile > keys || (a.causal && j0 + kTile - 1 > q0 + a.sk - a.sq);
@@ -581,17 +585,26 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
       tmemLoad32(s + half * 64 + lanes, x);
       tmemLoad32(s + half * 64 + lanes + 32, x + 32);
       tmemWaitLoad();
+      const auto probabilities = [&](auto masked) {
 #pragma unroll
-      for (int k = 0; k < 64; k += 2) {
-        float2 e = fma2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, {c, c}, l[k / 2]);
-        e.x = exp2Fast(e.x), e.y = exp2Fast(e.y);
-        if (some) {
-          e.x = k >= from ? e.x : 0.f;
-          e.y = k + 1 >= from ? e.y : 0.f;
+        for (int k = 0; k < 64; k += 4) {
+          const float4 ll = l[k / 4];
+          const float2 ls[2] = {{ll.x, ll.y}, {ll.z, ll.w}};
+#pragma unroll
+          for (int u = k; u < k + 4; u += 2) {
+            float2 e = fma2({__uint_as_float(x[u]), __uint_as_float(x[u + 1])}, {c, c}, ls[(u - k) / 2]);
+            e.x = exp2Fast(e.x), e.y = exp2Fast(e.y);
+            if (decltype(masked)::value) {
+              e.x = u >= from ? e.x : 0.f;
+              e.y = u + 1 >= from ? e.y : 0.f;
+            }
+            x[u] = __float_as_uint(e.x), x[u + 1] = __float_as_uint(e.y);
+            o[u / 2] = pack2<T>(e.x, e.y);
+          }
         }
-        x[k] = __float_as_uint(e.x), x[k + 1] = __float_as_uint(e.y);
-        o[k / 2] = pack2<T>(e.x, e.y);
-      }
+      };
+      if (some) probabilities(std::true_type());
+      else probabilities(std::false_type());
       tmemStore32(s + half * 64 + lanes, o);
       tmemWaitStore();
       tcBefore();
@@ -604,16 +617,25 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
       tmemLoad32(dp + half * 64 + lanes, y);
       tmemLoad32(dp + half * 64 + lanes + 32, y + 32);
       tmemWaitLoad();
+      const auto gradients = [&](auto masked) {
 #pragma unroll
-      for (int k = 0; k < 64; k += 2) {
-        float2 g = add2({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, d[k / 2]);
-        g = mul2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, g);
-        if (some) {
-          g.x = k >= from ? g.x : 0.f;
-          g.y = k + 1 >= from ? g.y : 0.f;
+        for (int k = 0; k < 64; k += 4) {
+          const float4 dd = d[k / 4];
+          const float2 ds[2] = {{dd.x, dd.y}, {dd.z, dd.w}};
+#pragma unroll
+          for (int u = k; u < k + 4; u += 2) {
+            float2 g = add2({__uint_as_float(y[u]), __uint_as_float(y[u + 1])}, ds[(u - k) / 2]);
+            g = mul2({__uint_as_float(x[u]), __uint_as_float(x[u + 1])}, g);
+            if (decltype(masked)::value) {
+              g.x = u >= from ? g.x : 0.f;
+              g.y = u + 1 >= from ? g.y : 0.f;
+            }
+            o[u / 2] = pack2<T>(g.x, g.y);
+          }
         }
-        o[k / 2] = pack2<T>(g.x, g.y);
-      }
+      };
+      if (some) gradients(std::true_type());
+      else gradients(std::false_type());
       tmemStore32(dp + half * 64 + lanes, o);
       tmemWaitStore();
       tcBefore();
@@ -670,8 +692,8 @@ int check(const tcpxbAttention* a, bool backward) {
   if (!a) return fail(TCPXB_T_INVALID, "null argument");
   if (a->b < 0 || a->sq < 0 || a->sk < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->d < 8 || a->d > kMaxD || a->d % 8)
     return fail(TCPXB_T_INVALID, "bad shape: b %d sq %d sk %d heads %d/%d d %d", a->b, a->sq, a->sk, a->heads, a->kv_heads, a->d);
-  if (a->b > 65535 || a->heads > 65535 || a->sq > 1 << 30 || a->sk > 1 << 30)
-    return fail(TCPXB_T_INVALID, "at most 65535 batches and heads and 2^30 tokens: b %d heads %d sq %d sk %d", a->b, a->heads, a->sq, a->sk);
+  if (a->b > 65535 || a->heads > 65535 || a->sq > 65535 * kTile || a->sk > 65535 * kTile)
+    return fail(TCPXB_T_INVALID, "at most 65535 batches, heads and tiles of 128 tokens: b %d heads %d sq %d sk %d", a->b, a->heads, a->sq, a->sk);
   if (a->dtype != TCPXB_T_BF16 && a->dtype != TCPXB_T_F16) return fail(TCPXB_T_INVALID, "attention takes bf16 and fp16, not type %d", a->dtype);
   if (!(a->scale > 0.f) || a->scale > 1e30f) return fail(TCPXB_T_INVALID, "scale has to be finite and above zero");
   const bool queries = (long long)a->b * a->sq > 0, keys = (long long)a->b * a->sk > 0;
@@ -716,13 +738,13 @@ template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaSt
   if (const int rc = makeArgs(a, backward, &x)) return rc;
   if (!backward) {
     if (!a.b || !a.sq) return TCPXB_T_OK;
-    return launch(forwardKernel<T, P>, dim3((a.sq + 2 * kTile - 1) / (2 * kTile), a.heads, a.b), Forward<T, P>::kShared, x, s, "attention forward");
+    return launch(forwardKernel<T, P>, dim3(a.heads, a.b, (a.sq + 2 * kTile - 1) / (2 * kTile)), Forward<T, P>::kShared, x, s, "attention forward");
   }
   if (a.b && a.sq)
-    if (const int rc = launch(queryKernel<T, P>, dim3((a.sq + kTile - 1) / kTile, a.heads, a.b), Queries<T, P>::kShared, x, s, "attention backward, queries"))
+    if (const int rc = launch(queryKernel<T, P>, dim3(a.heads, a.b, (a.sq + kTile - 1) / kTile), Queries<T, P>::kShared, x, s, "attention backward, queries"))
       return rc;
   if (!a.b || !a.sk) return TCPXB_T_OK;
-  return launch(keyKernel<T, P>, dim3((a.sk + kTile - 1) / kTile, a.kv_heads, a.b), Keys<T, P>::kShared, x, s, "attention backward, keys");
+  return launch(keyKernel<T, P>, dim3(a.kv_heads, a.b, (a.sk + kTile - 1) / kTile), Keys<T, P>::kShared, x, s, "attention backward, keys");
 }
 
 int dispatch(const tcpxbAttention* a, bool backward, void* stream) {
