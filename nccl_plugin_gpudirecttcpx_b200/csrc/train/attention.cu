@@ -138,7 +138,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
   const uint32_t tile0 = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, ring = tile0 + 2 * F::kTileBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   // the longest blocks first, over all heads and batches: with a causal mask the last queries see the most keys
   const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * 2 * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
   const int keys = keysOf(a, b);
@@ -156,7 +156,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
   tcBefore();
   __syncthreads();
   tcAfter();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = uniform(sh.tmem);
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -174,6 +174,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
     const uint32_t scores = mmaShape<T>(kTile, false), values = mmaShape<T>(steps * 16, true);
     for (int j = 0; j <= most; j++) {
@@ -189,21 +190,21 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
         if (j && j <= n[t]) {
           barWait(bar(F::kPFull + t), (j - 1) & 1, dead);
           tcAfter();
-          if (lane == 0) {
-            for (int k = 0; k < kTile / 16; k++) mmaFromTmem(o, s + k * 8, acrossRows(vTileAt, k), values, j > 1 || k);
+          if (leader) {
+            mmaTmemTile<32>(o, s, vTileAt, values, j > 1);
             if (j == n[t]) mmaCommit(bar(F::kOFull + t));
           }
         }
         if (j < n[t]) {
           if (j == 0) barWait(bar(F::kQFull + t), 0, dead);
-          if (lane == 0) {
+          if (leader) {
             // in issue order behind the product that reads P out of the same columns
-            for (int k = 0; k < steps; k++) mma(s, alongRow(tile0 + t * F::kTileBytes, k), alongRow(kTileAt, k), scores, k);
+            mmaTiles<P>(s, tile0 + t * F::kTileBytes, kTileAt, scores, steps);
             mmaCommit(bar(F::kSFull + t));
           }
         }
       }
-      if (lane == 0) {
+      if (leader) {
         // only where a load waits for it: no arrival may come after the block has gone
         if (ik + F::kSlots < 2 * most) mmaCommit(bar(F::kEmpty + ik % F::kSlots));
         if (j && iv + F::kSlots < 2 * most) mmaCommit(bar(F::kEmpty + iv % F::kSlots));
@@ -311,7 +312,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
   const uint32_t tile0 = (smemAddr(raw) + 1024 + 1023) / 1024 * 1024, qTile = tile0, doTile = tile0 + F::kTileBytes, kRing = tile0 + 2 * F::kTileBytes,
                  vRing = kRing + F::kKSlots * F::kTileBytes;
   const auto bar = [&](int i) { return smemAddr(bars) + 8 * i; };
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
   const int keys = keysOf(a, b), n = tiles(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
 
@@ -324,7 +325,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
   tcBefore();
   __syncthreads();
   tcAfter();
-  const uint32_t tmem = *tmemAt, dp = tmem + 2 * kTile, dq = tmem + 3 * kTile;
+  const uint32_t tmem = uniform(*tmemAt), dp = tmem + 2 * kTile, dq = tmem + 3 * kTile;
 
   if (warp == kLoadWarp) {
     if (lane == 0 && n) {
@@ -343,6 +344,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
     const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
     const auto score = [&](int j) {  // S of key tile j
@@ -350,16 +352,16 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       const uint32_t kTileAt = kRing + ks * F::kTileBytes;
       barWait(bar(F::kKFull + ks), j / F::kKSlots & 1, dead);
       if ((j + 1) * kTile > keys && keys < a.sk) clearRows<P>(kTileAt, keys - j * kTile);
-      if (lane == 0) {
-        for (int k = 0; k < steps; k++) mma(tmem + (j & 1) * kTile, alongRow(qTile, k), alongRow(kTileAt, k), scores, k);
+      if (leader) {
+        mmaTiles<P>(tmem + (j & 1) * kTile, qTile, kTileAt, scores, steps);
         mmaCommit(bar(F::kSFull + (j & 1)));
       }
     };
     const auto gradient = [&](int j) {  // dP of key tile j
       const int vs = j % F::kVSlots;
       barWait(bar(F::kVFull + vs), j / F::kVSlots & 1, dead);
-      if (lane == 0) {
-        for (int k = 0; k < steps; k++) mma(dp, alongRow(doTile, k), alongRow(vRing + vs * F::kTileBytes, k), scores, k);
+      if (leader) {
+        mmaTiles<P>(dp, doTile, vRing + vs * F::kTileBytes, scores, steps);
         mmaCommit(bar(F::kDpFull));
         if (j + F::kVSlots < n) mmaCommit(bar(F::kVEmpty + vs));
       }
@@ -373,11 +375,9 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
         barWait(bar(F::kDsFull), j & 1, dead);
         tcAfter();
         if (j + 1 < n) gradient(j + 1);
-        if (lane == 0) {
+        if (leader) {
           const int ks = j % F::kKSlots;
-          const uint32_t ds = tmem + (j & 1) * kTile;
-          for (int k = 0; k < kTile / 16; k++)
-            mmaFromTmem(dq, ds + k / 4 * 64 + k % 4 * 8, acrossRows(kRing + ks * F::kTileBytes, k), back, j || k);
+          mmaTmemTile<64>(dq, tmem + (j & 1) * kTile, kRing + ks * F::kTileBytes, back, j > 0);
           if (j + F::kKSlots < n) mmaCommit(bar(F::kKEmpty + ks));
           if (j == n - 1) mmaCommit(bar(F::kDone));
         }
@@ -481,7 +481,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
   const uint32_t kTileAt = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, vTileAt = kTileAt + F::kTileBytes, ring = vTileAt + F::kTileBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   const int j0 = blockIdx.z * kTile, kv = blockIdx.x, b = blockIdx.y, group = a.heads / a.kvHeads;
   const int keys = keysOf(a, b);
   const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kTile : 0;  // first query tile that sees a key of this one
@@ -497,7 +497,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
   tcBefore();
   __syncthreads();
   tcAfter();
-  const uint32_t tmem = sh.tmem, s = tmem, dp = tmem + kTile, dv = tmem + 2 * kTile, dk = tmem + 3 * kTile;
+  const uint32_t tmem = uniform(sh.tmem), s = tmem, dp = tmem + kTile, dv = tmem + 2 * kTile, dk = tmem + 3 * kTile;
 
   if (warp == kLoadWarp) {
     if (lane == 0 && n) {
@@ -529,6 +529,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
     const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
     if (n) {
@@ -539,28 +540,26 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
         if (it >= 0) {
           barWait(bar(F::kPFull), it & 1, dead);
           tcAfter();
-          if (lane == 0)
-            for (int k = 0; k < kTile / 16; k++)
-              mmaFromTmem(dv, s + k / 4 * 64 + k % 4 * 8, acrossRows(q + F::kTileBytes, k), back, it || k);
+          if (leader) mmaTmemTile<64>(dv, s, q + F::kTileBytes, back, it > 0);
         }
         if (it + 1 < n) {
           barWait(bar(F::kFull + next), (it + 1) / F::kStages & 1, dead);
-          if (lane == 0) {
-            for (int k = 0; k < steps; k++) mma(s, alongRow(kTileAt, k), alongRow(qn, k), scores, k);
+          if (leader) {
+            mmaTiles<P>(s, kTileAt, qn, scores, steps);
             mmaCommit(bar(F::kSFull));
           }
         }
         if (it >= 0) {
           barWait(bar(F::kDsFull), it & 1, dead);
           tcAfter();
-          if (lane == 0) {
-            for (int k = 0; k < kTile / 16; k++) mmaFromTmem(dk, dp + k / 4 * 64 + k % 4 * 8, acrossRows(q, k), back, it || k);
+          if (leader) {
+            mmaTmemTile<64>(dk, dp, q, back, it > 0);
             if (it + F::kStages < n) mmaCommit(bar(F::kEmpty + st));
             if (it == n - 1) mmaCommit(bar(F::kDone));
           }
         }
-        if (it + 1 < n && lane == 0) {
-          for (int k = 0; k < steps; k++) mma(dp, alongRow(vTileAt, k), alongRow(qn + F::kTileBytes, k), scores, k);
+        if (it + 1 < n && leader) {
+          mmaTiles<P>(dp, vTileAt, qn + F::kTileBytes, scores, steps);
           mmaCommit(bar(F::kDpFull));
         }
         __syncwarp();

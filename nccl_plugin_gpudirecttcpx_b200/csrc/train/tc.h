@@ -11,6 +11,15 @@ constexpr int kStatusTimeout = 3;  // TCPXB_ST_TIMEOUT
 
 __device__ __forceinline__ uint32_t smemAddr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
+// A value that is the same in all lanes, told to the compiler: descriptors and addresses of matrix
+// instructions are then kept where those take them from.
+template <class T> __device__ __forceinline__ T uniform(T x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ bool electOne() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---- barriers
 __device__ __forceinline__ void barInit(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -118,11 +127,6 @@ constexpr uint32_t kPanelBytes = 128 * 128;
 __device__ __forceinline__ uint64_t operandDesc(uint32_t addr, uint32_t panelStride) {
   return uint64_t((addr & 0x3ffff) >> 4) | uint64_t(panelStride >> 4) << 16 | uint64_t(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
-// Tile with the summed index along its rows' elements, at 16-element step k.
-__device__ __forceinline__ uint64_t alongRow(uint32_t tile, int k) { return operandDesc(tile + (k / 4) * kPanelBytes + (k % 4) * 32, 16); }
-// Tile with the summed index along its rows, at 16-row step k.
-__device__ __forceinline__ uint64_t acrossRows(uint32_t tile, int k) { return operandDesc(tile + k * 2048, kPanelBytes); }
-
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -136,6 +140,25 @@ __device__ __forceinline__ void mmaFromTmem(uint32_t d, uint32_t a, uint64_t b, 
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(shape), "r"(uint32_t(add))
       : "memory");
+}
+// One tile product is a run of instructions whose operands lie constants apart: only the first
+// descriptors are computed, so that the issuing thread keeps ahead of the matrix units (with
+// descriptors built for each instruction it needed 90 cycles for what they do in 32 to 64).
+// d = A B^T over `steps` x 16 head elements, both tiles in shared memory.
+template <int P> __device__ __forceinline__ void mmaTiles(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, int steps) {
+  const uint64_t da = operandDesc(a, 16), db = operandDesc(b, 16);
+#pragma unroll
+  for (int k = 0; k < P * 4; k++) {
+    const uint64_t off = (k / 4 * kPanelBytes + k % 4 * 32) >> 4;
+    if (k < steps) mma(d, da + off, db + off, shape, k > 0);
+  }
+}
+// d (+)= A B over 128 rows of B: A lies in tensor memory, two elements a column, in two runs of 32
+// columns that begin `half` columns apart; B's rows are the summed index.
+template <int kHalf> __device__ __forceinline__ void mmaTmemTile(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, bool add) {
+  const uint64_t db = operandDesc(b, kPanelBytes);
+#pragma unroll
+  for (int k = 0; k < 8; k++) mmaFromTmem(d, a + k / 4 * kHalf + k % 4 * 8, db + k * (2048 >> 4), shape, add || k > 0);
 }
 // The barrier gets one arrival when all matrix instructions that this thread has issued are done.
 __device__ __forceinline__ void mmaCommit(uint32_t bar) {
