@@ -93,14 +93,15 @@ typedef struct tcpxbAdamwTensor {
 } tcpxbAdamwTensor;
 
 typedef struct tcpxbAdamw {
-  float lr, beta1, beta2, eps, weight_decay;
-  const float* grad_norm;  // device scalar: gradients are scaled by min(1, max_norm / (grad_norm + 1e-6)); null: not clipped
+  double lr, beta1, beta2, eps, weight_decay;
+  float* grad_norm;        // device scalar: gradients are scaled by min(1, max_norm / (grad_norm + 1e-6)); null: not clipped
   float max_norm;
+  int32_t compute_norm;    // write *grad_norm first, as tcpxb_grad_norm would
   int32_t state_bits, dtype;
-  void* scratch;           // tcpxb_adamw_scratch_bytes(count)
+  void* scratch;           // tcpxb_adamw_scratch_bytes()
 } tcpxbAdamw;
 
-size_t tcpxb_adamw_scratch_bytes(int count);
+size_t tcpxb_adamw_scratch_bytes(const tcpxbAdamwTensor* tensors, int count);
 int tcpxb_adamw_step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw* a, void* stream);
 
 // *norm = sqrt(sum of squares over all gradients (`g`, `n` of each tensor)).

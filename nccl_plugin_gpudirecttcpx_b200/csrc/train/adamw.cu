@@ -24,13 +24,17 @@ namespace tcpxb_train {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 8192;
+// Elements of a CTA: short chunks while they do not fill the GPU a few times, else longer ones,
+// which begin and end less often (323 M weights with 8-bit states: 1.61 ms in chunks of 8192).
+constexpr int kShortChunk = 8192, kLongChunk = 32768;
+constexpr long long kManyElements = 148ll * 8 * 4 * kShortChunk;
 constexpr float kE4m3Max = 448.f;
 
 template <int N> struct List {
   tcpxbAdamwTensor t[N];
   unsigned end[N];  // chunks up to and with tensor i
   int count, first;  // `first`: number of t[0] in the caller's list
+  int chunk;
 };
 // Two sizes of the same launch: a short list does not pay for copying 30 KB of parameters.
 using Short = List<24>;
@@ -55,100 +59,6 @@ template <class L> __device__ __forceinline__ int tensorOf(const L& l, unsigned 
   return lo;
 }
 
-// Counts every tensor's step and takes what depends on it, in 64 bits: 1 - b^t cancels.
-template <class L> __global__ void prepareKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
-  auto* s = static_cast<Scratch*>(a.scratch);
-  if (threadIdx.x == 0 && l.first == 0) {
-    float coef = 1.f;
-    if (a.grad_norm) {
-      const float c = a.max_norm / (*a.grad_norm + 1e-6f);
-      coef = c < 1.f || c != c ? c : 1.f;
-    }
-    s->coef = coef;
-  }
-  for (int i = threadIdx.x; i < l.count; i += blockDim.x) {
-    const int t = ++*l.t[i].step;
-    s->rates[l.first + i].stepSize = float(double(a.lr) / (1.0 - pow(double(a.beta1), t)));
-    s->rates[l.first + i].rootCorrection = float(1.0 / sqrt(1.0 - pow(double(a.beta2), t)));
-  }
-}
-
-struct Step {
-  float beta1, beta2, eps, keep, stepSize, rootCorrection, coef;
-  __device__ __forceinline__ float operator()(float p, float g, float& m, float& v) const {
-    g *= coef;
-    m = m * beta1 + (1.f - beta1) * g;
-    v = v * beta2 + (1.f - beta2) * g * g;
-    return p * keep - stepSize * m / (sqrtf(v) * rootCorrection + eps);
-  }
-};
-
-__device__ __forceinline__ float fromE4m3(__nv_fp8_storage_t x) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3))); }
-
-// Largest magnitude of the warp; NaN is left out (its code is NaN by itself).
-__device__ __forceinline__ float warpTop(float x) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-  return x;
-}
-
-template <class T, class L, bool kSmall> __global__ void __launch_bounds__(kThreads) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
-  const int i = tensorOf(l, blockIdx.x);
-  const tcpxbAdamwTensor& t = l.t[i];
-  const long long begin = (long long)(blockIdx.x - (i ? l.end[i - 1] : 0)) * kChunk;
-  const long long end = min((long long)t.n, begin + kChunk);
-  const auto* s = static_cast<const Scratch*>(a.scratch);
-  const Step step{a.beta1, a.beta2, a.eps, 1.f - a.lr * a.weight_decay, s->rates[l.first + i].stepSize, s->rates[l.first + i].rootCorrection, s->coef};
-  T* p = static_cast<T*>(t.p);
-  const T* g = static_cast<const T*>(t.g);
-  if (!kSmall) {
-    float *m = static_cast<float*>(t.m), *v = static_cast<float*>(t.v);
-    for (long long e = begin + threadIdx.x; e < end; e += kThreads) {
-      float mm = m[e], vv = v[e];
-      const float w = step(t.master ? t.master[e] : toFloat(p[e]), toFloat(g[e]), mm, vv);
-      m[e] = mm, v[e] = vv, p[e] = fromFloat<T>(w);
-      if (t.master) t.master[e] = w;
-    }
-    return;
-  }
-  auto *m = static_cast<__nv_fp8_storage_t*>(t.m), *v = static_cast<__nv_fp8_storage_t*>(t.v);
-  const int lane = threadIdx.x % 32;
-  for (long long b = begin + threadIdx.x / 32 * TCPXB_ADAMW_BLOCK; b < end; b += kThreads / 32 * TCPXB_ADAMW_BLOCK) {
-    const long long block = b / TCPXB_ADAMW_BLOCK;
-    const float ms = t.m_scale[block], vs = t.v_scale[block];
-    float mm[8] = {}, vv[8] = {}, topM = 0.f, topV = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const long long e = b + k * 32 + lane;
-      if (e >= end) continue;
-      mm[k] = fromE4m3(m[e]) * ms;
-      const float root = fromE4m3(v[e]) * vs;
-      vv[k] = root * root;
-      const float w = step(t.master ? t.master[e] : toFloat(p[e]), toFloat(g[e]), mm[k], vv[k]);
-      p[e] = fromFloat<T>(w);
-      if (t.master) t.master[e] = w;
-      vv[k] = sqrtf(vv[k]);
-      topM = fmaxf(topM, fabsf(mm[k])), topV = fmaxf(topV, vv[k]);
-    }
-    topM = warpTop(topM), topV = warpTop(topV);
-    // below 1e-30 a block is held as zeros: the factor back would leave the range
-    const float toM = topM >= 1e-30f ? kE4m3Max / topM : 0.f, toV = topV >= 1e-30f ? kE4m3Max / topV : 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const long long e = b + k * 32 + lane;
-      if (e >= end) continue;
-      float root = vv[k] * toV;
-      if (root > 0.f) root = fmaxf(root, 0.001953125f);  // 2^-9, the smallest code above zero
-      m[e] = __nv_cvt_float_to_fp8(mm[k] * toM, __NV_SATFINITE, __NV_E4M3);
-      v[e] = __nv_cvt_float_to_fp8(root, __NV_SATFINITE, __NV_E4M3);
-    }
-    if (lane == 0) {
-      t.m_scale[block] = topM >= 1e-30f ? topM / kE4m3Max : 0.f;
-      t.v_scale[block] = topV >= 1e-30f ? topV / kE4m3Max : 0.f;
-    }
-  }
-}
-
 __device__ __forceinline__ double blockSum(double x) {
   __shared__ double part[32];
 #pragma unroll
@@ -160,39 +70,319 @@ __device__ __forceinline__ double blockSum(double x) {
   return x;
 }
 
+__device__ __forceinline__ float rootOfSum(const double* partial, long long n) {
+  double sum = 0;
+  for (long long i = threadIdx.x; i < n; i += blockDim.x) sum += partial[i];
+  return float(sqrt(blockSum(sum)));
+}
+
+// Counts every tensor's step and takes what depends on it, in 64 bits: 1 - b^t cancels.  The first
+// list's launch also takes the norm out of `partials` sums, where it is computed here.
+template <class L> __global__ void __launch_bounds__(512) prepareKernel(const __grid_constant__ L l, const tcpxbAdamw a, const double* partial, long long partials) {
+  auto* s = static_cast<Scratch*>(a.scratch);
+  if (l.first == 0) {
+    float norm = 0.f;
+    if (partial) norm = rootOfSum(partial, partials);
+    else if (a.grad_norm) norm = *a.grad_norm;
+    if (threadIdx.x == 0) {
+      if (partial) *a.grad_norm = norm;
+      float coef = 1.f;
+      if (a.grad_norm) {
+        const float c = a.max_norm / (norm + 1e-6f);
+        coef = c < 1.f || c != c ? c : 1.f;
+      }
+      s->coef = coef;
+    }
+  }
+  for (int i = threadIdx.x; i < l.count; i += blockDim.x) {
+    const int t = ++*l.t[i].step;
+    s->rates[l.first + i].stepSize = float(a.lr / (1.0 - pow(a.beta1, t)));
+    s->rates[l.first + i].rootCorrection = float(1.0 / sqrt(1.0 - pow(a.beta2, t)));
+  }
+}
+
+// Two elements.  m and v are taken in the formula's order, every product and sum rounded by
+// itself: 8-bit codes then fall as those of any plain 32-bit computation do.  The root and the
+// quotient are the approximate ones (2 units in the last place of 32 bits, a v under 2^-126 counts
+// as zero): they touch the weight's own step, and the exact ones would make the 8-bit kernel wait
+// for arithmetic.
+struct Step {
+  float beta1, beta2, rest1, rest2, eps, keep, stepSize, rootCorrection, coef;
+  __device__ __forceinline__ void operator()(float2& p, float2 g, float2& m, float2& v, float2& root) const {
+    g = mul2(g, {coef, coef});
+    m = add2(mul2(m, {beta1, beta1}), mul2(g, {rest1, rest1}));
+    v = add2(mul2(v, {beta2, beta2}), mul2(mul2(g, {rest2, rest2}), g));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.x) : "f"(v.x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.y) : "f"(v.y));
+    float2 below = fma2(root, {rootCorrection, rootCorrection}, {eps, eps});
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(below.x) : "f"(below.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(below.y) : "f"(below.y));
+    p = fma2(p, {keep, keep}, mul2(mul2(m, {-stepSize, -stepSize}), below));
+  }
+};
+
+// Eight elements of a lane, as pairs, and as they lie in memory.
+template <class T> __device__ __forceinline__ void pairs(const Vec8<T>& x, float2 (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) f[i] = {toFloat(x.x[2 * i]), toFloat(x.x[2 * i + 1])};
+}
+template <class T> __device__ __forceinline__ Vec8<T> rounded(const float2 (&f)[4]) {
+  Vec8<T> x;
+#pragma unroll
+  for (int i = 0; i < 4; i++) x.x[2 * i] = fromFloat<T>(f[i].x), x.x[2 * i + 1] = fromFloat<T>(f[i].y);
+  return x;
+}
+struct alignas(8) Codes { __nv_fp8x2_storage_t c[4]; };
+__device__ __forceinline__ void decode(const Codes& x, float scale, float2 (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) f[i] = mul2(__half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(x.c[i], __NV_E4M3))), {scale, scale});
+}
+__device__ __forceinline__ Codes encode(const float2 (&f)[4]) {
+  Codes x;
+#pragma unroll
+  for (int i = 0; i < 4; i++) x.c[i] = __nv_cvt_float2_to_fp8x2(f[i], __NV_SATFINITE, __NV_E4M3);
+  return x;
+}
+
+// Eight elements from `at` on: a vector, or those below `end` one by one.
+template <bool kVector, class V, class T> __device__ __forceinline__ V get(const T* p, long long at, long long end) {
+  if constexpr (kVector) return *reinterpret_cast<const V*>(p + at);
+  V x = {};
+  T* e = reinterpret_cast<T*>(&x);
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (at + i < end) e[i] = p[at + i];
+  return x;
+}
+template <bool kVector, class V, class T> __device__ __forceinline__ void put(T* p, long long at, long long end, const V& x) {
+  if constexpr (kVector) {
+    *reinterpret_cast<V*>(p + at) = x;
+  } else {
+    const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (at + i < end) p[at + i] = e[i];
+  }
+}
+
+template <class T> __device__ __forceinline__ bool aligned(const T* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// 32-bit states, whole vectors: a thread has two runs of eight elements in flight, 96 bytes each.
+template <class T> __device__ __forceinline__ void stepVectors(const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end) {
+  T* p = static_cast<T*>(t.p);
+  const T* g = static_cast<const T*>(t.g);
+  float *m = static_cast<float*>(t.m), *v = static_cast<float*>(t.v);
+#pragma unroll 2
+  for (long long e = begin + threadIdx.x * 8; e < end; e += kThreads * 8) {
+    float2 pp[4], gg[4], mm[4], vv[4], root;
+    if (t.master) pairs(*reinterpret_cast<const Vec8<float>*>(t.master + e), pp);
+    else pairs(*reinterpret_cast<const Vec8<T>*>(p + e), pp);
+    pairs(*reinterpret_cast<const Vec8<T>*>(g + e), gg);
+    pairs(*reinterpret_cast<const Vec8<float>*>(m + e), mm);
+    pairs(*reinterpret_cast<const Vec8<float>*>(v + e), vv);
+#pragma unroll
+    for (int i = 0; i < 4; i++) step(pp[i], gg[i], mm[i], vv[i], root);
+    *reinterpret_cast<Vec8<float>*>(m + e) = rounded<float>(mm);
+    *reinterpret_cast<Vec8<float>*>(v + e) = rounded<float>(vv);
+    *reinterpret_cast<Vec8<T>*>(p + e) = rounded<T>(pp);
+    if (t.master) *reinterpret_cast<Vec8<float>*>(t.master + e) = rounded<float>(pp);
+  }
+}
+
+// 32-bit states, any alignment and the ends: one element a lane, four in flight.
+template <class T> __device__ __forceinline__ void stepElements(const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end) {
+  T* p = static_cast<T*>(t.p);
+  const T* g = static_cast<const T*>(t.g);
+  float *m = static_cast<float*>(t.m), *v = static_cast<float*>(t.v);
+  for (long long e0 = begin + threadIdx.x; e0 < end; e0 += kThreads * 4) {
+    float pp[4] = {}, gg[4] = {}, mm[4] = {}, vv[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const long long e = e0 + i * kThreads;
+      if (e < end) pp[i] = t.master ? t.master[e] : toFloat(p[e]), gg[i] = toFloat(g[e]), mm[i] = m[e], vv[i] = v[e];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      float2 w = {pp[i], pp[i + 1]}, m2 = {mm[i], mm[i + 1]}, v2 = {vv[i], vv[i + 1]}, root;
+      step(w, {gg[i], gg[i + 1]}, m2, v2, root);
+      pp[i] = w.x, pp[i + 1] = w.y, mm[i] = m2.x, mm[i + 1] = m2.y, vv[i] = v2.x, vv[i + 1] = v2.y;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const long long e = e0 + i * kThreads;
+      if (e >= end) break;
+      m[e] = mm[i], v[e] = vv[i], p[e] = fromFloat<T>(pp[i]);
+      if (t.master) t.master[e] = pp[i];
+    }
+  }
+}
+
+// 8-bit states.  A warp has the next block's loads in flight while it works on one.
+template <class T> struct Raw {
+  Vec8<T> p, g;
+  Codes m, v;
+  float mScale, vScale;
+};
+template <bool kVector, class T> __device__ __forceinline__ void fetch(Raw<T>& r, const tcpxbAdamwTensor& t, long long b, long long end) {
+  const long long e = b + threadIdx.x % 32 * 8;
+  r.p = get<kVector, Vec8<T>>(static_cast<const T*>(t.p), e, end);
+  r.g = get<kVector, Vec8<T>>(static_cast<const T*>(t.g), e, end);
+  r.m = get<kVector, Codes>(static_cast<const __nv_fp8_storage_t*>(t.m), e, end);
+  r.v = get<kVector, Codes>(static_cast<const __nv_fp8_storage_t*>(t.v), e, end);
+  r.mScale = t.m_scale[b / TCPXB_ADAMW_BLOCK];
+  r.vScale = t.v_scale[b / TCPXB_ADAMW_BLOCK];
+}
+// Largest magnitudes of the warp; NaN is left out (its code is NaN by itself).
+__device__ __forceinline__ void warpTops(float& x, float& y) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+  }
+}
+template <bool kVector, class T> __device__ __forceinline__ void stepBlock(const Raw<T>& r, const tcpxbAdamwTensor& t, const Step& step, long long b, long long end) {
+  const int lane = threadIdx.x % 32;
+  const long long e = b + lane * 8;
+  float2 pp[4], gg[4], mm[4], vv[4], root[4];
+  if (t.master) pairs(get<kVector, Vec8<float>>(t.master, e, end), pp);
+  else pairs(r.p, pp);
+  pairs(r.g, gg);
+  decode(r.m, r.mScale, mm);
+  decode(r.v, r.vScale, vv);
+  float topM = 0.f, topV = 0.f;
+  // past the end everything is zero and stays so
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    vv[i] = mul2(vv[i], vv[i]);
+    step(pp[i], gg[i], mm[i], vv[i], root[i]);
+    topM = fmaxf(topM, fmaxf(fabsf(mm[i].x), fabsf(mm[i].y)));
+    topV = fmaxf(topV, fmaxf(root[i].x, root[i].y));
+  }
+  put<kVector>(static_cast<T*>(t.p), e, end, rounded<T>(pp));
+  if (t.master) put<kVector>(t.master, e, end, rounded<float>(pp));
+  warpTops(topM, topV);
+  // below 1e-30 a block is held as zeros: the factor back would leave the range
+  const float toM = topM >= 1e-30f ? kE4m3Max / topM : 0.f, toV = topV >= 1e-30f ? kE4m3Max / topV : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    mm[i] = mul2(mm[i], {toM, toM});
+    root[i] = mul2(root[i], {toV, toV});
+    // 2^-9 is the smallest code above zero
+    if (root[i].x > 0.f) root[i].x = fmaxf(root[i].x, 0.001953125f);
+    if (root[i].y > 0.f) root[i].y = fmaxf(root[i].y, 0.001953125f);
+  }
+  put<kVector>(static_cast<__nv_fp8_storage_t*>(t.m), e, end, encode(mm));
+  put<kVector>(static_cast<__nv_fp8_storage_t*>(t.v), e, end, encode(root));
+  if (lane == 0) {
+    t.m_scale[b / TCPXB_ADAMW_BLOCK] = topM >= 1e-30f ? topM / kE4m3Max : 0.f;
+    t.v_scale[b / TCPXB_ADAMW_BLOCK] = topV >= 1e-30f ? topV / kE4m3Max : 0.f;
+  }
+}
+
+template <class T, class L, bool kSmall, int kBlocks = kSmall ? 3 : 4> __global__ void __launch_bounds__(kThreads, kBlocks) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
+  const int i = tensorOf(l, blockIdx.x);
+  const tcpxbAdamwTensor t = l.t[i];
+  const long long begin = (long long)(blockIdx.x - (i ? l.end[i - 1] : 0)) * l.chunk;
+  const long long end = min((long long)t.n, begin + l.chunk);
+  const auto* s = static_cast<const Scratch*>(a.scratch);
+  const Step step{float(a.beta1), float(a.beta2), float(1 - a.beta1), float(1 - a.beta2), float(a.eps), float(1 - a.lr * a.weight_decay),
+                  s->rates[l.first + i].stepSize, s->rates[l.first + i].rootCorrection, s->coef};
+  const bool vectors = aligned(t.p) && aligned(t.g) && aligned(t.m) && aligned(t.v) && aligned(t.master);
+  if constexpr (!kSmall) {
+    const long long whole = vectors ? begin + (end - begin) / 8 * 8 : begin;
+    stepVectors<T>(t, step, begin, whole);
+    stepElements<T>(t, step, whole, end);
+  } else {
+    constexpr int kStride = kThreads / 32 * TCPXB_ADAMW_BLOCK;
+    long long b = begin + threadIdx.x / 32 * TCPXB_ADAMW_BLOCK;
+    Raw<T> r;
+    const long long whole = vectors ? end - TCPXB_ADAMW_BLOCK : begin - 1;  // last place where a vector block begins
+    if (b <= whole) fetch<true>(r, t, b, end);
+#pragma unroll 1
+    for (; b <= whole; b += kStride) {
+      Raw<T> next;
+      if (b + kStride <= whole) fetch<true>(next, t, b + kStride, end);
+      stepBlock<true>(r, t, step, b, end);
+      r = next;
+    }
+#pragma unroll 1
+    for (; b < end; b += kStride) {
+      fetch<false>(r, t, b, end);
+      stepBlock<false>(r, t, step, b, end);
+    }
+  }
+}
+
 template <class T, class L> __global__ void __launch_bounds__(kThreads) squaresKernel(const __grid_constant__ L l, double* partial) {
   const int i = tensorOf(l, blockIdx.x);
-  const long long begin = (long long)(blockIdx.x - (i ? l.end[i - 1] : 0)) * kChunk;
-  const long long end = min((long long)l.t[i].n, begin + kChunk);
+  const long long begin = (long long)(blockIdx.x - (i ? l.end[i - 1] : 0)) * l.chunk;
+  const long long end = min((long long)l.t[i].n, begin + l.chunk);
   const T* g = static_cast<const T*>(l.t[i].g);
-  float sum = 0.f;  // 32 squares a thread
-  for (long long e = begin + threadIdx.x; e < end; e += kThreads) {
-    const float x = toFloat(g[e]);
-    sum += x * x;
+  // eight squares in 32 bits, those sums in 64: what rounding is left averages out
+  double sum = 0;
+  const long long whole = aligned(g) ? begin + (end - begin) / 8 * 8 : begin;
+#pragma unroll 1
+  for (long long e0 = begin + threadIdx.x * 8; e0 < whole; e0 += kThreads * 32) {
+    Vec8<T> raw[4] = {};
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (e0 + u * kThreads * 8 < whole) raw[u] = *reinterpret_cast<const Vec8<T>*>(g + e0 + u * kThreads * 8);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      float2 x[4], y = {0.f, 0.f};
+      pairs(raw[u], x);
+#pragma unroll
+      for (int k = 0; k < 4; k++) y = fma2(x[k], x[k], y);
+      sum += y.x + y.y;
+    }
+  }
+#pragma unroll 1
+  for (long long e0 = whole + threadIdx.x; e0 < end; e0 += kThreads * 8) {
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const long long e = e0 + k * kThreads;
+      const float x = e < end ? toFloat(g[e]) : 0.f;
+      y += x * x;
+    }
+    sum += y;
   }
   const double all = blockSum(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = all;
 }
 
-__global__ void normKernel(const double* partial, long long n, float* norm) {
-  double sum = 0;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) sum += partial[i];
-  sum = blockSum(sum);
-  if (threadIdx.x == 0) *norm = float(sqrt(sum));
+__global__ void __launch_bounds__(1024) normKernel(const double* partial, long long n, float* norm) {
+  const float x = rootOfSum(partial, n);
+  if (threadIdx.x == 0) *norm = x;
 }
 
-long long chunksOf(const tcpxbAdamwTensor& t) { return (t.n + kChunk - 1) / kChunk; }
+int chunkOf(const tcpxbAdamwTensor* tensors, int count) {
+  long long all = 0;
+  for (int i = 0; i < count; i++) all += tensors[i].n;
+  return all < kManyElements ? kShortChunk : kLongChunk;
+}
+long long chunksOf(const tcpxbAdamwTensor& t, int chunk) { return (t.n + chunk - 1) / chunk; }
+size_t ratesBytes(int count) { return sizeof(Scratch) + sizeof(Rates) * size_t(count); }
+size_t partialBytes(const tcpxbAdamwTensor* tensors, int count) {
+  long long chunks = 0;
+  if (tensors) {
+    const int chunk = chunkOf(tensors, count);
+    for (int i = 0; i < count; i++) chunks += chunksOf(tensors[i], chunk);
+  }
+  return sizeof(double) * size_t(chunks + 1);
+}
 
 // Calls f(list, chunks) for the tensors in lists of at most N, leaving out those without elements.
 template <class L, int N, class F> int inLists(const tcpxbAdamwTensor* tensors, int count, F f) {
   static thread_local L l;
+  l.chunk = chunkOf(tensors, count);
   for (int first = 0; first < count;) {
     long long chunks = 0;
     l.count = 0, l.first = first;
     int i = first;
-    for (; i < count && l.count < N && chunks + chunksOf(tensors[i]) < (1ll << 31); i++) {
+    for (; i < count && l.count < N && chunks + chunksOf(tensors[i], l.chunk) < (1ll << 31); i++) {
       l.t[l.count] = tensors[i];
-      chunks += chunksOf(tensors[i]);
+      chunks += chunksOf(tensors[i], l.chunk);
       l.end[l.count++] = unsigned(chunks);
     }
     if (const int rc = f(l, chunks)) return rc;
@@ -217,10 +407,27 @@ int check(const tcpxbAdamwTensor* t, int count, int dtype, bool step, int bits) 
   return TCPXB_T_OK;
 }
 
-template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw& a, cudaStream_t s) {
+// Sums of squares of all chunks into `partial`; their number in *done.
+template <class T> int squares(const tcpxbAdamwTensor* tensors, int count, double* partial, long long* done, cudaStream_t s) {
   return inLists(tensors, count, [&](const auto& l, long long chunks) {
     using L = std::decay_t<decltype(l)>;
-    prepareKernel<<<1, l.count <= 128 ? 128 : 384, 0, s>>>(l, a);
+    if (!chunks) return int(TCPXB_T_OK);
+    squaresKernel<T, L><<<unsigned(chunks), kThreads, 0, s>>>(l, partial + *done);
+    *done += chunks;
+    return launched("gradient norm");
+  });
+}
+
+template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw& a, cudaStream_t s) {
+  double* partial = nullptr;
+  long long partials = 0;
+  if (a.compute_norm) {
+    partial = reinterpret_cast<double*>(static_cast<char*>(a.scratch) + ratesBytes(count));
+    if (const int rc = squares<T>(tensors, count, partial, &partials, s)) return rc;
+  }
+  return inLists(tensors, count, [&](const auto& l, long long chunks) {
+    using L = std::decay_t<decltype(l)>;
+    prepareKernel<<<1, partials > 128 ? 512 : l.count <= 128 ? 128 : 384, 0, s>>>(l, a, partial, partials);
     if (const int rc = launched("adamw, rates")) return rc;
     if (!chunks) return int(TCPXB_T_OK);
     if (a.state_bits == 8) stepKernel<T, L, true><<<unsigned(chunks), kThreads, 0, s>>>(l, a);
@@ -229,17 +436,10 @@ template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tc
   });
 }
 
-template <class T> int squares(const tcpxbAdamwTensor* tensors, int count, float* norm, double* partial, cudaStream_t s) {
+template <class T> int gradNorm(const tcpxbAdamwTensor* tensors, int count, float* out, double* partial, cudaStream_t s) {
   long long done = 0;
-  const int rc = inLists(tensors, count, [&](const auto& l, long long chunks) {
-    using L = std::decay_t<decltype(l)>;
-    if (!chunks) return int(TCPXB_T_OK);
-    squaresKernel<T, L><<<unsigned(chunks), kThreads, 0, s>>>(l, partial + done);
-    done += chunks;
-    return launched("gradient norm");
-  });
-  if (rc) return rc;
-  normKernel<<<1, 1024, 0, s>>>(partial, done, norm);
+  if (const int rc = squares<T>(tensors, count, partial, &done, s)) return rc;
+  normKernel<<<1, 1024, 0, s>>>(partial, done, out);
   return launched("gradient norm, sum");
 }
 
@@ -248,10 +448,13 @@ template <class T> int squares(const tcpxbAdamwTensor* tensors, int count, float
 
 using namespace tcpxb_train;
 
-extern "C" size_t tcpxb_adamw_scratch_bytes(int count) { return sizeof(Scratch) + sizeof(Rates) * size_t(count > 0 ? count : 0); }
+extern "C" size_t tcpxb_adamw_scratch_bytes(const tcpxbAdamwTensor* tensors, int count) {
+  return count > 0 ? ratesBytes(count) + partialBytes(tensors, count) : 0;
+}
 
 extern "C" int tcpxb_adamw_step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw* a, void* stream) {
-  if (!a || !a->scratch) return fail(TCPXB_T_INVALID, "null argument");
+  if (!a || !a->scratch || reinterpret_cast<uintptr_t>(a->scratch) % 8 || (a->compute_norm && !a->grad_norm))
+    return fail(TCPXB_T_INVALID, "the arguments, the scratch or the norm are null");
   if (a->state_bits != 8 && a->state_bits != 32) return fail(TCPXB_T_INVALID, "states have 8 or 32 bits, not %d", a->state_bits);
   if (const int rc = check(tensors, count, a->dtype, true, a->state_bits)) return rc;
   auto s = static_cast<cudaStream_t>(stream);
@@ -260,18 +463,14 @@ extern "C" int tcpxb_adamw_step(const tcpxbAdamwTensor* tensors, int count, cons
   return step<float>(tensors, count, *a, s);
 }
 
-extern "C" size_t tcpxb_grad_norm_scratch_bytes(const tcpxbAdamwTensor* tensors, int count) {
-  long long chunks = 0;
-  for (int i = 0; tensors && i < count; i++) chunks += chunksOf(tensors[i]);
-  return sizeof(double) * size_t(chunks + 1);
-}
+extern "C" size_t tcpxb_grad_norm_scratch_bytes(const tcpxbAdamwTensor* tensors, int count) { return partialBytes(tensors, count); }
 
 extern "C" int tcpxb_grad_norm(const tcpxbAdamwTensor* tensors, int count, int dtype, float* norm, void* scratch, void* stream) {
   if (!norm || !scratch) return fail(TCPXB_T_INVALID, "null argument");
   if (const int rc = check(tensors, count, dtype, false, 32)) return rc;
   auto s = static_cast<cudaStream_t>(stream);
   auto* partial = static_cast<double*>(scratch);
-  if (dtype == TCPXB_T_BF16) return squares<__nv_bfloat16>(tensors, count, norm, partial, s);
-  if (dtype == TCPXB_T_F16) return squares<__half>(tensors, count, norm, partial, s);
-  return squares<float>(tensors, count, norm, partial, s);
+  if (dtype == TCPXB_T_BF16) return gradNorm<__nv_bfloat16>(tensors, count, norm, partial, s);
+  if (dtype == TCPXB_T_F16) return gradNorm<__half>(tensors, count, norm, partial, s);
+  return gradNorm<float>(tensors, count, norm, partial, s);
 }

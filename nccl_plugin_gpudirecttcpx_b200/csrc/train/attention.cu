@@ -19,6 +19,7 @@
 //
 // Probabilities and score gradients are rounded to the inputs' type because the matrix units take
 // operands of one type; sums, statistics and everything else are 32-bit.
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -30,7 +31,9 @@ namespace {
 constexpr int kMaxD = 128;
 constexpr int kTile = 128;
 constexpr int kComputeWarps = 8, kLoadWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;  // the last two warps only complete a warpgroup
+// 384 threads get 168 registers each at launch: 2 x 128 x 208 + 128 x 80 is less than that
+constexpr int kComputeRegs = 208, kOtherRegs = 80;
 constexpr int kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -159,6 +162,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
   const uint32_t tmem = uniform(sh.tmem);
 
   if (warp == kLoadWarp) {
+    fewerRegisters<kOtherRegs>();
     if (lane == 0) {
       for (int t = 0; t < 2; t++)
         if (n[t]) {
@@ -174,6 +178,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    fewerRegisters<kOtherRegs>();
     const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
     const uint32_t scores = mmaShape<T>(kTile, false), values = mmaShape<T>(steps * 16, true);
@@ -211,7 +216,8 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
       }
       __syncwarp();
     }
-  } else {
+  } else if (warp < kComputeWarps) {
+    moreRegisters<kComputeRegs>();
     const int t = warp / 4, row = warp % 4 * 32 + lane, i = q0 + t * kTile + row;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const uint32_t s = tmem + t * kTile + lanes, o = tmem + 2 * kTile + t * kMaxD + lanes;
@@ -283,6 +289,8 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
     const float by = seen > 0 ? 1.f / sum : 0.f;
     if (q0 + t * kTile < a.sq) storeRow(static_cast<T*>(a.o) + at, live, o, 0, kMaxD, a.d, by, n[t] > 0);
     if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
+  } else {
+    fewerRegisters<kOtherRegs>();
   }
   finish(a, tmem, dead);
 }
@@ -291,7 +299,9 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
 // A block owns 128 queries and goes through the key tiles:  S = Q K^T, dP = dout V^T, then
 // dq += dS K.  Two buffers of scores: the next tile's exponentials start while the matrix units
 // still work on dP and dq of this one.  Both halves of the warps hold all rows, 64 keys each.
-// D_i is computed here, on the way in, and left for the other kernel.
+// D_i is computed here and left for the other kernel: on the way in from dout and out; where all
+// keys of the block lie in one tile, as sum_j P_ij dP_ij, which it equals.  In so short a row the
+// rounding of out would be most of the gradients' error, and there the whole row is at hand.
 template <class T, int P> struct Queries {
   static constexpr int kKSlots = 3, kVSlots = 2;
   static constexpr uint32_t kTileBytes = P * kPanelBytes;
@@ -328,6 +338,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
   const uint32_t tmem = uniform(*tmemAt), dp = tmem + 2 * kTile, dq = tmem + 3 * kTile;
 
   if (warp == kLoadWarp) {
+    fewerRegisters<kOtherRegs>();
     if (lane == 0 && n) {
       barExpect(bar(F::kQFull), 2 * F::kTileBytes);
       loadTile<P>(qTile, &a.q, bar(F::kQFull), q0, h, b);
@@ -344,6 +355,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    fewerRegisters<kOtherRegs>();
     const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
     const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
@@ -385,7 +397,8 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
         __syncwarp();
       }
     }
-  } else {
+  } else if (warp < kComputeWarps) {
+    moreRegisters<kComputeRegs>();
     const int half = warp / 4, row = warp % 4 * 32 + lane, i = q0 + row;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool live = i < a.sq;
@@ -393,7 +406,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
     const float c = a.scale * kLog2e;
     if (half == 0) {
       float sum = 0.f;
-      if (live) {
+      if (live && n > 1) {
         const T *o = static_cast<const T*>(a.out) + at, *g = static_cast<const T*>(a.doutPtr) + b * a.doutB + i * a.doutS + h * a.doutH;
         for (int k = 0; k < a.d; k += 8) {
           float x[8], y[8];
@@ -402,12 +415,12 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
 #pragma unroll
           for (int u = 0; u < 8; u++) sum += x[u] * y[u];
         }
-        a.delta[stat] = sum;
       }
+      if (live && n != 1) a.delta[stat] = sum;
       deltas[row] = sum;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float delta = deltas[row];
+    float delta = deltas[row];
     // a row that sees nothing, or lies behind the last query, has no probabilities
     float l = live ? a.lse[stat] * -kLog2e : -INFINITY;
     if (l == INFINITY) l = -INFINITY;
@@ -432,6 +445,23 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       tmemLoad32(dp + half * 64 + lanes + 32, y + 32);
       tmemWaitLoad();
       const int left = seen - j * kTile - half * 64;
+      if (n == 1) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 64; k++)
+          if (k < left) sum += __uint_as_float(x[k]) * __uint_as_float(y[k]);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // everybody has read the zeros
+        if (half) deltas[row] = sum;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (!half) {
+          sum += deltas[row];
+          if (live) a.delta[stat] = sum;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (!half) deltas[row] = sum;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        delta = deltas[row];
+      }
       const auto gradients = [&](auto masked) {
 #pragma unroll
         for (int k = 0; k < 64; k += 2) {
@@ -457,6 +487,8 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       tcAfter();
     }
     storeRow(static_cast<T*>(a.dq) + at, live, dq + lanes, half * 64, half * 64 + 64, a.d, seen > 0 ? a.scale : 0.f, n > 0);
+  } else {
+    fewerRegisters<kOtherRegs>();
   }
   finish(a, tmem, dead);
 }
@@ -500,13 +532,14 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
   const uint32_t tmem = uniform(sh.tmem), s = tmem, dp = tmem + kTile, dv = tmem + 2 * kTile, dk = tmem + 3 * kTile;
 
   if (warp == kLoadWarp) {
+    fewerRegisters<kOtherRegs>();
     if (lane == 0 && n) {
       barExpect(bar(F::kKvFull), 2 * F::kTileBytes);
       loadTile<P>(kTileAt, &a.k, bar(F::kKvFull), j0, kv, b);
       loadTile<P>(vTileAt, &a.v, bar(F::kKvFull), j0, kv, b);
     }
-    for (int it = 0; it < n; it++) {
-      const int st = it % F::kStages, turn = it / F::kStages, h = kv * group + it / each, q0 = (first + it % each) * kTile;
+    for (int it = 0, h = kv * group, qt = 0; it < n; it++) {
+      const int st = it % F::kStages, turn = it / F::kStages, q0 = (first + qt) * kTile;
       const long long stat = ((long long)b * a.heads + h) * a.sq;
       float l[4], d[4];
 #pragma unroll
@@ -526,9 +559,11 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
 #pragma unroll
       for (int u = 0; u < 4; u++) sh.stats[st][0][u * 32 + lane] = l[u], sh.stats[st][1][u * 32 + lane] = d[u];
       barArrive(bar(F::kFull + st));
+      if (++qt == each) qt = 0, h++;
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    fewerRegisters<kOtherRegs>();
     const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
     const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
@@ -565,13 +600,15 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
         __syncwarp();
       }
     }
-  } else {
+  } else if (warp < kComputeWarps) {
+    moreRegisters<kComputeRegs>();
     const int half = warp / 4, row = warp % 4 * 32 + lane, j = j0 + row;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool counts = j < keys;
     const float c = a.scale * kLog2e;
-    for (int it = 0; it < n; it++) {
-      const int st = it % F::kStages, q0 = (first + it % each) * kTile;
+    for (int it = 0, qt = 0; it < n; it++) {
+      const int st = it % F::kStages, q0 = (first + qt) * kTile;
+      if (++qt == each) qt = 0;
       const float4* l = reinterpret_cast<const float4*>(sh.stats[st][0] + half * 64);
       const float4* d = reinterpret_cast<const float4*>(sh.stats[st][1] + half * 64);
       // first query of this half that sees the row's key
@@ -649,6 +686,8 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
     const long long at = (((long long)b * a.sk + j) * a.kvHeads + kv) * a.d;
     storeRow(static_cast<T*>(a.dv) + at, live, dv + lanes, half * 64, half * 64 + 64, a.d, counts ? 1.f : 0.f, n > 0);
     storeRow(static_cast<T*>(a.dk) + at, live, dk + lanes, half * 64, half * 64 + 64, a.d, counts ? a.scale : 0.f, n > 0);
+  } else {
+    fewerRegisters<kOtherRegs>();
   }
   finish(a, tmem, dead);
 }
@@ -706,11 +745,6 @@ int check(const tcpxbAttention* a, bool backward) {
 }
 
 int makeArgs(const tcpxbAttention& a, bool backward, Args* x) {
-  // a thread that only autograd has used so far knows its device but has no context yet, which the driver's call needs
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaSetDevice(device);
-  if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "attention: %s", cudaGetErrorString(e));
   int rc = makeMap(&x->q, "q", a.q, a.b, a.sq, a.heads, a.d, a.dtype);
   if (!rc) rc = makeMap(&x->k, "k", a.k, a.b, a.sk, a.kv_heads, a.d, a.dtype);
   if (!rc) rc = makeMap(&x->v, "v", a.v, a.b, a.sk, a.kv_heads, a.d, a.dtype);
@@ -725,25 +759,37 @@ int makeArgs(const tcpxbAttention& a, bool backward, Args* x) {
   return TCPXB_T_OK;
 }
 
-int launch(void (*kernel)(Args), dim3 grid, size_t shared, const Args& a, cudaStream_t s, const char* what) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
-  if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
-  kernel<<<grid, kThreads, shared, s>>>(a);
+// Once for each kernel and device the block's shared memory is allowed; more than 64 devices would only ask again.
+template <void (*kKernel)(Args)> int launch(dim3 grid, size_t shared, const Args& a, int device, cudaStream_t s, const char* what) {
+  static std::atomic<uint64_t> allowed{0};
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+    if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  kKernel<<<grid, kThreads, shared, s>>>(a);
   return launched(what);
 }
 
 template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaStream_t s) {
+  // a thread that only autograd has used so far knows its device but has no context yet, which the driver's call needs
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaSetDevice(device);
+  if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "attention: %s", cudaGetErrorString(e));
   Args x;
   if (const int rc = makeArgs(a, backward, &x)) return rc;
   if (!backward) {
     if (!a.b || !a.sq) return TCPXB_T_OK;
-    return launch(forwardKernel<T, P>, dim3(a.heads, a.b, (a.sq + 2 * kTile - 1) / (2 * kTile)), Forward<T, P>::kShared, x, s, "attention forward");
+    return launch<forwardKernel<T, P>>(dim3(a.heads, a.b, (a.sq + 2 * kTile - 1) / (2 * kTile)), Forward<T, P>::kShared, x, device, s, "attention forward");
   }
   if (a.b && a.sq)
-    if (const int rc = launch(queryKernel<T, P>, dim3(a.heads, a.b, (a.sq + kTile - 1) / kTile), Queries<T, P>::kShared, x, s, "attention backward, queries"))
+    if (const int rc = launch<queryKernel<T, P>>(dim3(a.heads, a.b, (a.sq + kTile - 1) / kTile), Queries<T, P>::kShared, x, device, s,
+                                                 "attention backward, queries"))
       return rc;
   if (!a.b || !a.sk) return TCPXB_T_OK;
-  return launch(keyKernel<T, P>, dim3(a.kv_heads, a.b, (a.sk + kTile - 1) / kTile), Keys<T, P>::kShared, x, s, "attention backward, keys");
+  return launch<keyKernel<T, P>>(dim3(a.kv_heads, a.b, (a.sk + kTile - 1) / kTile), Keys<T, P>::kShared, x, device, s, "attention backward, keys");
 }
 
 int dispatch(const tcpxbAttention* a, bool backward, void* stream) {

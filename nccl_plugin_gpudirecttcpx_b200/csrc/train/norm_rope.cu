@@ -6,50 +6,69 @@
 //
 // Memory-bound: every element is read and written once.  A head's row is held by a group of
 // lanes, eight elements each (16 bytes of a 16-bit type), so the norm's sum is a few shuffles
-// and each lane owns whole pairs.  All sums are 32-bit; the result is rounded once.
+// and each lane owns whole pairs.  A block works on queries or on keys, and a warp takes a few
+// heads of one token at a time: their loads are all in flight before the first is used, and the
+// token's angles and the weight are read once for them.  All sums are 32-bit; the result is
+// rounded once.
 #include "common.h"
 
 namespace tcpxb_train {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxBlocks = 148 * 4;  // also the rows of the partial sums of dw
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxBlocks = 148 * 4;  // of the backward pass: the rows of the partial sums of dw
 constexpr int kMaxD = 256;
 
-struct Row {
-  long long token;
-  int head;
-  bool isQ;
+// Rows that a lane group has in flight.
+template <class T> constexpr int kRows = sizeof(T) == 2 ? 4 : 2;
+
+// What a launch does to queries, and to keys.
+struct Side {
+  tcpxbHeads x, dy;
+  const void* w;
+  void* out;
+  int heads;
+  unsigned parts, units;  // warps' shares of a token, and of all tokens
+};
+struct Job {
+  Side side[2];  // queries, keys
+  const float *cos, *sin;
+  const int64_t* pos;
+  float* partial;
+  unsigned s, qBlocks, kBlocks;
+  int d, positions;
+  float eps, perD;
 };
 
-__device__ __forceinline__ Row rowOf(const tcpxbNormRope& a, long long r) {
-  const int all = a.heads + a.kv_heads;
-  Row x;
-  x.token = r / all;
-  x.head = int(r % all);
-  x.isQ = x.head < a.heads;
-  if (!x.isQ) x.head -= a.heads;
+// The token and the first of the heads that a warp does next.
+struct Unit {
+  unsigned token, batch, at;  // at: the token's number in its batch
+  int head;
+};
+template <class T, int G> __device__ __forceinline__ Unit unitOf(const Job& j, const Side& side, unsigned u) {
+  Unit x;
+  x.token = u / side.parts;
+  x.head = int(u - x.token * side.parts) * (32 / G * kRows<T>) + int(threadIdx.x % 32 / G);
+  x.batch = x.token / j.s;
+  x.at = x.token - x.batch * j.s;
   return x;
 }
-
-template <class T> __device__ __forceinline__ const T* input(const tcpxbHeads& x, const tcpxbNormRope& a, const Row& r) {
-  return static_cast<const T*>(x.ptr) + r.token / a.s * x.stride_b + r.token % a.s * x.stride_s + r.head * x.stride_h;
-}
-template <class T> __device__ __forceinline__ T* output(void* q, void* k, const tcpxbNormRope& a, const Row& r) {
-  return r.isQ ? static_cast<T*>(q) + (r.token * a.heads + r.head) * a.d : static_cast<T*>(k) + (r.token * a.kv_heads + r.head) * a.d;
+template <class T> __device__ __forceinline__ const T* input(const tcpxbHeads& x, const Unit& u, int col) {
+  return static_cast<const T*>(x.ptr) + u.batch * x.stride_b + u.at * x.stride_s + u.head * x.stride_h + col;
 }
 
 // Four angles of a lane's eight elements; a token outside the tables has none.
-__device__ __forceinline__ void angles(const tcpxbNormRope& a, long long token, int col, float (&c)[4], float (&s)[4]) {
-  const long long p = a.pos ? a.pos[token] : token % a.s;
-  if (p < 0 || p >= a.positions) {
+__device__ __forceinline__ void angles(const Job& j, const Unit& u, int col, float (&c)[4], float (&s)[4]) {
+  const long long p = j.pos ? j.pos[u.token] : u.at;
+  if (p < 0 || p >= j.positions) {
 #pragma unroll
     for (int i = 0; i < 4; i++) c[i] = s[i] = NAN;
     return;
   }
-  const long long at = p * (a.d / 2) + col / 2;
-#pragma unroll
-  for (int i = 0; i < 4; i++) c[i] = a.cos[at + i], s[i] = a.sin[at + i];
+  const long long at = p * (j.d / 2) + col / 2;  // a multiple of four
+  const float4 x = *reinterpret_cast<const float4*>(j.cos + at), y = *reinterpret_cast<const float4*>(j.sin + at);
+  c[0] = x.x, c[1] = x.y, c[2] = x.z, c[3] = x.w;
+  s[0] = y.x, s[1] = y.y, s[2] = y.z, s[3] = y.w;
 }
 
 template <int G> __device__ __forceinline__ float groupSum(float x) {
@@ -58,112 +77,145 @@ template <int G> __device__ __forceinline__ float groupSum(float x) {
   return x;
 }
 
-template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads) forwardKernel(const tcpxbNormRope a) {
-  const long long rows = (long long)a.b * a.s * (a.heads + a.kv_heads);
-  const int lane = threadIdx.x % G, col = lane * 8;
-  const bool on = col < a.d;
-  float w[2][8] = {};
-  if (kNorm && on) {
-    load8(static_cast<const T*>(a.wq) + col, w[0]);
-    load8(static_cast<const T*>(a.wk) + col, w[1]);
+// A lane's eight elements as four pairs.
+template <class T> __device__ __forceinline__ void pairs(const Vec8<T>& v, float2 (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) f[i] = {toFloat(v.x[2 * i]), toFloat(v.x[2 * i + 1])};
+}
+template <class T> __device__ __forceinline__ void store(T* p, const float2 (&f)[4]) {
+  Vec8<T> v;
+#pragma unroll
+  for (int i = 0; i < 4; i++) v.x[2 * i] = fromFloat<T>(f[i].x), v.x[2 * i + 1] = fromFloat<T>(f[i].y);
+  *reinterpret_cast<Vec8<T>*>(p) = v;
+}
+__device__ __forceinline__ float sum(const float2 (&a)[4], const float2 (&b)[4]) {
+  float2 s = mul2(a[0], b[0]);
+#pragma unroll
+  for (int i = 1; i < 4; i++) s = fma2(a[i], b[i], s);
+  return s.x + s.y;
+}
+
+template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads) forwardKernel(const __grid_constant__ Job j) {
+  const bool keys = blockIdx.x >= j.qBlocks;
+  const Side& side = j.side[keys];
+  const unsigned unit = (blockIdx.x - (keys ? j.qBlocks : 0)) * kWarps + threadIdx.x / 32;
+  if (unit >= side.units) return;
+  const int col = threadIdx.x % G * 8;
+  const Unit u = unitOf<T, G>(j, side, unit);
+  const bool on = col < j.d;
+  const T* x = input<T>(side.x, u, col);
+  T* y = static_cast<T*>(side.out) + ((long long)u.token * side.heads + u.head) * j.d + col;
+  Vec8<T> raw[kRows<T>] = {};
+#pragma unroll
+  for (int i = 0; i < kRows<T>; i++)
+    if (on && u.head + i * (32 / G) < side.heads) raw[i] = *reinterpret_cast<const Vec8<T>*>(x + i * (32 / G) * side.x.stride_h);
+  float c[4] = {}, s[4] = {};
+  float2 w[4] = {};
+  if (on) {
+    angles(j, u, col, c, s);
+    if (kNorm) pairs(*reinterpret_cast<const Vec8<T>*>(static_cast<const T*>(side.w) + col), w);
   }
-  // the groups of a warp leave the loop together, so the shuffles are whole
-  const int perWarp = 32 / G;
-  const long long step = (long long)gridDim.x * (kThreads / G);
-  for (long long base = (long long)blockIdx.x * (kThreads / G) + threadIdx.x / 32 * perWarp; base < rows; base += step) {
-    const long long r = base + threadIdx.x % 32 / G;
-    const bool live = r < rows && on;
-    const Row at = rowOf(a, r);
-    float x[8] = {}, c[4], s[4];
-    if (live) load8(input<T>(at.isQ ? a.q : a.k, a, at) + col, x);
+#pragma unroll
+  for (int i = 0; i < kRows<T>; i++) {
+    float2 f[4];
+    pairs(raw[i], f);
     if (kNorm) {
-      float sq = 0.f;
+      const float r = rsqrtf(groupSum<G>(sum(f, f)) * j.perD + j.eps);
 #pragma unroll
-      for (int i = 0; i < 8; i++) sq += x[i] * x[i];
-      const float inv = rsqrtf(groupSum<G>(sq) / a.d + a.eps);
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] *= inv * (at.isQ ? w[0][i] : w[1][i]);
+      for (int k = 0; k < 4; k++) f[k] = mul2(mul2(f[k], {r, r}), w[k]);
     }
-    if (!live) continue;
-    angles(a, at.token, col, c, s);
-    float y[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      y[2 * i] = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
-      y[2 * i + 1] = x[2 * i] * s[i] + x[2 * i + 1] * c[i];
-    }
-    store8(output<T>(a.q_out, a.k_out, a, at) + col, y);
+    for (int k = 0; k < 4; k++) f[k] = {f[k].x * c[k] - f[k].y * s[k], f[k].x * s[k] + f[k].y * c[k]};
+    if (on && u.head + i * (32 / G) < side.heads) store(y + i * (32 / G) * j.d, f);
   }
 }
 
-template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads) backwardKernel(const tcpxbNormRope a) {
-  const long long rows = (long long)a.b * a.s * (a.heads + a.kv_heads);
-  const int lane = threadIdx.x % G, col = lane * 8;
-  const bool on = col < a.d;
-  float w[2][8] = {}, dw[2][8] = {};
-  if (kNorm && on) {
-    load8(static_cast<const T*>(a.wq) + col, w[0]);
-    load8(static_cast<const T*>(a.wk) + col, w[1]);
-  }
-  const int perWarp = 32 / G;
-  const long long step = (long long)gridDim.x * (kThreads / G);
-  for (long long base = (long long)blockIdx.x * (kThreads / G) + threadIdx.x / 32 * perWarp; base < rows; base += step) {
-    const long long r = base + threadIdx.x % 32 / G;
-    const bool live = r < rows && on;
-    const Row at = rowOf(a, r);
-    float dy[8] = {}, dn[8] = {}, x[8] = {}, c[4], s[4];
-    if (live) {
-      load8(input<T>(at.isQ ? a.dq_out : a.dk_out, a, at) + col, dy);
-      if (kNorm) load8(input<T>(at.isQ ? a.q : a.k, a, at) + col, x);
-      angles(a, at.token, col, c, s);
+// A few rows of a block's dw are in its lanes at the end: of queries in the first qBlocks, else of keys.
+template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads, 2) backwardKernel(const __grid_constant__ Job j) {
+  const bool keys = blockIdx.x >= j.qBlocks;
+  const Side& side = j.side[keys];
+  const unsigned block = blockIdx.x - (keys ? j.qBlocks : 0), blocks = keys ? j.kBlocks : j.qBlocks;
+  const int col = threadIdx.x % G * 8;
+  const bool on = col < j.d;
+  float2 w[4] = {}, dw[4] = {};
+  if (kNorm && on) pairs(*reinterpret_cast<const Vec8<T>*>(static_cast<const T*>(side.w) + col), w);
+  for (unsigned unit = block * kWarps + threadIdx.x / 32; unit < side.units; unit += blocks * kWarps) {
+    const Unit u = unitOf<T, G>(j, side, unit);
+    const T *x = input<T>(side.x, u, col), *dy = input<T>(side.dy, u, col);
+    T* dx = static_cast<T*>(side.out) + ((long long)u.token * side.heads + u.head) * j.d + col;
+    Vec8<T> rawX[kRows<T>] = {}, rawY[kRows<T>] = {};
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        dn[2 * i] = dy[2 * i] * c[i] + dy[2 * i + 1] * s[i];
-        dn[2 * i + 1] = dy[2 * i + 1] * c[i] - dy[2 * i] * s[i];
-      }
+    for (int i = 0; i < kRows<T>; i++) {
+      if (!on || u.head + i * (32 / G) >= side.heads) continue;
+      rawY[i] = *reinterpret_cast<const Vec8<T>*>(dy + i * (32 / G) * side.dy.stride_h);
+      if (kNorm) rawX[i] = *reinterpret_cast<const Vec8<T>*>(x + i * (32 / G) * side.x.stride_h);
     }
-    if (kNorm) {
-      float sq = 0.f, mix = 0.f;
+    float c[4] = {}, s[4] = {};
+    if (on) angles(j, u, col, c, s);
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        sq += x[i] * x[i];
-        mix += dn[i] * (at.isQ ? w[0][i] : w[1][i]) * x[i];
-      }
-      const float inv = rsqrtf(groupSum<G>(sq) / a.d + a.eps);
-      const float mean = groupSum<G>(mix) * inv / a.d;
+    for (int i = 0; i < kRows<T>; i++) {
+      const bool live = on && u.head + i * (32 / G) < side.heads;
+      float2 f[4];
+      pairs(rawY[i], f);
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float xh = x[i] * inv;
-        if (at.isQ) dw[0][i] += dn[i] * xh;
-        else dw[1][i] += dn[i] * xh;
-        dn[i] = inv * (dn[i] * (at.isQ ? w[0][i] : w[1][i]) - xh * mean);
+      for (int k = 0; k < 4; k++) f[k] = {f[k].x * c[k] + f[k].y * s[k], f[k].y * c[k] - f[k].x * s[k]};
+      if (kNorm) {
+        float2 xh[4], g[4];
+        pairs(rawX[i], xh);
+        const float r = rsqrtf(groupSum<G>(sum(xh, xh)) * j.perD + j.eps);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          xh[k] = mul2(xh[k], {r, r});
+          g[k] = mul2(f[k], w[k]);
+          if (live) dw[k] = fma2(f[k], xh[k], dw[k]);
+        }
+        const float mean = -groupSum<G>(sum(g, xh)) * j.perD;
+#pragma unroll
+        for (int k = 0; k < 4; k++) f[k] = mul2(fma2(xh[k], {mean, mean}, g[k]), {r, r});
       }
+      if (live) store(dx + i * (32 / G) * j.d, f);
     }
-    if (live) store8(output<T>(a.dq, a.dk, a, at) + col, dn);
   }
-  if (!kNorm) return;
-  // the block's groups, one after another in a fixed order
-  __shared__ float sums[2 * kMaxD];
-  for (int g = 0; g < kThreads / G; g++) {
-    if (threadIdx.x / G == g && on) {
+  if constexpr (kNorm) {
+    // the groups of a warp by shuffles, then the block's warps, in a fixed order
+    __shared__ float sums[kWarps][kMaxD];
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+    for (int k = 0; k < 8; k++) {
+      float x = k % 2 ? dw[k / 2].y : dw[k / 2].x;
 #pragma unroll
-        for (int i = 0; i < 8; i++) sums[t * kMaxD + col + i] = (g ? sums[t * kMaxD + col + i] : 0.f) + dw[t][i];
+      for (int o = 16; o; o >>= 1)
+        if (o >= G) x += __shfl_xor_sync(0xffffffffu, x, o);
+      if (threadIdx.x % 32 < G && on) sums[threadIdx.x / 32][col + k] = x;
     }
     __syncthreads();
+    for (int i = threadIdx.x; i < j.d; i += kThreads) {
+      float x = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; k++) x += sums[k][i];
+      j.partial[(long long)blockIdx.x * j.d + i] = x;
+    }
   }
-  for (int i = threadIdx.x; i < 2 * a.d; i += kThreads)
-    a.partial[(long long)blockIdx.x * 2 * a.d + i] = sums[i / a.d * kMaxD + i % a.d];
 }
 
-// dw: the blocks' partial sums, in the order of the blocks.
-template <class T> __global__ void weightKernel(const tcpxbNormRope a, int blocks) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= 2 * a.d) return;
-  float sum = 0.f;
-  for (int b = 0; b < blocks; b++) sum += a.partial[(long long)b * 2 * a.d + i];
-  static_cast<T*>(i < a.d ? a.dwq : a.dwk)[i % a.d] = fromFloat<T>(sum);
+// dw: the blocks' partial sums.  A block has 32 columns of one weight, and 32 warps that each take
+// every 32nd row.
+template <class T> __global__ void __launch_bounds__(1024) weightKernel(const __grid_constant__ Job j, T* dwq, T* dwk) {
+  __shared__ float sums[32][33];
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32, i = blockIdx.x * 32 + x;
+  const unsigned first = blockIdx.y ? j.qBlocks : 0, end = blockIdx.y ? j.qBlocks + j.kBlocks : j.qBlocks;
+  float part = 0.f;
+  if (i < j.d) {
+#pragma unroll 4
+    for (unsigned b = first + y; b < end; b += 32) part += j.partial[(long long)b * j.d + i];
+  }
+  sums[y][x] = part;
+  __syncthreads();
+  // the sum of column y, taken by warp y
+  part = sums[x][y];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+  const int c = blockIdx.x * 32 + y;
+  if (x == 0 && c < j.d) (blockIdx.y ? dwk : dwq)[c] = fromFloat<T>(part);
 }
 
 int check(const tcpxbNormRope* a, bool backward) {
@@ -171,33 +223,55 @@ int check(const tcpxbNormRope* a, bool backward) {
   if (a->dtype != TCPXB_T_BF16 && a->dtype != TCPXB_T_F16 && a->dtype != TCPXB_T_F32) return fail(TCPXB_T_INVALID, "unknown type %d", a->dtype);
   if (a->b < 0 || a->s < 0 || a->heads < 1 || a->kv_heads < 1 || a->d < 8 || a->d > kMaxD || a->d % 8)
     return fail(TCPXB_T_INVALID, "bad shape: b %d s %d heads %d/%d d %d", a->b, a->s, a->heads, a->kv_heads, a->d);
+  if ((long long)a->b * a->s * ((long long)a->heads + a->kv_heads) >= 1ll << 31)
+    return fail(TCPXB_T_INVALID, "at most 2^31 - 1 rows: b %d s %d heads %d/%d", a->b, a->s, a->heads, a->kv_heads);
   if (!a->wq != !a->wk) return fail(TCPXB_T_INVALID, "weights for queries and keys come together");
+  if (backward && a->wq && (!a->dwq || !a->dwk || !a->partial)) return fail(TCPXB_T_INVALID, "a weight's gradient or the scratch is null");
   if ((long long)a->b * a->s == 0) return TCPXB_T_OK;
   const int es = a->dtype == TCPXB_T_F32 ? 4 : 2;
   if (!a->cos || !a->sin || (!a->pos && a->positions < a->s)) return fail(TCPXB_T_INVALID, "tables are missing or shorter than the sequence");
+  for (const void* p : {static_cast<const void*>(a->cos), static_cast<const void*>(a->sin), a->wq, a->wk})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return fail(TCPXB_T_INVALID, "a table or weight is off the 16-byte boundary");
   const bool needX = !backward || a->wq;
   if (needX && (!headsOk(a->q, es) || !headsOk(a->k, es))) return fail(TCPXB_T_INVALID, "q or k is null or off the 16-byte boundary");
   if (!backward && (!a->q_out || !a->k_out)) return fail(TCPXB_T_INVALID, "an output is null");
-  if (backward && (!headsOk(a->dq_out, es) || !headsOk(a->dk_out, es) || !a->dq || !a->dk || (a->wq && (!a->dwq || !a->dwk || !a->partial))))
-    return fail(TCPXB_T_INVALID, "a gradient or the scratch is null or off the 16-byte boundary");
+  if (backward && (!headsOk(a->dq_out, es) || !headsOk(a->dk_out, es) || !a->dq || !a->dk))
+    return fail(TCPXB_T_INVALID, "a gradient is null or off the 16-byte boundary");
   return TCPXB_T_OK;
 }
 
 template <class T, int G> int run(const tcpxbNormRope& a, bool backward, cudaStream_t s) {
-  const long long rows = (long long)a.b * a.s * (a.heads + a.kv_heads), perBlock = kThreads / G;
-  const int blocks = int(rows < kMaxBlocks * perBlock ? (rows + perBlock - 1) / perBlock : kMaxBlocks);
+  const unsigned tokens = unsigned(a.b) * unsigned(a.s), perUnit = 32 / G * kRows<T>;
+  const auto side = [&](const tcpxbHeads& x, const tcpxbHeads& dy, const void* w, void* out, int heads) {
+    const unsigned parts = (unsigned(heads) + perUnit - 1) / perUnit;
+    return Side{x, dy, w, out, heads, parts, tokens * parts};
+  };
+  Job j;
+  j.side[0] = side(a.q, a.dq_out, a.wq, backward ? a.dq : a.q_out, a.heads);
+  j.side[1] = side(a.k, a.dk_out, a.wk, backward ? a.dk : a.k_out, a.kv_heads);
+  j.cos = a.cos, j.sin = a.sin, j.pos = a.pos, j.partial = a.partial;
+  j.s = unsigned(a.s), j.d = a.d, j.positions = a.positions, j.eps = a.eps, j.perD = 1.f / float(a.d);
+  j.qBlocks = (j.side[0].units + kWarps - 1) / kWarps, j.kBlocks = (j.side[1].units + kWarps - 1) / kWarps;
   if (!backward) {
-    if (!blocks) return TCPXB_T_OK;
-    if (a.wq) forwardKernel<T, G, true><<<blocks, kThreads, 0, s>>>(a);
-    else forwardKernel<T, G, false><<<blocks, kThreads, 0, s>>>(a);
+    if (!tokens) return TCPXB_T_OK;
+    if (a.wq) forwardKernel<T, G, true><<<j.qBlocks + j.kBlocks, kThreads, 0, s>>>(j);
+    else forwardKernel<T, G, false><<<j.qBlocks + j.kBlocks, kThreads, 0, s>>>(j);
     return launched("norm and rotation, forward");
   }
-  if (blocks) {
-    if (a.wq) backwardKernel<T, G, true><<<blocks, kThreads, 0, s>>>(a);
-    else backwardKernel<T, G, false><<<blocks, kThreads, 0, s>>>(a);
+  if (a.wq && j.qBlocks + j.kBlocks > unsigned(kMaxBlocks)) {
+    // the partial sums' rows are given out by the two sides' work
+    const unsigned long long all = (unsigned long long)j.qBlocks + j.kBlocks;
+    unsigned k = unsigned(j.kBlocks * (unsigned long long)kMaxBlocks / all);
+    k = k < 1 ? 1 : k > unsigned(kMaxBlocks) - 1 ? unsigned(kMaxBlocks) - 1 : k;
+    j.kBlocks = k < j.kBlocks ? k : j.kBlocks;
+    j.qBlocks = unsigned(kMaxBlocks) - k < j.qBlocks ? unsigned(kMaxBlocks) - k : j.qBlocks;
+  }
+  if (tokens) {
+    if (a.wq) backwardKernel<T, G, true><<<j.qBlocks + j.kBlocks, kThreads, 0, s>>>(j);
+    else backwardKernel<T, G, false><<<j.qBlocks + j.kBlocks, kThreads, 0, s>>>(j);
     if (const int rc = launched("norm and rotation, backward")) return rc;
   }
-  if (a.wq) weightKernel<T><<<(2 * a.d + 63) / 64, 64, 0, s>>>(a, blocks);
+  if (a.wq) weightKernel<T><<<dim3((a.d + 31) / 32, 2), 1024, 0, s>>>(j, static_cast<T*>(a.dwq), static_cast<T*>(a.dwk));
   return launched("norm and rotation, weights");
 }
 
@@ -222,6 +296,6 @@ int dispatch(const tcpxbNormRope* a, bool backward, void* stream) {
 
 using namespace tcpxb_train;
 
-extern "C" size_t tcpxb_norm_rope_scratch_bytes(int d) { return d > 0 ? sizeof(float) * 2 * d * kMaxBlocks : 0; }
+extern "C" size_t tcpxb_norm_rope_scratch_bytes(int d) { return d > 0 ? sizeof(float) * d * kMaxBlocks : 0; }
 extern "C" int tcpxb_norm_rope_forward(const tcpxbNormRope* a, void* stream) { return dispatch(a, false, stream); }
 extern "C" int tcpxb_norm_rope_backward(const tcpxbNormRope* a, void* stream) { return dispatch(a, true, stream); }

@@ -49,8 +49,12 @@ __device__ __forceinline__ uint64_t nowNs() {
 // Waits for the phase of `parity` to end, two seconds at most.  After that `*dead` makes every wait
 // of the block return at once: its loops run to their end on whatever memory they own, and the
 // block reports a timeout.
-__device__ __noinline__ void barWaitLong(uint32_t bar, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ void barWaitLong(uint32_t bar, uint32_t parity, volatile int* dead) {
+#pragma unroll 1
+  for (int i = 0; i < 64; i++)
+    if (barTry(bar, parity)) return;
   const uint64_t began = nowNs();
+#pragma unroll 1
   while (!barTry(bar, parity)) {
     if (*dead) return;
     if (nowNs() - began > 2000000000ull) {
@@ -60,9 +64,7 @@ __device__ __noinline__ void barWaitLong(uint32_t bar, uint32_t parity, volatile
   }
 }
 __device__ __forceinline__ void barWait(uint32_t bar, uint32_t parity, volatile int* dead) {
-#pragma unroll 1
-  for (int i = 0; i < 16; i++)
-    if (barTry(bar, parity)) return;
+  if (barTry(bar, parity) || barTry(bar, parity)) return;
   barWaitLong(bar, parity, dead);
 }
 
@@ -73,6 +75,9 @@ __device__ __forceinline__ void tmaLoad(uint32_t dst, const CUtensorMap* map, ui
       "l"(map), "r"(bar), "r"(col), "r"(row), "r"(head), "r"(batch)
       : "memory");
 }
+// Moves registers between the block's warpgroups: out of the shares of those that load and issue.
+template <int N> __device__ __forceinline__ void moreRegisters() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewerRegisters() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void fenceAsyncShared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fenceBarInit() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 
@@ -174,29 +179,6 @@ __device__ __forceinline__ float exp2Fast(float x) {
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Two 32-bit operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 template <class T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -22,34 +23,13 @@ MAX_HEAD_SIZE = 128  # of attention
 MAX_NORM_HEAD_SIZE = 256  # of qk_norm_rope
 
 _CODES = {torch.bfloat16: 1, torch.float32: 2, torch.float16: 3}
-_vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+_vp = ctypes.c_void_p
 
 
-class _Heads(ctypes.Structure):
-    _fields_ = [("ptr", _vp), ("stride_b", _i64), ("stride_s", _i64), ("stride_h", _i64)]
-
-
-class _Attention(ctypes.Structure):
-    _fields_ = [("q", _Heads), ("k", _Heads), ("v", _Heads), ("out", _vp), ("lse", _vp), ("dout", _Heads), ("dq", _vp), ("dk", _vp),
-                ("dv", _vp), ("delta", _vp), ("key_lengths", _vp), ("b", _i32), ("sq", _i32), ("sk", _i32), ("heads", _i32),
-                ("kv_heads", _i32), ("d", _i32), ("scale", _f32), ("causal", _i32), ("dtype", _i32), ("status", _vp)]
-
-
-class _NormRope(ctypes.Structure):
-    _fields_ = [("q", _Heads), ("k", _Heads), ("wq", _vp), ("wk", _vp), ("cos", _vp), ("sin", _vp), ("pos", _vp), ("q_out", _vp),
-                ("k_out", _vp), ("dq_out", _Heads), ("dk_out", _Heads), ("dq", _vp), ("dk", _vp), ("dwq", _vp), ("dwk", _vp),
-                ("partial", _vp), ("b", _i32), ("s", _i32), ("heads", _i32), ("kv_heads", _i32), ("d", _i32), ("positions", _i32),
-                ("eps", _f32), ("dtype", _i32)]
-
-
-class _AdamwTensor(ctypes.Structure):
-    _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("m_scale", _vp), ("v_scale", _vp), ("master", _vp), ("step", _vp),
-                ("n", _i64)]
-
-
-class _Adamw(ctypes.Structure):
-    _fields_ = [("lr", _f32), ("beta1", _f32), ("beta2", _f32), ("eps", _f32), ("weight_decay", _f32), ("grad_norm", _vp),
-                ("max_norm", _f32), ("state_bits", _i32), ("dtype", _i32), ("scratch", _vp)]
+# The C entries' argument structs (csrc/include/tcpxb/train.h); a heads descriptor is 4q.
+_ATTENTION = struct.Struct("@12q2P4q5P6if2iP")
+_NORM_ROPE = struct.Struct("@8q7P8q5P6ifi")
+_ADAMW = struct.Struct("@5dPf3iP")
 
 
 _lib = None
@@ -63,6 +43,7 @@ def _t():
         for name in ("tcpxb_attention_forward", "tcpxb_attention_backward", "tcpxb_norm_rope_forward", "tcpxb_norm_rope_backward"):
             getattr(lib, name).argtypes = [_vp, _vp]
         lib.tcpxb_norm_rope_scratch_bytes.restype = ctypes.c_size_t
+        lib.tcpxb_adamw_scratch_bytes.argtypes = [_vp, ctypes.c_int]
         lib.tcpxb_adamw_scratch_bytes.restype = ctypes.c_size_t
         lib.tcpxb_adamw_step.argtypes = [_vp, ctypes.c_int, _vp, _vp]
         lib.tcpxb_grad_norm_scratch_bytes.argtypes = [_vp, ctypes.c_int]
@@ -72,34 +53,51 @@ def _t():
     return _lib
 
 
-def _call(name: str, device: torch.device, *args) -> None:
+def _call(name: str, device: int, *args) -> None:
     """Runs a C entry on the tensors' device, whichever is current, and on that device's current stream."""
-    with torch.cuda.device(device):
-        rc = getattr(_t(), name)(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if torch._C._cuda_getDevice() == device:
+        rc = getattr(_t(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(_t(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
     if rc != 0:
         raise RuntimeError(f"{name} failed ({rc}): {_t().tcpxb_train_last_error().decode()}")
 
 
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _on_one_device(*ts: Optional[torch.Tensor]) -> torch.device:
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) != 1 or next(iter(devices)).type != "cuda":
-        raise ValueError(f"all tensors have to be on one CUDA device, got {sorted(map(str, devices))}")
-    return next(iter(devices))
+def _on_one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
+    """The number of the CUDA device that all of them are on."""
+    device = first.get_device()
+    if device >= 0 and first.is_cuda:
+        for t in rest:
+            if t is not None and t.get_device() != device:
+                break
+        else:
+            return device
+    raise ValueError(f"all tensors have to be on one CUDA device, got {sorted({str(t.device) for t in (first, *rest) if t is not None})}")
 
 
-def _heads(t: torch.Tensor) -> tuple:
-    """(descriptor, tensor that it points into): the tensor itself where its head rows start on 16-byte
-    boundaries and are not broadcast, else a contiguous copy."""
-    size = t.element_size()
-    strides = [st if n > 1 else 16 for n, st in zip(t.shape, t.stride())]
-    if (t.shape[3] > 1 and t.stride(3) != 1) or t.data_ptr() % 16 or any(st * size % 16 or st == 0 for st in strides[:3]):
+def _heads(t: torch.Tensor, per: int) -> tuple:
+    """(tensor, pointer, strides of batch, token and head): of the tensor itself where its head rows start on
+    16-byte boundaries (`per` elements) and are not broadcast, else of a contiguous copy."""
+    b, s, h, d = t.shape
+    sb, ss, sh, sd = t.stride()
+    # the stride of a single entry is of no influence
+    if b == 1:
+        sb = 16
+    if s == 1:
+        ss = 16
+    if h == 1:
+        sh = 16
+    p = t.data_ptr()
+    if p % 16 or (sb | ss | sh) % per or (sd != 1 and d > 1) or not (sb and ss and sh):
         t = t.clone(memory_format=torch.contiguous_format)
-        strides = list(t.stride())
-    return _Heads(t.data_ptr(), *strides[:3]), t
+        sb, ss, sh = t.stride()[:3]
+        p = t.data_ptr()
+    return t, p, sb, ss, sh
 
 
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -113,17 +111,19 @@ def _check_attention(q, k, v, scale, key_lengths) -> float:
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
             raise ValueError(f"{name} has to be [batch, tokens, heads, head size], got {tuple(t.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"attention takes bfloat16 or float16 of one kind, got {q.dtype}, {k.dtype}, {v.dtype}")
+    dtype = q.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
+        raise TypeError(f"attention takes bfloat16 or float16 of one kind, got {dtype}, {k.dtype}, {v.dtype}")
     b, _, h, d = q.shape
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+    kb, _, hk, kd = k.shape
+    if k.shape != v.shape or kb != b or kd != d:
         raise ValueError(f"shapes do not match: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if h < 1 or k.shape[2] < 1 or h % k.shape[2]:
-        raise ValueError(f"{h} query heads are no multiple of {k.shape[2]} key heads")
+    if h < 1 or hk < 1 or h % hk:
+        raise ValueError(f"{h} query heads are no multiple of {hk} key heads")
     if d % 8 or not 8 <= d <= MAX_HEAD_SIZE:
         raise ValueError(f"the head size has to be a multiple of 8 up to {MAX_HEAD_SIZE}, got {d}")
     if key_lengths is not None:
-        if key_lengths.dtype != torch.int32:
+        if key_lengths.dtype is not torch.int32:
             raise TypeError(f"key_lengths has to be int32, got {key_lengths.dtype}")
         if key_lengths.shape != (b,):
             raise ValueError(f"key_lengths has to be [{b}], got {tuple(key_lengths.shape)}")
@@ -133,21 +133,13 @@ def _check_attention(q, k, v, scale, key_lengths) -> float:
     return scale
 
 
-def _attention_args(q, k, v, scale, causal, key_lengths):
-    a = _Attention()
-    a.q, q = _heads(q)
-    a.k, k = _heads(k)
-    a.v, v = _heads(v)
-    key_lengths = None if key_lengths is None else key_lengths.contiguous()
-    a.key_lengths = _ptr(key_lengths)
-    a.b, a.sq, a.heads, a.d = q.shape
-    a.sk, a.kv_heads = k.shape[1:3]
-    a.scale, a.causal, a.dtype = scale, int(bool(causal)), _CODES[q.dtype]
-    return a, (q, k, v, key_lengths)
+def _check_status(status: Optional[torch.Tensor]) -> None:
+    if status is not None and (status.dtype is not torch.int32 or status.numel() < 1 or not status.is_contiguous()):
+        raise ValueError("status has to be a contiguous int32 tensor (ops.status_buffer())")
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False, scale: Optional[float] = None,
-                      key_lengths: Optional[torch.Tensor] = None) -> tuple:
+                      key_lengths: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> tuple:
     """(out, lse) of softmax(scale q k^T) v; not recorded by autograd (see `attention`).
 
     q is [batch, queries, heads, head size], k and v [batch, keys, key heads, head size]; query heads
@@ -156,40 +148,56 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
     16-byte boundaries are copied first.  `causal`: query i sees keys up to i + keys - queries.
     `key_lengths` ([batch], int32): keys at and behind a batch's length are not seen, whatever they
     hold.  A query that sees no key gets zeros.  `out` is contiguous; `lse` [batch, heads, queries]
-    (float32) is the natural logarithm of each row's sum of exponentials, -inf for an empty row."""
+    (float32) is the natural logarithm of each row's sum of exponentials, -inf for an empty row.
+    `status` (`ops.status_buffer()`): its first word becomes 3 where a wait inside the kernel ran out of
+    time and the outputs are void."""
     scale = _check_attention(q, k, v, scale, key_lengths)
-    dev = _on_one_device(q, k, v, key_lengths)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev)
-    a, keep = _attention_args(q, k, v, scale, causal, key_lengths)
-    a.out, a.lse = out.data_ptr(), lse.data_ptr()
-    _call("tcpxb_attention_forward", dev, ctypes.byref(a))
+    _check_status(status)
+    dev = _on_one_device(q, k, v, key_lengths, status)
+    b, sq, h, d = q.shape
+    sk, hk = k.shape[1:3]
+    out, lse = q.new_empty((b, sq, h, d)), q.new_empty((b, h, sq), dtype=torch.float32)
+    q, *qa = _heads(q, 8)
+    k, *ka = _heads(k, 8)
+    v, *va = _heads(v, 8)
+    if key_lengths is not None:
+        key_lengths = key_lengths.contiguous()
+    _call("tcpxb_attention_forward", dev, _ATTENTION.pack(*qa, *ka, *va, out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, _ptr(key_lengths),
+                                                          b, sq, sk, h, hk, d, scale, bool(causal), _CODES[q.dtype], _ptr(status)))
     return out, lse
 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, *,
-                       causal: bool = False, scale: Optional[float] = None, key_lengths: Optional[torch.Tensor] = None) -> tuple:
+                       causal: bool = False, scale: Optional[float] = None, key_lengths: Optional[torch.Tensor] = None,
+                       status: Optional[torch.Tensor] = None) -> tuple:
     """(dq, dk, dv) from what `attention_forward` returned for the same arguments.  The probabilities
     are computed again from the scores and `lse`.  The same inputs give the same bits every time."""
     scale = _check_attention(q, k, v, scale, key_lengths)
+    b, sq, h, d = q.shape
+    sk, hk = k.shape[1:3]
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape:
             raise ValueError(f"{name} has to be {tuple(q.shape)}, got {tuple(t.shape)}")
-        if t.dtype != q.dtype:
+        if t.dtype is not q.dtype:
             raise TypeError(f"{name} has to be {q.dtype}, got {t.dtype}")
-    if lse.shape != (q.shape[0], q.shape[2], q.shape[1]):
+    if lse.shape != (b, h, sq):
         raise ValueError(f"lse has to be [batch, heads, queries], got {tuple(lse.shape)}")
-    if lse.dtype != torch.float32:
+    if lse.dtype is not torch.float32:
         raise TypeError(f"lse has to be float32, got {lse.dtype}")
-    dev = _on_one_device(dout, q, k, v, out, lse, key_lengths)
-    a, keep = _attention_args(q, k, v, scale, causal, key_lengths)
-    a.dout, dout = _heads(dout)
+    _check_status(status)
+    dev = _on_one_device(dout, q, k, v, out, lse, key_lengths, status)
+    dq, dk, dv = q.new_empty((b, sq, h, d)), k.new_empty((b, sk, hk, d)), v.new_empty((b, sk, hk, d))
+    delta = lse.new_empty((b, h, sq))
     out, lse = _aligned(out), lse.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-    delta = torch.empty_like(lse)
-    a.out, a.lse, a.delta = out.data_ptr(), lse.data_ptr(), delta.data_ptr()
-    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    _call("tcpxb_attention_backward", dev, ctypes.byref(a))
+    q, *qa = _heads(q, 8)
+    k, *ka = _heads(k, 8)
+    v, *va = _heads(v, 8)
+    dout, *da = _heads(dout, 8)
+    if key_lengths is not None:
+        key_lengths = key_lengths.contiguous()
+    _call("tcpxb_attention_backward", dev, _ATTENTION.pack(*qa, *ka, *va, out.data_ptr(), lse.data_ptr(), *da, dq.data_ptr(), dk.data_ptr(),
+                                                           dv.data_ptr(), delta.data_ptr(), _ptr(key_lengths), b, sq, sk, h, hk, d, scale,
+                                                           bool(causal), _CODES[q.dtype], _ptr(status)))
     return dq, dk, dv
 
 
@@ -252,25 +260,20 @@ def _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions) -> None
         raise ValueError(f"eps has to be finite and not below zero, got {eps}")
 
 
-def _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps, positions):
-    a = _NormRope()
-    cos, sin, q_weight, k_weight = _aligned(cos), _aligned(sin), _aligned(q_weight), _aligned(k_weight)
-    positions = None if positions is None else positions.contiguous()
-    a.cos, a.sin, a.wq, a.wk, a.pos = _ptr(cos), _ptr(sin), _ptr(q_weight), _ptr(k_weight), _ptr(positions)
-    a.b, a.s, a.heads, a.d = q.shape
-    a.kv_heads, a.positions, a.eps, a.dtype = k.shape[2], cos.shape[0], eps, _CODES[q.dtype]
-    return a, (cos, sin, q_weight, k_weight, positions)
-
-
 def _norm_rope_forward(q, k, cos, sin, q_weight, k_weight, eps, positions) -> tuple:
     _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions)
     dev = _on_one_device(q, k, cos, sin, q_weight, k_weight, positions)
-    a, keep = _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps, positions)
-    a.q, q = _heads(q)
-    a.k, k = _heads(k)
-    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
-    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
-    _call("tcpxb_norm_rope_forward", dev, ctypes.byref(a))
+    b, s, h, d = q.shape
+    hk, per = k.shape[2], 16 // q.element_size()
+    q_out, k_out = q.new_empty((b, s, h, d)), k.new_empty((b, s, hk, d))
+    cos, sin, q_weight, k_weight = _aligned(cos), _aligned(sin), _aligned(q_weight), _aligned(k_weight)
+    if positions is not None:
+        positions = positions.contiguous()
+    q, *qa = _heads(q, per)
+    k, *ka = _heads(k, per)
+    _call("tcpxb_norm_rope_forward", dev, _NORM_ROPE.pack(*qa, *ka, _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), _ptr(positions),
+                                                          q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, b, s, h, hk, d,
+                                                          cos.shape[0], eps, _CODES[q.dtype]))
     return q_out, k_out
 
 
@@ -283,22 +286,27 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     for name, t, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
         if t.shape != x.shape:
             raise ValueError(f"{name} has to be {tuple(x.shape)}, got {tuple(t.shape)}")
-        if t.dtype != x.dtype:
+        if t.dtype is not x.dtype:
             raise TypeError(f"{name} has to be {x.dtype}, got {t.dtype}")
     dev = _on_one_device(dq_out, dk_out, q, k, cos, sin, q_weight, k_weight, positions)
-    a, keep = _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps, positions)
-    a.dq_out, dq_out = _heads(dq_out)
-    a.dk_out, dk_out = _heads(dk_out)
-    dq, dk = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
-    a.dq, a.dk = dq.data_ptr(), dk.data_ptr()
-    dwq = dwk = None
+    b, s, h, d = q.shape
+    hk, per = k.shape[2], 16 // q.element_size()
+    dq, dk = q.new_empty((b, s, h, d)), k.new_empty((b, s, hk, d))
+    dwq = dwk = partial = None
+    qa = ka = (0, 0, 0, 0)
     if q_weight is not None:
-        a.q, q = _heads(q)
-        a.k, k = _heads(k)
-        dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
-        partial = torch.empty(_t().tcpxb_norm_rope_scratch_bytes(a.d), dtype=torch.uint8, device=dev)
-        a.dwq, a.dwk, a.partial = dwq.data_ptr(), dwk.data_ptr(), partial.data_ptr()
-    _call("tcpxb_norm_rope_backward", dev, ctypes.byref(a))
+        dwq, dwk = q_weight.new_empty((d,)), k_weight.new_empty((d,))
+        partial = cos.new_empty(_t().tcpxb_norm_rope_scratch_bytes(d) // 4)
+        q, *qa = _heads(q, per)
+        k, *ka = _heads(k, per)
+    cos, sin, q_weight, k_weight = _aligned(cos), _aligned(sin), _aligned(q_weight), _aligned(k_weight)
+    if positions is not None:
+        positions = positions.contiguous()
+    dq_out, *dqa = _heads(dq_out, per)
+    dk_out, *dka = _heads(dk_out, per)
+    _call("tcpxb_norm_rope_backward", dev, _NORM_ROPE.pack(*qa, *ka, _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), _ptr(positions), 0, 0,
+                                                           *dqa, *dka, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk), _ptr(partial), b, s, h, hk, d,
+                                                           cos.shape[0], eps, _CODES[dq.dtype]))
     return dq, dk, dwq, dwk
 
 
@@ -337,39 +345,48 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
 
 
 # ----------------------------------------------------------------------- AdamW
-def _flat_list(name: str, ts: Sequence[torch.Tensor], like: Sequence[torch.Tensor], dtype: torch.dtype, numels=None) -> None:
-    if len(ts) != len(like):
-        raise ValueError(f"{len(like)} tensors, but {len(ts)} {name}")
-    for i, (t, p) in enumerate(zip(ts, like)):
-        if t.dtype != dtype:
+def _flat_list(name: str, ts: Sequence[torch.Tensor], numels: Sequence[int], dtype: torch.dtype, device: int) -> list:
+    """The tensors' addresses; `device`: -1 stands for the CPU, where the arguments are all that can be checked."""
+    if len(ts) != len(numels):
+        raise ValueError(f"{len(numels)} tensors, but {len(ts)} {name}")
+    at = []
+    for i, t in enumerate(ts):
+        if t.dtype is not dtype:
             raise TypeError(f"{name}[{i}] has to be {dtype}, got {t.dtype}")
-        if t.numel() != (p.numel() if numels is None else numels[i]):
+        if t.numel() != numels[i]:
             raise ValueError(f"{name}[{i}] has {t.numel()} elements")
         if not t.is_contiguous():
             raise ValueError(f"{name}[{i}] has to be contiguous")
+        if t.get_device() != device:
+            raise ValueError(f"{name}[{i}] is on another device")
+        at.append(t.data_ptr())
+    return at
+
+
+def _table(*columns: Sequence[int]) -> ctypes.Array:
+    """The C entry's list of tensors: rows of nine words, from lists of each word."""
+    rows = [x for row in zip(*columns) for x in row]
+    return (ctypes.c_int64 * len(rows))(*rows)
 
 
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """Root of the sum of all squares, as a float32 scalar on the device.  Contiguous CUDA tensors of one
     type (bfloat16, float16, float32); squares of a few elements are added in 32 bits, those sums in 64,
-    in an order that depends on the sizes alone."""
+    in an order that depends on sizes and alignments alone."""
     grads = list(grads)
     if not grads:
         raise ValueError("no gradients")
-    if grads[0].dtype not in _CODES:
-        raise TypeError(f"gradients have to be bfloat16, float16 or float32, got {grads[0].dtype}")
-    _flat_list("grads", grads, grads, grads[0].dtype)
-    dev = _on_one_device(*grads)
-    table = (_AdamwTensor * len(grads))()
-    for e, g in zip(table, grads):
-        e.g, e.n = g.data_ptr(), g.numel()
-    return _queue_norm(table, len(grads), grads[0].dtype, dev)
-
-
-def _queue_norm(table, count: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    scratch = torch.empty(_t().tcpxb_grad_norm_scratch_bytes(table, count), dtype=torch.uint8, device=dev)
-    _call("tcpxb_grad_norm", dev, table, count, _CODES[dtype], norm.data_ptr(), scratch.data_ptr())
+    dtype = grads[0].dtype
+    if dtype not in _CODES:
+        raise TypeError(f"gradients have to be bfloat16, float16 or float32, got {dtype}")
+    numels = [g.numel() for g in grads]
+    at = _flat_list("grads", grads, numels, dtype, grads[0].get_device())
+    dev = _on_one_device(grads[0])
+    none = [0] * len(grads)
+    table = _table(none, at, none, none, none, none, none, none, numels)
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    scratch = grads[0].new_empty(_t().tcpxb_grad_norm_scratch_bytes(table, len(grads)), dtype=torch.uint8)
+    _call("tcpxb_grad_norm", dev, table, len(grads), _CODES[dtype], norm.data_ptr(), scratch.data_ptr())
     return norm
 
 
@@ -378,7 +395,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                weight_decay: float = 1e-2, max_grad_norm: Optional[float] = None, norm: Optional[torch.Tensor] = None,
                exp_avg_scales: Optional[Sequence[torch.Tensor]] = None, exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
                masters: Optional[Sequence[torch.Tensor]] = None) -> Optional[torch.Tensor]:
-    """One AdamW step over all tensors, in place, in two launches (four with clipping).
+    """One AdamW step over all tensors, in place, in two launches (three with clipping).
 
     `params` and `grads`: contiguous tensors of one type (bfloat16, float16, float32) on one device.
     States in 32 bits: `exp_avgs` and `exp_avg_sqs` are float32 tensors of the params' sizes.  In 8 bits:
@@ -398,29 +415,32 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     bits = 8 if exp_avg_scales is not None else 32
     if (exp_avg_sq_scales is None) != (bits == 32):
         raise ValueError("8-bit states need the scales of both")
-    _flat_list("params", params, params, dtype)
-    _flat_list("grads", grads, params, dtype)
+    count, device = len(params), params[0].get_device()
+    numels = [p.numel() for p in params]
+    p_at = _flat_list("params", params, numels, dtype, device)
+    g_at = _flat_list("grads", grads, numels, dtype, device)
     state = torch.float8_e4m3fn if bits == 8 else torch.float32
-    _flat_list("exp_avgs", exp_avgs, params, state)
-    _flat_list("exp_avg_sqs", exp_avg_sqs, params, state)
-    lists = [params, grads, exp_avgs, exp_avg_sqs]
+    m_at = _flat_list("exp_avgs", exp_avgs, numels, state, device)
+    v_at = _flat_list("exp_avg_sqs", exp_avg_sqs, numels, state, device)
+    none = [0] * count
+    ms_at = vs_at = master_at = none
+    written = p_at + m_at + v_at
     if bits == 8:
-        exp_avg_scales, exp_avg_sq_scales = list(exp_avg_scales), list(exp_avg_sq_scales)
-        blocks = [-(-p.numel() // STATE_BLOCK) for p in params]
-        _flat_list("exp_avg_scales", exp_avg_scales, params, torch.float32, blocks)
-        _flat_list("exp_avg_sq_scales", exp_avg_sq_scales, params, torch.float32, blocks)
-        lists += [exp_avg_scales, exp_avg_sq_scales]
+        blocks = [-(-n // STATE_BLOCK) for n in numels]
+        ms_at = _flat_list("exp_avg_scales", list(exp_avg_scales), blocks, torch.float32, device)
+        vs_at = _flat_list("exp_avg_sq_scales", list(exp_avg_sq_scales), blocks, torch.float32, device)
+        written += ms_at + vs_at
     if masters is not None:
-        masters = list(masters)
-        if dtype == torch.float32:
+        if dtype is torch.float32:
             raise ValueError("masters stand behind 16-bit params")
-        _flat_list("masters", masters, params, torch.float32)
-        lists.append(masters)
-    if steps.dtype != torch.int32:
+        master_at = _flat_list("masters", list(masters), numels, torch.float32, device)
+        written += master_at
+    if steps.dtype is not torch.int32:
         raise TypeError(f"steps has to be int32, got {steps.dtype}")
-    if steps.shape != (len(params),) or not steps.is_contiguous():
-        raise ValueError(f"steps has to be a contiguous [{len(params)}], got {tuple(steps.shape)}")
-    written = [t.data_ptr() for ts in lists if ts is not grads for t in ts if t.numel()]
+    if steps.shape != (count,) or not steps.is_contiguous():
+        raise ValueError(f"steps has to be a contiguous [{count}], got {tuple(steps.shape)}")
+    if 0 in numels:  # a tensor without elements has no address of its own
+        written = [x for x, n in zip(written, numels * (len(written) // count)) if n]
     if len(set(written)) != len(written):
         raise ValueError("a tensor is given twice")
     beta1, beta2 = betas
@@ -428,22 +448,15 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError(f"bad numbers: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
     if max_grad_norm is not None and not 0 <= max_grad_norm < math.inf:
         raise ValueError(f"max_grad_norm has to be finite and not below zero, got {max_grad_norm}")
-    if norm is not None and (norm.dtype != torch.float32 or norm.numel() != 1 or max_grad_norm is None):
+    if norm is not None and (norm.dtype is not torch.float32 or norm.numel() != 1 or max_grad_norm is None):
         raise ValueError("norm has to be one float32 value, given with max_grad_norm")
-    dev = _on_one_device(steps, norm, *(t for ts in lists for t in ts))
-    count = len(params)
-    table = (_AdamwTensor * count)()
-    step_ptr = steps.data_ptr()
-    for i, e in enumerate(table):
-        e.p, e.g, e.m, e.v = params[i].data_ptr(), grads[i].data_ptr(), exp_avgs[i].data_ptr(), exp_avg_sqs[i].data_ptr()
-        e.step, e.n = step_ptr + 4 * i, params[i].numel()
-        if bits == 8:
-            e.m_scale, e.v_scale = exp_avg_scales[i].data_ptr(), exp_avg_sq_scales[i].data_ptr()
-        if masters is not None:
-            e.master = masters[i].data_ptr()
-    if max_grad_norm is not None and norm is None:
-        norm = _queue_norm(table, count, dtype, dev)
-    scratch = torch.empty(_t().tcpxb_adamw_scratch_bytes(count), dtype=torch.uint8, device=dev)
-    a = _Adamw(lr, beta1, beta2, eps, weight_decay, _ptr(norm), max_grad_norm or 0.0, bits, _CODES[dtype], scratch.data_ptr())
-    _call("tcpxb_adamw_step", dev, table, count, ctypes.byref(a))
+    dev = _on_one_device(params[0], steps, norm)
+    step_at = steps.data_ptr()
+    table = _table(p_at, g_at, m_at, v_at, ms_at, vs_at, master_at, range(step_at, step_at + 4 * count, 4), numels)
+    compute = max_grad_norm is not None and norm is None
+    if compute:
+        norm = steps.new_empty((), dtype=torch.float32)
+    scratch = steps.new_empty(_t().tcpxb_adamw_scratch_bytes(table, count), dtype=torch.uint8)
+    _call("tcpxb_adamw_step", dev, table, count, _ADAMW.pack(lr, beta1, beta2, eps, weight_decay, _ptr(norm), max_grad_norm or 0.0, compute, bits,
+                                                             _CODES[dtype], scratch.data_ptr()))
     return norm

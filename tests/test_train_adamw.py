@@ -257,15 +257,17 @@ def test_refusals():
 
 def test_the_c_entry_refuses():
     import ctypes
+    import train_abi as A
     from nccl_plugin_gpudirecttcpx_b200.ops import train as T
     lib = T._t()
-    t = (T._AdamwTensor * 1)(T._AdamwTensor(4096, 4096, 4096, 4096, None, None, None, 4096, 10))
+    assert ctypes.sizeof(A.Adamw) == T._ADAMW.size
+    t = (A.AdamwTensor * 1)(A.AdamwTensor(4096, 4096, 4096, 4096, None, None, None, 4096, 10))
     good = dict(lr=1e-3, beta1=0.9, beta2=0.9, eps=1e-8, weight_decay=0.0, state_bits=32, dtype=1, scratch=4096)
-    assert lib.tcpxb_adamw_step(t, 1, None, None) == -1 and lib.tcpxb_adamw_step(None, 1, ctypes.byref(T._Adamw(**good)), None) == -1
-    for kw in ({"state_bits": 16}, {"dtype": 9}, {"scratch": None}, {"state_bits": 8}):
-        assert lib.tcpxb_adamw_step(t, 1, ctypes.byref(T._Adamw(**{**good, **kw})), None) == -1
+    assert lib.tcpxb_adamw_step(t, 1, None, None) == -1 and lib.tcpxb_adamw_step(None, 1, ctypes.byref(A.Adamw(**good)), None) == -1
+    for kw in ({"state_bits": 16}, {"dtype": 9}, {"scratch": None}, {"state_bits": 8}, {"compute_norm": 1}):
+        assert lib.tcpxb_adamw_step(t, 1, ctypes.byref(A.Adamw(**{**good, **kw})), None) == -1
     for field, x in (("p", None), ("g", None), ("m", None), ("step", None), ("n", -1)):
-        u = (T._AdamwTensor * 1)(T._AdamwTensor(4096, 4096, 4096, 4096, None, None, None, 4096, 10))
+        u = (A.AdamwTensor * 1)(A.AdamwTensor(4096, 4096, 4096, 4096, None, None, None, 4096, 10))
         setattr(u[0], field, x)
-        assert lib.tcpxb_adamw_step(u, 1, ctypes.byref(T._Adamw(**good)), None) == -1, field
+        assert lib.tcpxb_adamw_step(u, 1, ctypes.byref(A.Adamw(**good)), None) == -1, field
     assert lib.tcpxb_grad_norm(t, 1, 1, None, 4096, None) == -1

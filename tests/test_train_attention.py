@@ -260,20 +260,23 @@ def test_refusals():
 def test_the_c_entry_refuses():
     """What the Python checks keep out is an error code of the C entry too, before it touches the device."""
     import ctypes
+    import train_abi as A
     from nccl_plugin_gpudirecttcpx_b200.ops import train as T
     lib = T._t()
+    assert ctypes.sizeof(A.Attention) == T._ATTENTION.size
     assert lib.tcpxb_attention_forward(None, None) == -1
 
     def args(**kw):
-        a = T._Attention(b=1, sq=4, sk=4, heads=4, kv_heads=2, d=64, scale=0.1, dtype=1, out=4096, lse=4096)
+        a = A.Attention(b=1, sq=4, sk=4, heads=4, kv_heads=2, d=64, scale=0.1, dtype=1, out=4096, lse=4096)
         for n in ("q", "k", "v"):
-            setattr(a, n, T._Heads(4096, 1024, 256, 64))
+            for field, x in ((n, 4096), (n + "_b", 1024), (n + "_s", 256), (n + "_h", 64)):
+                setattr(a, field, x)
         for n, x in kw.items():
             setattr(a, n, x)
         return ctypes.byref(a)
 
     for kw in ({"b": -1}, {"kv_heads": 3}, {"kv_heads": 0}, {"d": 60}, {"d": 136}, {"d": 0}, {"dtype": 2}, {"scale": 0.0}, {"scale": math.nan},
-               {"out": 0}, {"q": T._Heads(4098, 1024, 256, 64)}, {"k": T._Heads(4096, 1024, 257, 64)}, {"v": T._Heads(0, 0, 0, 0)}):
+               {"out": 0}, {"q": 4098}, {"k_s": 257}, {"v": 0}, {"v_s": 0}, {"sk": 1 << 24}):
         assert lib.tcpxb_attention_forward(args(**kw), None) == -1, kw
         assert lib.tcpxb_train_last_error()
     assert lib.tcpxb_attention_backward(args(), None) == -1

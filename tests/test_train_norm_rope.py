@@ -196,18 +196,19 @@ def test_refusals():
 
 def test_the_c_entry_refuses():
     import ctypes
+    import train_abi as A
     from nccl_plugin_gpudirecttcpx_b200.ops import train as T
     lib = T._t()
+    assert ctypes.sizeof(A.NormRope) == T._NORM_ROPE.size
     assert lib.tcpxb_norm_rope_forward(None, None) == -1
 
     def args(**kw):
-        heads = T._Heads(4096, 1024, 256, 64)
-        a = T._NormRope(b=1, s=4, heads=4, kv_heads=2, d=64, positions=4, eps=1e-6, dtype=1, q=heads, k=heads, cos=4096, sin=4096, q_out=4096, k_out=4096)
+        a = A.NormRope(b=1, s=4, heads=4, kv_heads=2, d=64, positions=4, eps=1e-6, dtype=1, q=4096, k=4096, q_s=256, k_s=256, q_h=64, k_h=64, cos=4096, sin=4096, q_out=4096, k_out=4096)
         for n, x in kw.items():
             setattr(a, n, x)
         return ctypes.byref(a)
 
     for kw in ({"b": -1}, {"heads": 0}, {"d": 60}, {"d": 264}, {"dtype": 0}, {"positions": 3}, {"cos": 0}, {"wq": 4096}, {"q_out": 0},
-               {"q": T._Heads(4098, 0, 0, 0)}, {"k": T._Heads(4096, 1, 0, 0)}):
+               {"q": 4098}, {"k_s": 1}, {"cos": 4100}, {"b": 1 << 30}):
         assert lib.tcpxb_norm_rope_forward(args(**kw), None) == -1, kw
     assert lib.tcpxb_norm_rope_backward(args(), None) == -1
