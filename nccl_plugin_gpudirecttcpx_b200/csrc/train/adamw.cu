@@ -28,7 +28,7 @@ constexpr int kThreads = 256;
 // which begin and end less often (323 M weights with 8-bit states: 1.61 ms in chunks of 8192).
 constexpr int kShortChunk = 8192, kLongChunk = 32768;
 constexpr long long kManyElements = 148ll * 8 * 4 * kShortChunk;
-constexpr float kE4m3Max = 448.f;
+constexpr float kE4m3Max = 448.f, kLeastCode = 0.001953125f;  // the largest code, and 2^-9, the smallest above zero
 
 template <int N> struct List {
   tcpxbAdamwTensor t[N];
@@ -217,39 +217,31 @@ template <class T> __device__ __forceinline__ void stepElements(const tcpxbAdamw
   }
 }
 
-// 8-bit states.  A warp has the next block's loads in flight while it works on one.
-template <class T> struct Raw {
-  Vec8<T> p, g;
+// 8-bit states: what a lane holds of a block.  W: the type that the weights are read in.
+template <class T, class W> struct Raw {
+  Vec8<W> w;
+  Vec8<T> g;
   Codes m, v;
-  float mScale, vScale;
 };
-template <bool kVector, class T> __device__ __forceinline__ void fetch(Raw<T>& r, const tcpxbAdamwTensor& t, long long b, long long end) {
-  const long long e = b + threadIdx.x % 32 * 8;
-  r.p = get<kVector, Vec8<T>>(static_cast<const T*>(t.p), e, end);
-  r.g = get<kVector, Vec8<T>>(static_cast<const T*>(t.g), e, end);
-  r.m = get<kVector, Codes>(static_cast<const __nv_fp8_storage_t*>(t.m), e, end);
-  r.v = get<kVector, Codes>(static_cast<const __nv_fp8_storage_t*>(t.v), e, end);
-  r.mScale = t.m_scale[b / TCPXB_ADAMW_BLOCK];
-  r.vScale = t.v_scale[b / TCPXB_ADAMW_BLOCK];
+// Largest magnitude of the warp; NaN is left out (its code is NaN by itself).
+__device__ __forceinline__ float warpTop(float x) {
+  float y;
+  asm("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
 }
-// Largest magnitudes of the warp; NaN is left out (its code is NaN by itself).
-__device__ __forceinline__ void warpTops(float& x, float& y) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
-  }
-}
-template <bool kVector, class T> __device__ __forceinline__ void stepBlock(const Raw<T>& r, const tcpxbAdamwTensor& t, const Step& step, long long b, long long end) {
+// About 220 instructions a block, of which 64 are the step itself: at this count issue and memory
+// take the same time, so the rest is kept short (the warp's maximum is one instruction, the four
+// divisions of a block are done by four lanes at once).
+template <bool kVector, class T, class W>
+__device__ __forceinline__ void stepBlock(const Raw<T, W>& r, const tcpxbAdamwTensor& t, const Step& step, long long b, long long end, float& mScale, float& vScale) {
   const int lane = threadIdx.x % 32;
   const long long e = b + lane * 8;
   float2 pp[4], gg[4], mm[4], vv[4], root[4];
-  if (t.master) pairs(get<kVector, Vec8<float>>(t.master, e, end), pp);
-  else pairs(r.p, pp);
+  pairs(r.w, pp);
   pairs(r.g, gg);
-  decode(r.m, r.mScale, mm);
-  decode(r.v, r.vScale, vv);
-  float topM = 0.f, topV = 0.f;
+  decode(r.m, mScale, mm);
+  decode(r.v, vScale, vv);
+  float topM = 0.f, topV = 0.f, least = INFINITY;
   // past the end everything is zero and stays so
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -257,67 +249,139 @@ template <bool kVector, class T> __device__ __forceinline__ void stepBlock(const
     step(pp[i], gg[i], mm[i], vv[i], root[i]);
     topM = fmaxf(topM, fmaxf(fabsf(mm[i].x), fabsf(mm[i].y)));
     topV = fmaxf(topV, fmaxf(root[i].x, root[i].y));
+    least = fminf(least, fminf(root[i].x, root[i].y));
   }
   put<kVector>(static_cast<T*>(t.p), e, end, rounded<T>(pp));
-  if (t.master) put<kVector>(t.master, e, end, rounded<float>(pp));
-  warpTops(topM, topV);
-  // below 1e-30 a block is held as zeros: the factor back would leave the range
-  const float toM = topM >= 1e-30f ? kE4m3Max / topM : 0.f, toV = topV >= 1e-30f ? kE4m3Max / topV : 0.f;
+  if constexpr (!std::is_same_v<T, W>) put<kVector>(t.master, e, end, rounded<float>(pp));
+  topM = warpTop(topM), topV = warpTop(topV);
+  // lanes 0 and 1 take the factors to codes, 2 and 3 the scales, of m and of the root.  Below 1e-30
+  // a block is held as zeros: the factor would leave the range.
+  const float top = lane & 1 ? topV : topM;
+  float ratio = lane & 2 ? top / kE4m3Max : kE4m3Max / top;
+  if (!(top >= 1e-30f)) ratio = 0.f;
+  const float toM = __shfl_sync(0xffffffffu, ratio, 0), toV = __shfl_sync(0xffffffffu, ratio, 1);
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     mm[i] = mul2(mm[i], {toM, toM});
     root[i] = mul2(root[i], {toV, toV});
-    // 2^-9 is the smallest code above zero
-    if (root[i].x > 0.f) root[i].x = fmaxf(root[i].x, 0.001953125f);
-    if (root[i].y > 0.f) root[i].y = fmaxf(root[i].y, 0.001953125f);
+  }
+  if (least * toV < kLeastCode) {
+    // rare: roots under the smallest code above zero become that code, zeros stay
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (root[i].x > 0.f) root[i].x = fmaxf(root[i].x, kLeastCode);
+      if (root[i].y > 0.f) root[i].y = fmaxf(root[i].y, kLeastCode);
+    }
   }
   put<kVector>(static_cast<__nv_fp8_storage_t*>(t.m), e, end, encode(mm));
   put<kVector>(static_cast<__nv_fp8_storage_t*>(t.v), e, end, encode(root));
-  if (lane == 0) {
-    t.m_scale[b / TCPXB_ADAMW_BLOCK] = topM >= 1e-30f ? topM / kE4m3Max : 0.f;
-    t.v_scale[b / TCPXB_ADAMW_BLOCK] = topV >= 1e-30f ? topV / kE4m3Max : 0.f;
+  mScale = __shfl_sync(0xffffffffu, ratio, 2), vScale = __shfl_sync(0xffffffffu, ratio, 3);
+}
+
+template <int kBytes> __device__ __forceinline__ void copyAsync(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "n"(kBytes) : "memory");
+}
+
+// The blocks of a chunk, every fourth one by a warp.  A lane copies its own share of the blocks
+// ahead into shared memory, three of them in flight (a register prefetch of one left memory idle:
+// 0.66 ms for 323 M weights with no arithmetic at all).  The chunk's scales are read before the
+// first block and written after the last: one in between waits for the stores to its neighbours
+// (0.94 ms).
+constexpr int kSmallWarps = 4, kStages = 4;
+static_assert(kLongChunk / TCPXB_ADAMW_BLOCK / kSmallWarps <= 32, "a lane holds the scales of one block of its warp");
+
+template <class T, class W> __device__ __forceinline__ void stepBlocks(char* shared, const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end, bool vectors) {
+  using Share = Raw<T, W>;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  Share* ring = reinterpret_cast<Share*>(shared) + warp * kStages * 32 + lane;  // kStages apart by 32
+  const W* weights = static_cast<const W*>(std::is_same_v<T, W> ? t.p : t.master);
+  const int blocks = int((end - begin + TCPXB_ADAMW_BLOCK - 1) / TCPXB_ADAMW_BLOCK), whole = vectors ? int((end - begin) / TCPXB_ADAMW_BLOCK) : 0;
+  const long long block0 = begin / TCPXB_ADAMW_BLOCK;
+  float mScale = 0.f, vScale = 0.f;  // of the warp's block number `lane`
+  if (warp + kSmallWarps * lane < blocks) {
+    mScale = t.m_scale[block0 + warp + kSmallWarps * lane];
+    vScale = t.v_scale[block0 + warp + kSmallWarps * lane];
+  }
+  const auto copy = [&](int k) {
+    const int n = warp + kSmallWarps * k;
+    if (n < whole) {
+      const long long e = begin + n * TCPXB_ADAMW_BLOCK + lane * 8;
+      Share* to = ring + k % kStages * 32;
+#pragma unroll
+      for (int i = 0; i < int(sizeof(Vec8<W>)); i += 16) copyAsync<16>(reinterpret_cast<char*>(&to->w) + i, reinterpret_cast<const char*>(weights + e) + i);
+#pragma unroll
+      for (int i = 0; i < int(sizeof(Vec8<T>)); i += 16)
+        copyAsync<16>(reinterpret_cast<char*>(&to->g) + i, reinterpret_cast<const char*>(static_cast<const T*>(t.g) + e) + i);
+      copyAsync<8>(&to->m, static_cast<const char*>(t.m) + e);
+      copyAsync<8>(&to->v, static_cast<const char*>(t.v) + e);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 1; k++) copy(k);
+  int k = 0;
+#pragma unroll 1
+  for (; warp + kSmallWarps * k < whole; k++) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    const Share r = ring[k % kStages * 32];  // a lane reads what it copied itself
+    copy(k + kStages - 1);
+    float m = __shfl_sync(0xffffffffu, mScale, k), v = __shfl_sync(0xffffffffu, vScale, k);
+    stepBlock<true>(r, t, step, begin + (warp + kSmallWarps * k) * TCPXB_ADAMW_BLOCK, end, m, v);
+    if (lane == k) mScale = m, vScale = v;
+  }
+#pragma unroll 1
+  for (; warp + kSmallWarps * k < blocks; k++) {
+    const long long b = begin + (warp + kSmallWarps * k) * TCPXB_ADAMW_BLOCK, e = b + lane * 8;
+    const Share r = {get<false, Vec8<W>>(weights, e, end), get<false, Vec8<T>>(static_cast<const T*>(t.g), e, end),
+                     get<false, Codes>(static_cast<const __nv_fp8_storage_t*>(t.m), e, end), get<false, Codes>(static_cast<const __nv_fp8_storage_t*>(t.v), e, end)};
+    float m = __shfl_sync(0xffffffffu, mScale, k), v = __shfl_sync(0xffffffffu, vScale, k);
+    stepBlock<false>(r, t, step, b, end, m, v);
+    if (lane == k) mScale = m, vScale = v;
+  }
+  if (warp + kSmallWarps * lane < blocks) {
+    t.m_scale[block0 + warp + kSmallWarps * lane] = mScale;
+    t.v_scale[block0 + warp + kSmallWarps * lane] = vScale;
   }
 }
 
-template <class T, class L, bool kSmall, int kBlocks = kSmall ? 3 : 4> __global__ void __launch_bounds__(kThreads, kBlocks) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
-  const int i = tensorOf(l, blockIdx.x);
-  const tcpxbAdamwTensor t = l.t[i];
-  const long long begin = (long long)(blockIdx.x - (i ? l.end[i - 1] : 0)) * l.chunk;
-  const long long end = min((long long)t.n, begin + l.chunk);
-  const auto* s = static_cast<const Scratch*>(a.scratch);
-  const Step step{float(a.beta1), float(a.beta2), float(1 - a.beta1), float(1 - a.beta2), float(a.eps), float(1 - a.lr * a.weight_decay),
-                  s->rates[l.first + i].stepSize, s->rates[l.first + i].rootCorrection, s->coef};
-  const bool vectors = aligned(t.p) && aligned(t.g) && aligned(t.m) && aligned(t.v) && aligned(t.master);
-  if constexpr (!kSmall) {
-    const long long whole = vectors ? begin + (end - begin) / 8 * 8 : begin;
-    stepVectors<T>(t, step, begin, whole);
-    stepElements<T>(t, step, whole, end);
-  } else {
-    constexpr int kStride = kThreads / 32 * TCPXB_ADAMW_BLOCK;
-    long long b = begin + threadIdx.x / 32 * TCPXB_ADAMW_BLOCK;
-    Raw<T> r;
-    const long long whole = vectors ? end - TCPXB_ADAMW_BLOCK : begin - 1;  // last place where a vector block begins
-    if (b <= whole) fetch<true>(r, t, b, end);
-#pragma unroll 1
-    for (; b <= whole; b += kStride) {
-      Raw<T> next;
-      if (b + kStride <= whole) fetch<true>(next, t, b + kStride, end);
-      stepBlock<true>(r, t, step, b, end);
-      r = next;
-    }
-#pragma unroll 1
-    for (; b < end; b += kStride) {
-      fetch<false>(r, t, b, end);
-      stepBlock<false>(r, t, step, b, end);
-    }
+// What a CTA works on: elements [begin, end) of a tensor.
+template <class L> struct Chunk {
+  int tensor;
+  long long begin, end;
+  __device__ __forceinline__ explicit Chunk(const L& l) {
+    tensor = tensorOf(l, blockIdx.x);
+    begin = (long long)(blockIdx.x - (tensor ? l.end[tensor - 1] : 0)) * l.chunk;
+    end = min((long long)l.t[tensor].n, begin + l.chunk);
   }
+};
+__device__ __forceinline__ Step stepOf(const tcpxbAdamw& a, int tensor) {
+  const auto* s = static_cast<const Scratch*>(a.scratch);
+  return {float(a.beta1), float(a.beta2), float(1 - a.beta1), float(1 - a.beta2), float(a.eps), float(1 - a.lr * a.weight_decay),
+          s->rates[tensor].stepSize, s->rates[tensor].rootCorrection, s->coef};
+}
+__device__ __forceinline__ bool inVectors(const tcpxbAdamwTensor& t) { return aligned(t.p) && aligned(t.g) && aligned(t.m) && aligned(t.v) && aligned(t.master); }
+
+template <class T, class L> __global__ void __launch_bounds__(kThreads, 4) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
+  const Chunk<L> c(l);
+  const tcpxbAdamwTensor t = l.t[c.tensor];
+  const Step step = stepOf(a, l.first + c.tensor);
+  const long long whole = inVectors(t) ? c.begin + (c.end - c.begin) / 8 * 8 : c.begin;
+  stepVectors<T>(t, step, c.begin, whole);
+  stepElements<T>(t, step, whole, c.end);
+}
+
+template <class T, class W, class L> __global__ void __launch_bounds__(kSmallWarps * 32, sizeof(W) == 2 ? 8 : 4) stepSmallKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
+  __shared__ alignas(16) char shared[kSmallWarps * kStages * 32 * sizeof(Raw<T, W>)];
+  const Chunk<L> c(l);
+  const tcpxbAdamwTensor t = l.t[c.tensor];
+  const Step step = stepOf(a, l.first + c.tensor);
+  stepBlocks<T, W>(shared, t, step, c.begin, c.end, inVectors(t));
 }
 
 template <class T, class L> __global__ void __launch_bounds__(kThreads) squaresKernel(const __grid_constant__ L l, double* partial) {
-  const int i = tensorOf(l, blockIdx.x);
-  const long long begin = (long long)(blockIdx.x - (i ? l.end[i - 1] : 0)) * l.chunk;
-  const long long end = min((long long)l.t[i].n, begin + l.chunk);
-  const T* g = static_cast<const T*>(l.t[i].g);
+  const Chunk<L> c(l);
+  const long long begin = c.begin, end = c.end;
+  const T* g = static_cast<const T*>(l.t[c.tensor].g);
   // eight squares in 32 bits, those sums in 64: what rounding is left averages out
   double sum = 0;
   const long long whole = aligned(g) ? begin + (end - begin) / 8 * 8 : begin;
@@ -394,13 +458,23 @@ template <class F> int inLists(const tcpxbAdamwTensor* tensors, int count, F f) 
   return count <= 24 ? inLists<Short, 24>(tensors, count, f) : inLists<Long, 380>(tensors, count, f);
 }
 
+// Whether the first tensor with elements has 32-bit weights behind it.
+bool withMasters(const tcpxbAdamwTensor* t, int count) {
+  int i = 0;
+  while (i < count && !t[i].n) i++;
+  return i < count && t[i].master;
+}
+
 int check(const tcpxbAdamwTensor* t, int count, int dtype, bool step, int bits) {
   if (count < 0 || (count && !t)) return fail(TCPXB_T_INVALID, "null list");
   if (dtype != TCPXB_T_BF16 && dtype != TCPXB_T_F16 && dtype != TCPXB_T_F32) return fail(TCPXB_T_INVALID, "unknown type %d", dtype);
+  const bool masters = withMasters(t, count);
   for (int i = 0; i < count; i++) {
     if (t[i].n < 0 || t[i].n > (1ll << 43)) return fail(TCPXB_T_INVALID, "tensor %d has a bad size", i);
     if (t[i].n && !t[i].g) return fail(TCPXB_T_INVALID, "tensor %d has no gradient", i);
     if (!step) continue;
+    if (t[i].n && (bool(t[i].master) != masters || (t[i].master && dtype == TCPXB_T_F32)))
+      return fail(TCPXB_T_INVALID, "32-bit masters stand behind all tensors or none, of a 16-bit type (tensor %d)", i);
     if (!t[i].step || (t[i].n && (!t[i].p || !t[i].m || !t[i].v || (bits == 8 && (!t[i].m_scale || !t[i].v_scale)))))
       return fail(TCPXB_T_INVALID, "tensor %d lacks its weights, states, scales or step", i);
   }
@@ -419,6 +493,7 @@ template <class T> int squares(const tcpxbAdamwTensor* tensors, int count, doubl
 }
 
 template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw& a, cudaStream_t s) {
+  const bool masters = withMasters(tensors, count);
   double* partial = nullptr;
   long long partials = 0;
   if (a.compute_norm) {
@@ -430,8 +505,9 @@ template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tc
     prepareKernel<<<1, partials > 128 ? 512 : l.count <= 128 ? 128 : 384, 0, s>>>(l, a, partial, partials);
     if (const int rc = launched("adamw, rates")) return rc;
     if (!chunks) return int(TCPXB_T_OK);
-    if (a.state_bits == 8) stepKernel<T, L, true><<<unsigned(chunks), kThreads, 0, s>>>(l, a);
-    else stepKernel<T, L, false><<<unsigned(chunks), kThreads, 0, s>>>(l, a);
+    if (a.state_bits == 8 && masters) stepSmallKernel<T, float, L><<<unsigned(chunks), kSmallWarps * 32, 0, s>>>(l, a);
+    else if (a.state_bits == 8) stepSmallKernel<T, T, L><<<unsigned(chunks), kSmallWarps * 32, 0, s>>>(l, a);
+    else stepKernel<T, L><<<unsigned(chunks), kThreads, 0, s>>>(l, a);
     return launched("adamw");
   });
 }
