@@ -11,11 +11,16 @@
 // atomics: a gradient does not depend on the order in which blocks run, and no 32-bit copy of dq
 // goes through memory.
 //
-// All three kernels work on tiles of 128 x 128 scores.  One warp loads tiles with TMA, one thread
-// issues the matrix instructions, and the other eight warps turn scores into the operand of the
+// All three kernels work on tiles of scores, 128 rows high.  One warp loads tiles with TMA, one
+// thread issues the matrix instructions, and eight warps turn scores into the operand of the
 // next product, in tensor memory: the score tile is read into registers (a thread has one row, or
 // half of one) and P or dS is written back over it in 16 bits.  A head size under 64 or between
 // 64 and 128 fills its panel with zeros from the load.
+//
+// Head sizes above 64 take score tiles of 128 columns and one block on an SM: all of its tensor
+// memory.  Up to 64 the products are half as long while the exponentials stay, so what counts is
+// to keep the other units busy: tiles of 64 columns, half the tensor memory, two blocks on an SM
+// that fill each other's waits, and each other's beginnings and ends.
 //
 // Probabilities and score gradients are rounded to the inputs' type because the matrix units take
 // operands of one type; sums, statistics and everything else are 32-bit.
@@ -31,10 +36,25 @@ namespace {
 constexpr int kMaxD = 128;
 constexpr int kTile = 128;
 constexpr int kComputeWarps = 8, kLoadWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 384;  // the last two warps only complete a warpgroup
-// 384 threads get 168 registers each at launch: 2 x 128 x 208 + 128 x 80 is less than that
-constexpr int kComputeRegs = 208, kOtherRegs = 80;
-constexpr int kTmemCols = 512;
+
+// P: panels of 64 head elements.
+template <int P> struct Tiling {
+  static constexpr int kCols = P == 1 ? 64 : 128;  // of a score tile
+  static constexpr int kHalf = kCols / 2;          // those of a thread in the backward pass
+  static constexpr int kBlocks = P == 1 ? 2 : 1;   // on an SM
+  static constexpr int kTmem = P == 1 ? 256 : 512;
+  static constexpr int kHeadCols = P * 64;         // of a sum over scores
+  static constexpr uint32_t kRowTile = P * kPanelBytes, kColTile = P * kCols * 128;
+  // With one block the compute warps take registers from the others, for which two idle warps
+  // complete a third warpgroup: 2 x 128 x 208 + 128 x 80 is less than the 384 x 168 of the launch.
+  static constexpr int kThreads = P == 1 ? 320 : 384;
+  static __device__ __forceinline__ void compute() {
+    if constexpr (P == 2) moreRegisters<208>();
+  }
+  static __device__ __forceinline__ void other() {
+    if constexpr (P == 2) fewerRegisters<80>();
+  }
+};
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Args {
@@ -55,20 +75,25 @@ __device__ __forceinline__ int keysOf(const Args& a, int b) { return a.keyLength
 // Keys that query i sees, of `keys`.
 __device__ __forceinline__ int seenBy(const Args& a, int i, int keys) { return a.causal ? min(keys, max(0, i + a.sk - a.sq + 1)) : keys; }
 
-__device__ __forceinline__ int tiles(int n) { return (n + kTile - 1) / kTile; }
+template <int P> __device__ __forceinline__ int colTiles(int n) { return (n + Tiling<P>::kCols - 1) / Tiling<P>::kCols; }
 
-template <int P> __device__ __forceinline__ void loadTile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int batch) {
+// `R` rows in boxes of kCols.
+template <int P, int R> __device__ __forceinline__ void loadTile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int batch) {
+  constexpr int kBox = Tiling<P>::kCols;
 #pragma unroll
-  for (int p = 0; p < P; p++) tmaLoad(dst + p * kPanelBytes, map, bar, p * 64, row, head, batch);
+  for (int p = 0; p < P; p++)
+#pragma unroll
+    for (int r = 0; r < R; r += kBox) tmaLoad(dst + p * R * 128 + r * 128, map, bar, p * 64, row + r, head, batch);
 }
 
 // Rows from `first` on become zero: what lies behind a key length may hold anything, and zero
 // times NaN would reach the sums.  A warp does it between the load and the product that reads it.
 template <int P> __device__ __forceinline__ void clearRows(uint32_t tile, int first) {
-  for (int r = first * 8 + int(threadIdx.x % 32); r < kTile * 8; r += 32) {
+  constexpr int kCols = Tiling<P>::kCols;
+  for (int r = first * 8 + int(threadIdx.x % 32); r < kCols * 8; r += 32) {
 #pragma unroll
     for (int p = 0; p < P; p++)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + p * kPanelBytes + r * 16), "r"(0) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + p * kCols * 128 + r * 16), "r"(0) : "memory");
   }
   fenceAsyncShared();
   __syncwarp();
@@ -83,7 +108,7 @@ struct Shared {
 constexpr int kSharedBytes = 6144;
 static_assert(sizeof(Shared) <= kSharedBytes, "barriers and statistics");
 
-__device__ __forceinline__ void finish(const Args& a, uint32_t tmem, volatile int* dead) {
+template <int P> __device__ __forceinline__ void finish(const Args& a, uint32_t tmem, volatile int* dead) {
   tcBefore();
   __syncthreads();
   if (*dead) {
@@ -92,7 +117,7 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tmem, volatile in
     while (nowNs() - began < 1000000) __nanosleep(1000);
     if (threadIdx.x == 0 && a.status) atomicMax(a.status, kStatusTimeout);
   }
-  if (threadIdx.x / 32 == kMmaWarp) tmemFree(tmem, kTmemCols);
+  if (threadIdx.x / 32 == kMmaWarp) tmemFree(tmem, Tiling<P>::kTmem);
 }
 
 // Eight 32-bit values as one 16-byte store; by zero they are zeros, whatever they were.
@@ -128,17 +153,19 @@ template <class T> __device__ __forceinline__ void storeRow(T* row, bool live, u
 // than 2^8 since its last rescaling: probabilities then reach 2^8, which costs no precision.
 template <class T, int P> struct Forward {
   static constexpr int kSlots = P == 2 ? 4 : 8;  // tiles of keys and values in turn
-  static constexpr uint32_t kTileBytes = P * kPanelBytes;
-  static constexpr size_t kShared = kSharedBytes + 1024 + (2 + kSlots) * kTileBytes;
+  static constexpr uint32_t kTileBytes = Tiling<P>::kColTile, kQBytes = Tiling<P>::kRowTile;
+  static constexpr size_t kShared = kSharedBytes + 1024 + 2 * kQBytes + kSlots * kTileBytes;
   enum { kQFull = 0, kFull = 2, kEmpty = kFull + kSlots, kSFull = kEmpty + kSlots, kPFull = kSFull + 2, kOFull = kPFull + 2, kBars = kOFull + 2 };
 };
 
-template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forwardKernel(const __grid_constant__ Args a) {
+template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) forwardKernel(const __grid_constant__ Args a) {
   using F = Forward<T, P>;
+  using L = Tiling<P>;
+  constexpr int kCols = L::kCols;
   static_assert(F::kBars <= 32, "barriers");
   extern __shared__ char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
-  const uint32_t tile0 = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, ring = tile0 + 2 * F::kTileBytes;
+  const uint32_t tile0 = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, ring = tile0 + 2 * F::kQBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
@@ -147,7 +174,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
   const int keys = keysOf(a, b);
   int n[2];
 #pragma unroll
-  for (int t = 0; t < 2; t++) n[t] = q0 + t * kTile < a.sq ? tiles(seenBy(a, min(q0 + t * kTile + kTile, a.sq) - 1, keys)) : 0;
+  for (int t = 0; t < 2; t++) n[t] = q0 + t * kTile < a.sq ? colTiles<P>(seenBy(a, min(q0 + t * kTile + kTile, a.sq) - 1, keys)) : 0;
   const int most = max(n[0], n[1]);
 
   if (threadIdx.x == 0) {
@@ -155,48 +182,48 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
     sh.dead = 0;
     fenceBarInit();
   }
-  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), kTmemCols);
+  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), L::kTmem);
   tcBefore();
   __syncthreads();
   tcAfter();
   const uint32_t tmem = uniform(sh.tmem);
 
   if (warp == kLoadWarp) {
-    fewerRegisters<kOtherRegs>();
+    L::other();
     if (lane == 0) {
       for (int t = 0; t < 2; t++)
         if (n[t]) {
-          barExpect(bar(F::kQFull + t), F::kTileBytes);
-          loadTile<P>(tile0 + t * F::kTileBytes, &a.q, bar(F::kQFull + t), q0 + t * kTile, h, b);
+          barExpect(bar(F::kQFull + t), F::kQBytes);
+          loadTile<P, kTile>(tile0 + t * F::kQBytes, &a.q, bar(F::kQFull + t), q0 + t * kTile, h, b);
         }
       for (int i = 0; i < 2 * most; i++) {
         const int slot = i % F::kSlots, turn = i / F::kSlots;
         if (turn) barWait(bar(F::kEmpty + slot), (turn - 1) & 1, dead);
         barExpect(bar(F::kFull + slot), F::kTileBytes);
-        loadTile<P>(ring + slot * F::kTileBytes, i & 1 ? &a.v : &a.k, bar(F::kFull + slot), i / 2 * kTile, kv, b);
+        loadTile<P, kCols>(ring + slot * F::kTileBytes, i & 1 ? &a.v : &a.k, bar(F::kFull + slot), i / 2 * kCols, kv, b);
       }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    fewerRegisters<kOtherRegs>();
+    L::other();
     const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
-    const uint32_t scores = mmaShape<T>(kTile, false), values = mmaShape<T>(steps * 16, true);
+    const uint32_t scores = mmaShape<T>(kCols, false), values = mmaShape<T>(steps * 16, true);
     for (int j = 0; j <= most; j++) {
       const int ik = 2 * j, iv = 2 * j - 1;  // numbers of K_j and V_j-1
       const uint32_t kTileAt = ring + ik % F::kSlots * F::kTileBytes, vTileAt = ring + (iv + F::kSlots) % F::kSlots * F::kTileBytes;
       if (j < most) barWait(bar(F::kFull + ik % F::kSlots), ik / F::kSlots & 1, dead);
       if (j) {
         barWait(bar(F::kFull + iv % F::kSlots), iv / F::kSlots & 1, dead);
-        if (j * kTile > keys && keys < a.sk) clearRows<P>(vTileAt, keys - (j - 1) * kTile);
+        if (j * kCols > keys && keys < a.sk) clearRows<P>(vTileAt, keys - (j - 1) * kCols);
       }
       for (int t = 0; t < 2; t++) {
-        const uint32_t s = tmem + t * kTile, o = tmem + 2 * kTile + t * kMaxD;
+        const uint32_t s = tmem + t * kCols, o = tmem + 2 * kCols + t * L::kHeadCols;
         if (j && j <= n[t]) {
           barWait(bar(F::kPFull + t), (j - 1) & 1, dead);
           tcAfter();
           if (leader) {
-            mmaTmemTile<32>(o, s, vTileAt, values, j > 1);
+            mmaTmemTile<kCols, kCols / 4>(o, s, vTileAt, values, j > 1);
             if (j == n[t]) mmaCommit(bar(F::kOFull + t));
           }
         }
@@ -204,7 +231,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
           if (j == 0) barWait(bar(F::kQFull + t), 0, dead);
           if (leader) {
             // in issue order behind the product that reads P out of the same columns
-            mmaTiles<P>(s, tile0 + t * F::kTileBytes, kTileAt, scores, steps);
+            mmaTiles<P>(s, tile0 + t * F::kQBytes, kTileAt, scores, steps);
             mmaCommit(bar(F::kSFull + t));
           }
         }
@@ -217,30 +244,29 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
       __syncwarp();
     }
   } else if (warp < kComputeWarps) {
-    moreRegisters<kComputeRegs>();
+    L::compute();
     const int t = warp / 4, row = warp % 4 * 32 + lane, i = q0 + t * kTile + row;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
-    const uint32_t s = tmem + t * kTile + lanes, o = tmem + 2 * kTile + t * kMaxD + lanes;
+    const uint32_t s = tmem + t * kCols + lanes, o = tmem + 2 * kCols + t * L::kHeadCols + lanes;
     const float c = a.scale * kLog2e;
     const int seen = seenBy(a, i, keys);                       // of this row
-    const int whole = seenBy(a, q0 + t * kTile, keys) / kTile;  // tiles that every row sees whole
+    const int whole = seenBy(a, q0 + t * kTile, keys) / kCols;  // tiles that every row sees whole
     float top = -INFINITY;
     float2 sum2 = {0.f, 0.f};
     for (int j = 0; j < n[t]; j++) {
       barWait(bar(F::kSFull + t), j & 1, dead);
       tcAfter();
-      uint32_t x[kTile];
-#pragma unroll
-      for (int k = 0; k < kTile; k += 32) tmemLoad32(s + k, x + k);
+      uint32_t x[kCols];
+      tmemLoad<kCols>(s, x);
       tmemWaitLoad();
       if (j >= whole) {
-        const int left = seen - j * kTile;
+        const int left = seen - j * kCols;
 #pragma unroll
-        for (int k = 0; k < kTile; k++) x[k] = k < left ? x[k] : 0xff800000u;
+        for (int k = 0; k < kCols; k++) x[k] = k < left ? x[k] : 0xff800000u;
       }
       float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int k = 0; k < kTile; k += 8)
+      for (int k = 0; k < kCols; k += 8)
 #pragma unroll
         for (int u = 0; u < 4; u++) m[u] = max3(m[u], __uint_as_float(x[k + u]), __uint_as_float(x[k + 4 + u]));
       const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
@@ -250,28 +276,30 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
         if (grown) top = now;
         sum2 = mul2(sum2, {keep, keep});
         if (j) {
-          for (int k = 0; k < (a.d + 31) / 32 * 32; k += 32) {
-            uint32_t r[32];
-            tmemLoad32(o + k, r);
+#pragma unroll 1
+          for (int k = 0; k < a.d; k += 16) {
+            uint32_t r[16];
+            tmemLoad16(o + k, r);
             tmemWaitLoad();
 #pragma unroll
-            for (int u = 0; u < 32; u++) r[u] = __float_as_uint(__uint_as_float(r[u]) * keep);
-            tmemStore32(o + k, r);
+            for (int u = 0; u < 16; u++) r[u] = __float_as_uint(__uint_as_float(r[u]) * keep);
+            tmemStore16(o + k, r);
           }
         }
       }
+      constexpr int kRun = P == 1 ? 32 : 64;  // columns that are stored at once
       const float base = top == -INFINITY ? 0.f : -top * c;
 #pragma unroll
-      for (int k = 0; k < kTile; k += 64) {
-        uint32_t p[32];
+      for (int k = 0; k < kCols; k += kRun) {
+        uint32_t p[kRun / 2];
 #pragma unroll
-        for (int u = 0; u < 64; u += 2) {
+        for (int u = 0; u < kRun; u += 2) {
           float2 e = fma2({__uint_as_float(x[k + u]), __uint_as_float(x[k + u + 1])}, {c, c}, {base, base});
           e.x = exp2Fast(e.x), e.y = exp2Fast(e.y);
           sum2 = add2(sum2, e);
           p[u / 2] = pack2<T>(e.x, e.y);
         }
-        tmemStore32(s + k / 2, p);
+        tmemStore<kRun / 2>(s + k / 2, p);
       }
       tmemWaitStore();
       tcBefore();
@@ -290,82 +318,84 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) forward
     if (q0 + t * kTile < a.sq) storeRow(static_cast<T*>(a.o) + at, live, o, 0, kMaxD, a.d, by, n[t] > 0);
     if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
   } else {
-    fewerRegisters<kOtherRegs>();
+    L::other();
   }
-  finish(a, tmem, dead);
+  finish<P>(a, tmem, dead);
 }
 
 // ------------------------------------------------------------------ backward, queries
 // A block owns 128 queries and goes through the key tiles:  S = Q K^T, dP = dout V^T, then
 // dq += dS K.  Two buffers of scores: the next tile's exponentials start while the matrix units
-// still work on dP and dq of this one.  Both halves of the warps hold all rows, 64 keys each.
+// still work on dP and dq of this one.  Both halves of the warps hold all rows, each half of the tile's keys.
 // D_i is computed here and left for the other kernel: on the way in from dout and out; where all
 // keys of the block lie in one tile, as sum_j P_ij dP_ij, which it equals.  In so short a row the
 // rounding of out would be most of the gradients' error, and there the whole row is at hand.
 template <class T, int P> struct Queries {
-  static constexpr int kKSlots = 3, kVSlots = 2;
-  static constexpr uint32_t kTileBytes = P * kPanelBytes;
-  static constexpr size_t kShared = 1024 + 1024 + (2 + kKSlots + kVSlots) * kTileBytes;
+  static constexpr int kKSlots = P == 2 ? 3 : 5, kVSlots = P == 2 ? 2 : 3;
+  static constexpr uint32_t kTileBytes = Tiling<P>::kColTile, kQBytes = Tiling<P>::kRowTile;
+  static constexpr size_t kShared = 1024 + 1024 + 2 * kQBytes + (kKSlots + kVSlots) * kTileBytes;
   enum { kQFull = 0, kKFull = 1, kVFull = kKFull + kKSlots, kKEmpty = kVFull + kVSlots, kVEmpty = kKEmpty + kKSlots, kSFull = kVEmpty + kVSlots,
          kDpFull = kSFull + 2, kDsFull, kDone, kBars };
 };
 
 // A score that the row or key does not count for leaves exactly zero.
-template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKernel(const __grid_constant__ Args a) {
+template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) queryKernel(const __grid_constant__ Args a) {
   using F = Queries<T, P>;
+  using L = Tiling<P>;
+  constexpr int kCols = L::kCols, kHalf = L::kHalf;
   static_assert(F::kBars <= 32, "barriers");
   extern __shared__ char raw[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(raw);
   uint32_t* tmemAt = reinterpret_cast<uint32_t*>(raw + 256);
   volatile int* dead = reinterpret_cast<int*>(raw + 264);
   float* deltas = reinterpret_cast<float*>(raw + 512);
-  const uint32_t tile0 = (smemAddr(raw) + 1024 + 1023) / 1024 * 1024, qTile = tile0, doTile = tile0 + F::kTileBytes, kRing = tile0 + 2 * F::kTileBytes,
+  const uint32_t tile0 = (smemAddr(raw) + 1024 + 1023) / 1024 * 1024, qTile = tile0, doTile = tile0 + F::kQBytes, kRing = tile0 + 2 * F::kQBytes,
                  vRing = kRing + F::kKSlots * F::kTileBytes;
   const auto bar = [&](int i) { return smemAddr(bars) + 8 * i; };
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
-  const int keys = keysOf(a, b), n = tiles(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
+  const int keys = keysOf(a, b), n = colTiles<P>(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < F::kBars; i++) barInit(bar(i), i == F::kDsFull ? kComputeWarps : 1);
     *dead = 0;
     fenceBarInit();
   }
-  if (warp == kMmaWarp) tmemAlloc(smemAddr(tmemAt), kTmemCols);
+  if (warp == kMmaWarp) tmemAlloc(smemAddr(tmemAt), L::kTmem);
   tcBefore();
   __syncthreads();
   tcAfter();
-  const uint32_t tmem = uniform(*tmemAt), dp = tmem + 2 * kTile, dq = tmem + 3 * kTile;
+  const uint32_t tmem = uniform(*tmemAt), dp = tmem + 2 * kCols, dq = tmem + 3 * kCols;
 
   if (warp == kLoadWarp) {
-    fewerRegisters<kOtherRegs>();
+    L::other();
     if (lane == 0 && n) {
-      barExpect(bar(F::kQFull), 2 * F::kTileBytes);
-      loadTile<P>(qTile, &a.q, bar(F::kQFull), q0, h, b);
-      loadTile<P>(doTile, &a.dout, bar(F::kQFull), q0, h, b);
+      barExpect(bar(F::kQFull), 2 * F::kQBytes);
+      loadTile<P, kTile>(qTile, &a.q, bar(F::kQFull), q0, h, b);
+      loadTile<P, kTile>(doTile, &a.dout, bar(F::kQFull), q0, h, b);
       for (int j = 0; j < n; j++) {
         const int ks = j % F::kKSlots, vs = j % F::kVSlots;
         if (j >= F::kKSlots) barWait(bar(F::kKEmpty + ks), (j / F::kKSlots - 1) & 1, dead);
         barExpect(bar(F::kKFull + ks), F::kTileBytes);
-        loadTile<P>(kRing + ks * F::kTileBytes, &a.k, bar(F::kKFull + ks), j * kTile, kv, b);
+        loadTile<P, kCols>(kRing + ks * F::kTileBytes, &a.k, bar(F::kKFull + ks), j * kCols, kv, b);
         if (j >= F::kVSlots) barWait(bar(F::kVEmpty + vs), (j / F::kVSlots - 1) & 1, dead);
         barExpect(bar(F::kVFull + vs), F::kTileBytes);
-        loadTile<P>(vRing + vs * F::kTileBytes, &a.v, bar(F::kVFull + vs), j * kTile, kv, b);
+        loadTile<P, kCols>(vRing + vs * F::kTileBytes, &a.v, bar(F::kVFull + vs), j * kCols, kv, b);
       }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    fewerRegisters<kOtherRegs>();
+    L::other();
     const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
-    const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
+    const uint32_t scores = mmaShape<T>(kCols, false), back = mmaShape<T>(steps * 16, true);
     const auto score = [&](int j) {  // S of key tile j
       const int ks = j % F::kKSlots;
       const uint32_t kTileAt = kRing + ks * F::kTileBytes;
       barWait(bar(F::kKFull + ks), j / F::kKSlots & 1, dead);
-      if ((j + 1) * kTile > keys && keys < a.sk) clearRows<P>(kTileAt, keys - j * kTile);
+      if ((j + 1) * kCols > keys && keys < a.sk) clearRows<P>(kTileAt, keys - j * kCols);
       if (leader) {
-        mmaTiles<P>(tmem + (j & 1) * kTile, qTile, kTileAt, scores, steps);
+        mmaTiles<P>(tmem + (j & 1) * kCols, qTile, kTileAt, scores, steps);
         mmaCommit(bar(F::kSFull + (j & 1)));
       }
     };
@@ -389,7 +419,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
         if (j + 1 < n) gradient(j + 1);
         if (leader) {
           const int ks = j % F::kKSlots;
-          mmaTmemTile<64>(dq, tmem + (j & 1) * kTile, kRing + ks * F::kTileBytes, back, j > 0);
+          mmaTmemTile<kCols, kHalf>(dq, tmem + (j & 1) * kCols, kRing + ks * F::kTileBytes, back, j > 0);
           if (j + F::kKSlots < n) mmaCommit(bar(F::kKEmpty + ks));
           if (j == n - 1) mmaCommit(bar(F::kDone));
         }
@@ -398,7 +428,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       }
     }
   } else if (warp < kComputeWarps) {
-    moreRegisters<kComputeRegs>();
+    L::compute();
     const int half = warp / 4, row = warp % 4 * 32 + lane, i = q0 + row;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool live = i < a.sq;
@@ -424,31 +454,29 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
     // a row that sees nothing, or lies behind the last query, has no probabilities
     float l = live ? a.lse[stat] * -kLog2e : -INFINITY;
     if (l == INFINITY) l = -INFINITY;
-    const int seen = live ? seenBy(a, i, keys) : 0, whole = seenBy(a, q0, keys) / kTile;
+    const int seen = live ? seenBy(a, i, keys) : 0, whole = seenBy(a, q0, keys) / kCols;
     for (int j = 0; j < n; j++) {
-      const uint32_t s = tmem + (j & 1) * kTile + half * 64 + lanes;
+      const uint32_t s = tmem + (j & 1) * kCols + half * kHalf + lanes;
       barWait(bar(F::kSFull + (j & 1)), j / 2 & 1, dead);
       tcAfter();
-      uint32_t x[64];
-      tmemLoad32(s, x);
-      tmemLoad32(s + 32, x + 32);
+      uint32_t x[kHalf];
+      tmemLoad<kHalf>(s, x);
       tmemWaitLoad();
 #pragma unroll
-      for (int k = 0; k < 64; k += 2) {
+      for (int k = 0; k < kHalf; k += 2) {
         const float2 e = fma2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, {c, c}, {l, l});
         x[k] = __float_as_uint(exp2Fast(e.x)), x[k + 1] = __float_as_uint(exp2Fast(e.y));
       }
       barWait(bar(F::kDpFull), j & 1, dead);
       tcAfter();
-      uint32_t y[64], ds[32];
-      tmemLoad32(dp + half * 64 + lanes, y);
-      tmemLoad32(dp + half * 64 + lanes + 32, y + 32);
+      uint32_t y[kHalf], ds[kHalf / 2];
+      tmemLoad<kHalf>(dp + half * kHalf + lanes, y);
       tmemWaitLoad();
-      const int left = seen - j * kTile - half * 64;
+      const int left = seen - j * kCols - half * kHalf;
       if (n == 1) {
         float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < 64; k++)
+        for (int k = 0; k < kHalf; k++)
           if (k < left) sum += __uint_as_float(x[k]) * __uint_as_float(y[k]);
         asm volatile("bar.sync 1, 256;" ::: "memory");  // everybody has read the zeros
         if (half) deltas[row] = sum;
@@ -464,7 +492,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       }
       const auto gradients = [&](auto masked) {
 #pragma unroll
-        for (int k = 0; k < 64; k += 2) {
+        for (int k = 0; k < kHalf; k += 2) {
           float2 g = add2({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, {-delta, -delta});
           g = mul2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, g);
           if (decltype(masked)::value) {
@@ -476,7 +504,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       };
       if (j < whole) gradients(std::false_type());
       else gradients(std::true_type());
-      tmemStore32(s, ds);
+      tmemStore<kHalf / 2>(s, ds);
       tmemWaitStore();
       tcBefore();
       __syncwarp();
@@ -486,11 +514,11 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
       barWait(bar(F::kDone), 0, dead);
       tcAfter();
     }
-    storeRow(static_cast<T*>(a.dq) + at, live, dq + lanes, half * 64, half * 64 + 64, a.d, seen > 0 ? a.scale : 0.f, n > 0);
+    storeRow(static_cast<T*>(a.dq) + at, live, dq + lanes, half * L::kHeadCols / 2, (half + 1) * L::kHeadCols / 2, a.d, seen > 0 ? a.scale : 0.f, n > 0);
   } else {
-    fewerRegisters<kOtherRegs>();
+    L::other();
   }
-  finish(a, tmem, dead);
+  finish<P>(a, tmem, dead);
 }
 
 // ------------------------------------------------------------------ backward, keys
@@ -500,24 +528,26 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) queryKe
 // the next scores.
 template <class T, int P> struct Keys {
   static constexpr int kStages = P == 2 ? 2 : 4;
-  static constexpr uint32_t kTileBytes = P * kPanelBytes;
-  static constexpr size_t kShared = kSharedBytes + 1024 + (2 + 2 * kStages) * kTileBytes;
+  static constexpr uint32_t kTileBytes = Tiling<P>::kColTile, kKBytes = Tiling<P>::kRowTile;
+  static constexpr size_t kShared = kSharedBytes + 1024 + 2 * kKBytes + 2 * kStages * kTileBytes;
   enum { kKvFull = 0, kFull = 1, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kDpFull, kPFull, kDsFull, kDone, kBars };
 };
 
-template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKernel(const __grid_constant__ Args a) {
+template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) keyKernel(const __grid_constant__ Args a) {
   using F = Keys<T, P>;
+  using L = Tiling<P>;
+  constexpr int kCols = L::kCols, kHalf = L::kHalf;
   static_assert(F::kBars <= 32 && F::kStages <= 4, "barriers");
   extern __shared__ char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
-  const uint32_t kTileAt = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, vTileAt = kTileAt + F::kTileBytes, ring = vTileAt + F::kTileBytes;
+  const uint32_t kTileAt = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, vTileAt = kTileAt + F::kKBytes, ring = vTileAt + F::kKBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   const int j0 = blockIdx.z * kTile, kv = blockIdx.x, b = blockIdx.y, group = a.heads / a.kvHeads;
   const int keys = keysOf(a, b);
-  const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kTile : 0;  // first query tile that sees a key of this one
-  const int each = j0 < keys ? max(0, tiles(a.sq) - first) : 0, n = each * group;
+  const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kCols : 0;  // first query tile that sees a key of this one
+  const int each = j0 < keys ? max(0, colTiles<P>(a.sq) - first) : 0, n = each * group;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < F::kBars; i++)
@@ -525,25 +555,25 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
     sh.dead = 0;
     fenceBarInit();
   }
-  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), kTmemCols);
+  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), L::kTmem);
   tcBefore();
   __syncthreads();
   tcAfter();
-  const uint32_t tmem = uniform(sh.tmem), s = tmem, dp = tmem + kTile, dv = tmem + 2 * kTile, dk = tmem + 3 * kTile;
+  const uint32_t tmem = uniform(sh.tmem), s = tmem, dp = tmem + kCols, dv = tmem + 2 * kCols, dk = dv + L::kHeadCols;
 
   if (warp == kLoadWarp) {
-    fewerRegisters<kOtherRegs>();
+    L::other();
     if (lane == 0 && n) {
-      barExpect(bar(F::kKvFull), 2 * F::kTileBytes);
-      loadTile<P>(kTileAt, &a.k, bar(F::kKvFull), j0, kv, b);
-      loadTile<P>(vTileAt, &a.v, bar(F::kKvFull), j0, kv, b);
+      barExpect(bar(F::kKvFull), 2 * F::kKBytes);
+      loadTile<P, kTile>(kTileAt, &a.k, bar(F::kKvFull), j0, kv, b);
+      loadTile<P, kTile>(vTileAt, &a.v, bar(F::kKvFull), j0, kv, b);
     }
     for (int it = 0, h = kv * group, qt = 0; it < n; it++) {
-      const int st = it % F::kStages, turn = it / F::kStages, q0 = (first + qt) * kTile;
+      const int st = it % F::kStages, turn = it / F::kStages, q0 = (first + qt) * kCols;
       const long long stat = ((long long)b * a.heads + h) * a.sq;
-      float l[4], d[4];
+      float l[kCols / 32], d[kCols / 32];
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
+      for (int u = 0; u < kCols / 32; u++) {
         const int i = q0 + u * 32 + lane;
         l[u] = i < a.sq ? a.lse[stat + i] * -kLog2e : -INFINITY;
         if (l[u] == INFINITY) l[u] = -INFINITY;
@@ -553,20 +583,20 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
       if (lane == 0) {
         const uint32_t q = ring + 2 * st * F::kTileBytes;
         barExpect(bar(F::kFull + st), 2 * F::kTileBytes);
-        loadTile<P>(q, &a.q, bar(F::kFull + st), q0, h, b);
-        loadTile<P>(q + F::kTileBytes, &a.dout, bar(F::kFull + st), q0, h, b);
+        loadTile<P, kCols>(q, &a.q, bar(F::kFull + st), q0, h, b);
+        loadTile<P, kCols>(q + F::kTileBytes, &a.dout, bar(F::kFull + st), q0, h, b);
       }
 #pragma unroll
-      for (int u = 0; u < 4; u++) sh.stats[st][0][u * 32 + lane] = l[u], sh.stats[st][1][u * 32 + lane] = d[u];
+      for (int u = 0; u < kCols / 32; u++) sh.stats[st][0][u * 32 + lane] = l[u], sh.stats[st][1][u * 32 + lane] = d[u];
       barArrive(bar(F::kFull + st));
       if (++qt == each) qt = 0, h++;
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    fewerRegisters<kOtherRegs>();
+    L::other();
     const bool leader = electOne();
     const int steps = (a.d + 15) / 16;
-    const uint32_t scores = mmaShape<T>(kTile, false), back = mmaShape<T>(steps * 16, true);
+    const uint32_t scores = mmaShape<T>(kCols, false), back = mmaShape<T>(steps * 16, true);
     if (n) {
       barWait(bar(F::kKvFull), 0, dead);
       for (int it = -1; it < n; it++) {
@@ -575,7 +605,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
         if (it >= 0) {
           barWait(bar(F::kPFull), it & 1, dead);
           tcAfter();
-          if (leader) mmaTmemTile<64>(dv, s, q + F::kTileBytes, back, it > 0);
+          if (leader) mmaTmemTile<kCols, kHalf>(dv, s, q + F::kTileBytes, back, it > 0);
         }
         if (it + 1 < n) {
           barWait(bar(F::kFull + next), (it + 1) / F::kStages & 1, dead);
@@ -588,7 +618,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
           barWait(bar(F::kDsFull), it & 1, dead);
           tcAfter();
           if (leader) {
-            mmaTmemTile<64>(dk, dp, q, back, it > 0);
+            mmaTmemTile<kCols, kHalf>(dk, dp, q, back, it > 0);
             if (it + F::kStages < n) mmaCommit(bar(F::kEmpty + st));
             if (it == n - 1) mmaCommit(bar(F::kDone));
           }
@@ -601,29 +631,28 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
       }
     }
   } else if (warp < kComputeWarps) {
-    moreRegisters<kComputeRegs>();
+    L::compute();
     const int half = warp / 4, row = warp % 4 * 32 + lane, j = j0 + row;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool counts = j < keys;
     const float c = a.scale * kLog2e;
     for (int it = 0, qt = 0; it < n; it++) {
-      const int st = it % F::kStages, q0 = (first + qt) * kTile;
+      const int st = it % F::kStages, q0 = (first + qt) * kCols;
       if (++qt == each) qt = 0;
-      const float4* l = reinterpret_cast<const float4*>(sh.stats[st][0] + half * 64);
-      const float4* d = reinterpret_cast<const float4*>(sh.stats[st][1] + half * 64);
+      const float4* l = reinterpret_cast<const float4*>(sh.stats[st][0] + half * kHalf);
+      const float4* d = reinterpret_cast<const float4*>(sh.stats[st][1] + half * kHalf);
       // first query of this half that sees the row's key
-      const int from = !counts ? 64 : a.causal ? j - (a.sk - a.sq) - q0 - half * 64 : 0;
+      const int from = !counts ? kHalf : a.causal ? j - (a.sk - a.sq) - q0 - half * kHalf : 0;
       const bool some = j0 + kTile > keys || (a.causal && j0 + kTile - 1 > q0 + a.sk - a.sq);
       barWait(bar(F::kFull + st), it / F::kStages & 1, dead);
       barWait(bar(F::kSFull), it & 1, dead);
       tcAfter();
-      uint32_t x[64], o[32];
-      tmemLoad32(s + half * 64 + lanes, x);
-      tmemLoad32(s + half * 64 + lanes + 32, x + 32);
+      uint32_t x[kHalf], o[kHalf / 2];
+      tmemLoad<kHalf>(s + half * kHalf + lanes, x);
       tmemWaitLoad();
       const auto probabilities = [&](auto masked) {
 #pragma unroll
-        for (int k = 0; k < 64; k += 4) {
+        for (int k = 0; k < kHalf; k += 4) {
           const float4 ll = l[k / 4];
           const float2 ls[2] = {{ll.x, ll.y}, {ll.z, ll.w}};
 #pragma unroll
@@ -641,7 +670,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
       };
       if (some) probabilities(std::true_type());
       else probabilities(std::false_type());
-      tmemStore32(s + half * 64 + lanes, o);
+      tmemStore<kHalf / 2>(s + half * kHalf + lanes, o);
       tmemWaitStore();
       tcBefore();
       __syncwarp();
@@ -649,13 +678,12 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
 
       barWait(bar(F::kDpFull), it & 1, dead);
       tcAfter();
-      uint32_t y[64];
-      tmemLoad32(dp + half * 64 + lanes, y);
-      tmemLoad32(dp + half * 64 + lanes + 32, y + 32);
+      uint32_t y[kHalf];
+      tmemLoad<kHalf>(dp + half * kHalf + lanes, y);
       tmemWaitLoad();
       const auto gradients = [&](auto masked) {
 #pragma unroll
-        for (int k = 0; k < 64; k += 4) {
+        for (int k = 0; k < kHalf; k += 4) {
           const float4 dd = d[k / 4];
           const float2 ds[2] = {{dd.x, dd.y}, {dd.z, dd.w}};
 #pragma unroll
@@ -672,7 +700,7 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
       };
       if (some) gradients(std::true_type());
       else gradients(std::false_type());
-      tmemStore32(dp + half * 64 + lanes, o);
+      tmemStore<kHalf / 2>(dp + half * kHalf + lanes, o);
       tmemWaitStore();
       tcBefore();
       __syncwarp();
@@ -684,12 +712,12 @@ template <class T, int P> __global__ void __launch_bounds__(kThreads, 1) keyKern
     }
     const bool live = j < a.sk;
     const long long at = (((long long)b * a.sk + j) * a.kvHeads + kv) * a.d;
-    storeRow(static_cast<T*>(a.dv) + at, live, dv + lanes, half * 64, half * 64 + 64, a.d, counts ? 1.f : 0.f, n > 0);
-    storeRow(static_cast<T*>(a.dk) + at, live, dk + lanes, half * 64, half * 64 + 64, a.d, counts ? a.scale : 0.f, n > 0);
+    storeRow(static_cast<T*>(a.dv) + at, live, dv + lanes, half * L::kHeadCols / 2, (half + 1) * L::kHeadCols / 2, a.d, counts ? 1.f : 0.f, n > 0);
+    storeRow(static_cast<T*>(a.dk) + at, live, dk + lanes, half * L::kHeadCols / 2, (half + 1) * L::kHeadCols / 2, a.d, counts ? a.scale : 0.f, n > 0);
   } else {
-    fewerRegisters<kOtherRegs>();
+    L::other();
   }
-  finish(a, tmem, dead);
+  finish<P>(a, tmem, dead);
 }
 
 // ------------------------------------------------------------------ host
@@ -706,7 +734,7 @@ Encode encoder() {
   return f;
 }
 
-int makeMap(CUtensorMap* map, const char* name, const tcpxbHeads& x, int b, int s, int heads, int d, int dtype) {
+int makeMap(CUtensorMap* map, const char* name, const tcpxbHeads& x, int b, int s, int heads, int d, int rows, int dtype) {
   std::memset(map, 0, sizeof(*map));
   if ((long long)b * s == 0) return TCPXB_T_OK;  // nothing is loaded
   const Encode encode = encoder();
@@ -715,7 +743,7 @@ int makeMap(CUtensorMap* map, const char* name, const tcpxbHeads& x, int b, int 
   cuuint64_t strides[3] = {cuuint64_t(x.stride_s) * 2, cuuint64_t(x.stride_h) * 2, cuuint64_t(x.stride_b) * 2};
   for (int i = 0; i < 3; i++)
     if (dims[i + 1] == 1) strides[i] = 256;  // of no influence
-  const cuuint32_t box[4] = {64, kTile, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, cuuint32_t(rows), 1, 1}, ones[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, dtype == TCPXB_T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, x.ptr, dims, strides, box,
                             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -744,11 +772,11 @@ int check(const tcpxbAttention* a, bool backward) {
   return TCPXB_T_OK;
 }
 
-int makeArgs(const tcpxbAttention& a, bool backward, Args* x) {
-  int rc = makeMap(&x->q, "q", a.q, a.b, a.sq, a.heads, a.d, a.dtype);
-  if (!rc) rc = makeMap(&x->k, "k", a.k, a.b, a.sk, a.kv_heads, a.d, a.dtype);
-  if (!rc) rc = makeMap(&x->v, "v", a.v, a.b, a.sk, a.kv_heads, a.d, a.dtype);
-  if (!rc && backward) rc = makeMap(&x->dout, "dout", a.dout, a.b, a.sq, a.heads, a.d, a.dtype);
+int makeArgs(const tcpxbAttention& a, bool backward, int rows, Args* x) {
+  int rc = makeMap(&x->q, "q", a.q, a.b, a.sq, a.heads, a.d, rows, a.dtype);
+  if (!rc) rc = makeMap(&x->k, "k", a.k, a.b, a.sk, a.kv_heads, a.d, rows, a.dtype);
+  if (!rc) rc = makeMap(&x->v, "v", a.v, a.b, a.sk, a.kv_heads, a.d, rows, a.dtype);
+  if (!rc && backward) rc = makeMap(&x->dout, "dout", a.dout, a.b, a.sq, a.heads, a.d, rows, a.dtype);
   if (rc) return rc;
   x->out = x->o = a.out;
   x->doutPtr = a.dout.ptr;
@@ -760,7 +788,7 @@ int makeArgs(const tcpxbAttention& a, bool backward, Args* x) {
 }
 
 // Once for each kernel and device the block's shared memory is allowed; more than 64 devices would only ask again.
-template <void (*kKernel)(Args)> int launch(dim3 grid, size_t shared, const Args& a, int device, cudaStream_t s, const char* what) {
+template <void (*kKernel)(Args)> int launch(dim3 grid, int threads, size_t shared, const Args& a, int device, cudaStream_t s, const char* what) {
   static std::atomic<uint64_t> allowed{0};
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   if (!(allowed.load(std::memory_order_relaxed) & bit)) {
@@ -768,7 +796,7 @@ template <void (*kKernel)(Args)> int launch(dim3 grid, size_t shared, const Args
     if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  kKernel<<<grid, kThreads, shared, s>>>(a);
+  kKernel<<<grid, threads, shared, s>>>(a);
   return launched(what);
 }
 
@@ -779,17 +807,17 @@ template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaSt
   if (e == cudaSuccess) e = cudaSetDevice(device);
   if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "attention: %s", cudaGetErrorString(e));
   Args x;
-  if (const int rc = makeArgs(a, backward, &x)) return rc;
+  if (const int rc = makeArgs(a, backward, Tiling<P>::kCols, &x)) return rc;
   if (!backward) {
     if (!a.b || !a.sq) return TCPXB_T_OK;
-    return launch<forwardKernel<T, P>>(dim3(a.heads, a.b, (a.sq + 2 * kTile - 1) / (2 * kTile)), Forward<T, P>::kShared, x, device, s, "attention forward");
+    return launch<forwardKernel<T, P>>(dim3(a.heads, a.b, (a.sq + 2 * kTile - 1) / (2 * kTile)), Tiling<P>::kThreads, Forward<T, P>::kShared, x, device, s, "attention forward");
   }
   if (a.b && a.sq)
-    if (const int rc = launch<queryKernel<T, P>>(dim3(a.heads, a.b, (a.sq + kTile - 1) / kTile), Queries<T, P>::kShared, x, device, s,
+    if (const int rc = launch<queryKernel<T, P>>(dim3(a.heads, a.b, (a.sq + kTile - 1) / kTile), Tiling<P>::kThreads, Queries<T, P>::kShared, x, device, s,
                                                  "attention backward, queries"))
       return rc;
   if (!a.b || !a.sk) return TCPXB_T_OK;
-  return launch<keyKernel<T, P>>(dim3(a.kv_heads, a.b, (a.sk + kTile - 1) / kTile), Keys<T, P>::kShared, x, device, s, "attention backward, keys");
+  return launch<keyKernel<T, P>>(dim3(a.kv_heads, a.b, (a.sk + kTile - 1) / kTile), Tiling<P>::kThreads, Keys<T, P>::kShared, x, device, s, "attention backward, keys");
 }
 
 int dispatch(const tcpxbAttention* a, bool backward, void* stream) {

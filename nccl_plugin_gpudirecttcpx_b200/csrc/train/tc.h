@@ -68,7 +68,7 @@ __device__ __forceinline__ void barWait(uint32_t bar, uint32_t parity, volatile 
   barWaitLong(bar, parity, dead);
 }
 
-// ---- TMA: a box of 64 elements by 128 rows of [head size, tokens, heads, batch], 128-byte swizzle
+// ---- TMA: a box of 64 elements by 64 or 128 rows of [head size, tokens, heads, batch], 128-byte swizzle
 __device__ __forceinline__ void tmaLoad(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int row, int head, int batch) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
@@ -118,6 +118,31 @@ __device__ __forceinline__ void tmemStore32(uint32_t at, const uint32_t* r) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmemStore16(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmemLoad16(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+template <int N> __device__ __forceinline__ void tmemLoad(uint32_t at, uint32_t* r) {
+  static_assert(N % 32 == 0, "columns");
+#pragma unroll
+  for (int k = 0; k < N; k += 32) tmemLoad32(at + k, r + k);
+}
+template <int N> __device__ __forceinline__ void tmemStore(uint32_t at, const uint32_t* r) {
+  static_assert(N == 16 || N == 32, "columns");
+  if constexpr (N == 32) tmemStore32(at, r);
+  else tmemStore16(at, r);
+}
+
 // ---- matrix instructions: D[128 x n] (+)= A[128 x 16] B[n x 16], 32-bit sums
 template <class T> struct MmaType;
 template <> struct MmaType<__half> { static constexpr uint32_t code = 0; };
@@ -158,12 +183,12 @@ template <int P> __device__ __forceinline__ void mmaTiles(uint32_t d, uint32_t a
     if (k < steps) mma(d, da + off, db + off, shape, k > 0);
   }
 }
-// d (+)= A B over 128 rows of B: A lies in tensor memory, two elements a column, in two runs of 32
-// columns that begin `half` columns apart; B's rows are the summed index.
-template <int kHalf> __device__ __forceinline__ void mmaTmemTile(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, bool add) {
-  const uint64_t db = operandDesc(b, kPanelBytes);
+// d (+)= A B over the K rows of B, the summed index: A lies in tensor memory, two elements a
+// column, in two runs of K / 4 columns that begin kHalf columns apart.
+template <int K, int kHalf> __device__ __forceinline__ void mmaTmemTile(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, bool add) {
+  const uint64_t db = operandDesc(b, K * 128);
 #pragma unroll
-  for (int k = 0; k < 8; k++) mmaFromTmem(d, a + k / 4 * kHalf + k % 4 * 8, db + k * (2048 >> 4), shape, add || k > 0);
+  for (int k = 0; k < K / 16; k++) mmaFromTmem(d, a + k / (K / 32) * kHalf + k % (K / 32) * 8, db + k * (2048 >> 4), shape, add || k > 0);
 }
 // The barrier gets one arrival when all matrix instructions that this thread has issued are done.
 __device__ __forceinline__ void mmaCommit(uint32_t bar) {
