@@ -632,80 +632,94 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
     }
   } else if (warp < kComputeWarps) {
     L::compute();
-    const int half = warp / 4, row = warp % 4 * 32 + lane, j = j0 + row;
+    const int half = warp / 4;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
-    const bool counts = j < keys;
     const float c = a.scale * kLog2e;
+    // Scores are read in blocks of 16 lanes by 8 columns: a thread has two columns of each block,
+    // whose statistics it reads from shared memory once for four rows.  (With a row to a thread
+    // every statistic went to every thread, and reading them took as long as the exponentials.)
+    constexpr int kBlocks8 = kHalf / 8, kRegs = kHalf / 2;
+    const int row0 = warp % 4 * 32 + lane / 4, col0 = lane % 4 * 2;
     for (int it = 0, qt = 0; it < n; it++) {
       const int st = it % F::kStages, q0 = (first + qt) * kCols;
       if (++qt == each) qt = 0;
-      const float4* l = reinterpret_cast<const float4*>(sh.stats[st][0] + half * kHalf);
-      const float4* d = reinterpret_cast<const float4*>(sh.stats[st][1] + half * kHalf);
-      // first query of this half that sees the row's key
-      const int from = !counts ? kHalf : a.causal ? j - (a.sk - a.sq) - q0 - half * kHalf : 0;
+      const float* l = sh.stats[st][0] + half * kHalf + col0;
+      const float* d = sh.stats[st][1] + half * kHalf + col0;
+      // first column of the half that sees key j0 + row, less the thread's first
+      const int edge = a.causal ? j0 - (a.sk - a.sq) - q0 - half * kHalf - col0 : -kTile - kCols;
       const bool some = j0 + kTile > keys || (a.causal && j0 + kTile - 1 > q0 + a.sk - a.sq);
+      const auto from = [&](int row) { return j0 + row < keys ? edge + row : kCols; };
       barWait(bar(F::kFull + st), it / F::kStages & 1, dead);
       barWait(bar(F::kSFull), it & 1, dead);
       tcAfter();
-      uint32_t x[kHalf], o[kHalf / 2];
-      tmemLoad<kHalf>(s + half * kHalf + lanes, x);
+      uint32_t x[2][kRegs];
+      tmemLoadBlocks<kRegs>(s + half * kHalf + lanes, x[0]);
+      tmemLoadBlocks<kRegs>(s + half * kHalf + lanes + (16 << 16), x[1]);
       tmemWaitLoad();
       const auto probabilities = [&](auto masked) {
 #pragma unroll
-        for (int k = 0; k < kHalf; k += 4) {
-          const float4 ll = l[k / 4];
-          const float2 ls[2] = {{ll.x, ll.y}, {ll.z, ll.w}};
+        for (int k = 0; k < kBlocks8; k++) {
+          const float2 ls = *reinterpret_cast<const float2*>(l + k * 8);
 #pragma unroll
-          for (int u = k; u < k + 4; u += 2) {
-            float2 e = fma2({__uint_as_float(x[u]), __uint_as_float(x[u + 1])}, {c, c}, ls[(u - k) / 2]);
+          for (int u = 0; u < 4; u++) {  // rows row0 + 8 u
+            uint32_t* v = x[u / 2] + k * 4 + u % 2 * 2;
+            float2 e = fma2({__uint_as_float(v[0]), __uint_as_float(v[1])}, {c, c}, ls);
             e.x = exp2Fast(e.x), e.y = exp2Fast(e.y);
             if (decltype(masked)::value) {
-              e.x = u >= from ? e.x : 0.f;
-              e.y = u + 1 >= from ? e.y : 0.f;
+              e.x = k * 8 >= from(row0 + u * 8) ? e.x : 0.f;
+              e.y = k * 8 + 1 >= from(row0 + u * 8) ? e.y : 0.f;
             }
-            x[u] = __float_as_uint(e.x), x[u + 1] = __float_as_uint(e.y);
-            o[u / 2] = pack2<T>(e.x, e.y);
+            v[0] = __float_as_uint(e.x), v[1] = __float_as_uint(e.y);
           }
         }
       };
       if (some) probabilities(std::true_type());
       else probabilities(std::false_type());
-      tmemStore<kHalf / 2>(s + half * kHalf + lanes, o);
-      tmemWaitStore();
-      tcBefore();
-      __syncwarp();
+      const auto store = [&](uint32_t at) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          uint32_t o[kRegs / 2];
+#pragma unroll
+          for (int k = 0; k < kRegs / 2; k++) o[k] = pack2<T>(__uint_as_float(x[r][2 * k]), __uint_as_float(x[r][2 * k + 1]));
+          tmemStoreBlocks<kRegs / 2>(at + half * kHalf + lanes + (r * 16 << 16), o);
+        }
+        tmemWaitStore();
+        tcBefore();
+        __syncwarp();
+      };
+      store(s);
       if (lane == 0) barArrive(bar(F::kPFull));
 
       barWait(bar(F::kDpFull), it & 1, dead);
       tcAfter();
-      uint32_t y[kHalf];
-      tmemLoad<kHalf>(dp + half * kHalf + lanes, y);
+      uint32_t y[2][kRegs];
+      tmemLoadBlocks<kRegs>(dp + half * kHalf + lanes, y[0]);
+      tmemLoadBlocks<kRegs>(dp + half * kHalf + lanes + (16 << 16), y[1]);
       tmemWaitLoad();
       const auto gradients = [&](auto masked) {
 #pragma unroll
-        for (int k = 0; k < kHalf; k += 4) {
-          const float4 dd = d[k / 4];
-          const float2 ds[2] = {{dd.x, dd.y}, {dd.z, dd.w}};
+        for (int k = 0; k < kBlocks8; k++) {
+          const float2 ds = *reinterpret_cast<const float2*>(d + k * 8);
 #pragma unroll
-          for (int u = k; u < k + 4; u += 2) {
-            float2 g = add2({__uint_as_float(y[u]), __uint_as_float(y[u + 1])}, ds[(u - k) / 2]);
-            g = mul2({__uint_as_float(x[u]), __uint_as_float(x[u + 1])}, g);
+          for (int u = 0; u < 4; u++) {
+            uint32_t *v = x[u / 2] + k * 4 + u % 2 * 2, *w = y[u / 2] + k * 4 + u % 2 * 2;
+            float2 g = add2({__uint_as_float(w[0]), __uint_as_float(w[1])}, ds);
+            g = mul2({__uint_as_float(v[0]), __uint_as_float(v[1])}, g);
             if (decltype(masked)::value) {
-              g.x = u >= from ? g.x : 0.f;
-              g.y = u + 1 >= from ? g.y : 0.f;
+              g.x = k * 8 >= from(row0 + u * 8) ? g.x : 0.f;
+              g.y = k * 8 + 1 >= from(row0 + u * 8) ? g.y : 0.f;
             }
-            o[u / 2] = pack2<T>(g.x, g.y);
+            v[0] = __float_as_uint(g.x), v[1] = __float_as_uint(g.y);
           }
         }
       };
       if (some) gradients(std::true_type());
       else gradients(std::false_type());
-      tmemStore<kHalf / 2>(dp + half * kHalf + lanes, o);
-      tmemWaitStore();
-      tcBefore();
-      __syncwarp();
+      store(dp);
       if (lane == 0) barArrive(bar(F::kDsFull));
     }
+    const int row = warp % 4 * 32 + lane, j = j0 + row;
+    const bool counts = j < keys;
     if (n) {
       barWait(bar(F::kDone), 0, dead);
       tcAfter();

@@ -143,6 +143,41 @@ template <int N> __device__ __forceinline__ void tmemStore(uint32_t at, const ui
   else tmemStore16(at, r);
 }
 
+// The other arrangement: 16 lanes by 8 columns, of which thread i holds columns 2 (i % 4) and the
+// next, of lanes i / 4 and i / 4 + 8: r[4b .. 4b + 3] are those four of column block b.  `at` names
+// the first of the 16 lanes.  N registers, 2 N columns.
+template <int N> __device__ __forceinline__ void tmemLoadBlocks(uint32_t at, uint32_t* r) {
+  static_assert(N == 16 || N == 32, "registers");
+  if constexpr (N == 16)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+  else
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+// Back in 16 bits: 16 lanes by 4 columns of two elements each; r[2b] and r[2b + 1] are thread i's
+// pair of block b in lanes i / 4 and i / 4 + 8.
+template <int N> __device__ __forceinline__ void tmemStoreBlocks(uint32_t at, const uint32_t* r) {
+  static_assert(N == 8 || N == 16, "registers");
+  if constexpr (N == 8)
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  else
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
 // ---- matrix instructions: D[128 x n] (+)= A[128 x 16] B[n x 16], 32-bit sums
 template <class T> struct MmaType;
 template <> struct MmaType<__half> { static constexpr uint32_t code = 0; };
