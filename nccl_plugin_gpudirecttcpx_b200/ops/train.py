@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
 from typing import Optional, Sequence
 
@@ -32,36 +33,40 @@ _NORM_ROPE = struct.Struct("@8q7P8q5P6ifi")
 _ADAMW = struct.Struct("@5dPf3iP")
 
 
-_lib = None
+_entries: dict = {}
 
 
 def _t():
-    global _lib
-    if _lib is None:
-        lib = native.load("libtcpxb_train.so")
-        lib.tcpxb_train_last_error.restype = ctypes.c_char_p
-        for name in ("tcpxb_attention_forward", "tcpxb_attention_backward", "tcpxb_norm_rope_forward", "tcpxb_norm_rope_backward"):
-            getattr(lib, name).argtypes = [_vp, _vp]
-        lib.tcpxb_norm_rope_scratch_bytes.restype = ctypes.c_size_t
-        lib.tcpxb_adamw_scratch_bytes.argtypes = [_vp, ctypes.c_int]
-        lib.tcpxb_adamw_scratch_bytes.restype = ctypes.c_size_t
-        lib.tcpxb_adamw_step.argtypes = [_vp, ctypes.c_int, _vp, _vp]
-        lib.tcpxb_grad_norm_scratch_bytes.argtypes = [_vp, ctypes.c_int]
-        lib.tcpxb_grad_norm_scratch_bytes.restype = ctypes.c_size_t
-        lib.tcpxb_grad_norm.argtypes = [_vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]
-        _lib = lib
-    return _lib
+    return native.load("libtcpxb_train.so")
+
+
+def _entry(name: str):
+    """A C entry with its signature."""
+    if not _entries:
+        lib = _t()
+        size, text, i32 = ctypes.c_size_t, ctypes.c_char_p, ctypes.c_int
+        for entry, result, *args in (
+                ("tcpxb_train_last_error", text),
+                ("tcpxb_attention_forward", i32, _vp, _vp), ("tcpxb_attention_backward", i32, _vp, _vp),
+                ("tcpxb_norm_rope_forward", i32, _vp, _vp), ("tcpxb_norm_rope_backward", i32, _vp, _vp), ("tcpxb_norm_rope_scratch_bytes", size, i32),
+                ("tcpxb_adamw_scratch_bytes", size, _vp, i32), ("tcpxb_adamw_step", i32, _vp, i32, _vp, _vp),
+                ("tcpxb_grad_norm_scratch_bytes", size, _vp, i32), ("tcpxb_grad_norm", i32, _vp, i32, i32, _vp, _vp, _vp)):
+            f = getattr(lib, entry)
+            f.restype, f.argtypes = result, args
+            _entries[entry] = f
+    return _entries[name]
 
 
 def _call(name: str, device: int, *args) -> None:
     """Runs a C entry on the tensors' device, whichever is current, and on that device's current stream."""
+    entry = _entries.get(name) or _entry(name)
     if torch._C._cuda_getDevice() == device:
-        rc = getattr(_t(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            rc = getattr(_t(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     if rc != 0:
-        raise RuntimeError(f"{name} failed ({rc}): {_t().tcpxb_train_last_error().decode()}")
+        raise RuntimeError(f"{name} failed ({rc}): {_entry('tcpxb_train_last_error')().decode()}")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -107,16 +112,16 @@ def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 # ------------------------------------------------------------------- attention
-def _check_attention(q, k, v, scale, key_lengths) -> float:
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"{name} has to be [batch, tokens, heads, head size], got {tuple(t.shape)}")
+def _check_attention(q, k, v, scale, key_lengths) -> tuple:
+    """(batch, queries, keys, heads, key heads, head size, scale)."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k and v have to be [batch, tokens, heads, head size], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     dtype = q.dtype
     if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError(f"attention takes bfloat16 or float16 of one kind, got {dtype}, {k.dtype}, {v.dtype}")
-    b, _, h, d = q.shape
-    kb, _, hk, kd = k.shape
-    if k.shape != v.shape or kb != b or kd != d:
+    b, sq, h, d = q.shape
+    kb, sk, hk, kd = k.shape
+    if kb != b or kd != d or v.shape != k.shape:
         raise ValueError(f"shapes do not match: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if h < 1 or hk < 1 or h % hk:
         raise ValueError(f"{h} query heads are no multiple of {hk} key heads")
@@ -130,7 +135,7 @@ def _check_attention(q, k, v, scale, key_lengths) -> float:
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0 < scale < 1e30:
         raise ValueError(f"scale has to be finite and above zero, got {scale}")
-    return scale
+    return b, sq, sk, h, hk, d, scale
 
 
 def _check_status(status: Optional[torch.Tensor]) -> None:
@@ -151,11 +156,9 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
     (float32) is the natural logarithm of each row's sum of exponentials, -inf for an empty row.
     `status` (`ops.status_buffer()`): its first word becomes 3 where a wait inside the kernel ran out of
     time and the outputs are void."""
-    scale = _check_attention(q, k, v, scale, key_lengths)
+    b, sq, sk, h, hk, d, scale = _check_attention(q, k, v, scale, key_lengths)
     _check_status(status)
     dev = _on_one_device(q, k, v, key_lengths, status)
-    b, sq, h, d = q.shape
-    sk, hk = k.shape[1:3]
     out, lse = q.new_empty((b, sq, h, d)), q.new_empty((b, h, sq), dtype=torch.float32)
     q, *qa = _heads(q, 8)
     k, *ka = _heads(k, 8)
@@ -172,9 +175,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                        status: Optional[torch.Tensor] = None) -> tuple:
     """(dq, dk, dv) from what `attention_forward` returned for the same arguments.  The probabilities
     are computed again from the scores and `lse`.  The same inputs give the same bits every time."""
-    scale = _check_attention(q, k, v, scale, key_lengths)
-    b, sq, h, d = q.shape
-    sk, hk = k.shape[1:3]
+    b, sq, sk, h, hk, d, scale = _check_attention(q, k, v, scale, key_lengths)
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape:
             raise ValueError(f"{name} has to be {tuple(q.shape)}, got {tuple(t.shape)}")
@@ -226,45 +227,49 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
 
 # ---------------------------------------------------------------- qk_norm_rope
-def _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions) -> None:
-    for name, t in (("q", q), ("k", k)):
-        if t.dim() != 4:
-            raise ValueError(f"{name} has to be [batch, tokens, heads, head size], got {tuple(t.shape)}")
-    if q.dtype not in _CODES or k.dtype != q.dtype:
-        raise TypeError(f"q and k have to be bfloat16, float16 or float32 of one kind, got {q.dtype} and {k.dtype}")
+def _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions) -> tuple:
+    """(batch, tokens, heads, key heads, head size, rows of the tables)."""
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"q and k have to be [batch, tokens, heads, head size], got {tuple(q.shape)} and {tuple(k.shape)}")
+    dtype = q.dtype
+    if dtype not in _CODES or k.dtype is not dtype:
+        raise TypeError(f"q and k have to be bfloat16, float16 or float32 of one kind, got {dtype} and {k.dtype}")
     b, s, h, d = q.shape
-    if k.shape[:2] != q.shape[:2] or k.shape[3] != d or h < 1 or k.shape[2] < 1:
+    kb, ks, hk, kd = k.shape
+    if kb != b or ks != s or kd != d or h < 1 or hk < 1:
         raise ValueError(f"shapes do not match: q {tuple(q.shape)}, k {tuple(k.shape)}")
     if d % 8 or not 8 <= d <= MAX_NORM_HEAD_SIZE:
         raise ValueError(f"the head size has to be a multiple of 8 up to {MAX_NORM_HEAD_SIZE}, got {d}")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise TypeError(f"cos and sin have to be float32, got {cos.dtype} and {sin.dtype}")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != d // 2:
+    table = cos.shape
+    if len(table) != 2 or sin.shape != table or table[1] != d // 2:
         raise ValueError(f"cos and sin have to be [positions, {d // 2}], got {tuple(cos.shape)} and {tuple(sin.shape)}")
     if positions is None:
-        if cos.shape[0] < s:
-            raise ValueError(f"the tables hold {cos.shape[0]} positions of {s}")
+        if table[0] < s:
+            raise ValueError(f"the tables hold {table[0]} positions of {s}")
     else:
-        if positions.dtype != torch.int64:
+        if positions.dtype is not torch.int64:
             raise TypeError(f"positions has to be int64, got {positions.dtype}")
         if positions.shape != (b, s):
             raise ValueError(f"positions has to be [{b}, {s}], got {tuple(positions.shape)}")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("q_weight and k_weight come together")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and w.shape != (d,):
-            raise ValueError(f"{name} has to be [{d}], got {tuple(w.shape)}")
-        if w is not None and w.dtype != q.dtype:
-            raise TypeError(f"{name} has to be {q.dtype}, got {w.dtype}")
+    if q_weight is not None:
+        if q_weight.shape != (d,) or k_weight.shape != (d,):
+            raise ValueError(f"the weights have to be [{d}], got {tuple(q_weight.shape)} and {tuple(k_weight.shape)}")
+        if q_weight.dtype is not dtype or k_weight.dtype is not dtype:
+            raise TypeError(f"the weights have to be {dtype}, got {q_weight.dtype} and {k_weight.dtype}")
     if not 0 <= eps < math.inf:
         raise ValueError(f"eps has to be finite and not below zero, got {eps}")
+    return b, s, h, hk, d, table[0]
 
 
 def _norm_rope_forward(q, k, cos, sin, q_weight, k_weight, eps, positions) -> tuple:
-    _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions)
+    b, s, h, hk, d, rows = _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions)
     dev = _on_one_device(q, k, cos, sin, q_weight, k_weight, positions)
-    b, s, h, d = q.shape
-    hk, per = k.shape[2], 16 // q.element_size()
+    code = _CODES[q.dtype]
+    per = 4 if code == 2 else 8
     q_out, k_out = q.new_empty((b, s, h, d)), k.new_empty((b, s, hk, d))
     cos, sin, q_weight, k_weight = _aligned(cos), _aligned(sin), _aligned(q_weight), _aligned(k_weight)
     if positions is not None:
@@ -273,7 +278,7 @@ def _norm_rope_forward(q, k, cos, sin, q_weight, k_weight, eps, positions) -> tu
     k, *ka = _heads(k, per)
     _call("tcpxb_norm_rope_forward", dev, _NORM_ROPE.pack(*qa, *ka, _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), _ptr(positions),
                                                           q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, b, s, h, hk, d,
-                                                          cos.shape[0], eps, _CODES[q.dtype]))
+                                                          rows, eps, code))
     return q_out, k_out
 
 
@@ -282,21 +287,21 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
                           eps: float = 1e-6, positions: Optional[torch.Tensor] = None) -> tuple:
     """(dq, dk, dq_weight, dk_weight) of `qk_norm_rope` from the gradients of its outputs and its own
     arguments (the weights' are None without weights).  The same inputs give the same bits every time."""
-    _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions)
+    b, s, h, hk, d, rows = _check_norm_rope(q, k, cos, sin, q_weight, k_weight, eps, positions)
     for name, t, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
         if t.shape != x.shape:
             raise ValueError(f"{name} has to be {tuple(x.shape)}, got {tuple(t.shape)}")
         if t.dtype is not x.dtype:
             raise TypeError(f"{name} has to be {x.dtype}, got {t.dtype}")
     dev = _on_one_device(dq_out, dk_out, q, k, cos, sin, q_weight, k_weight, positions)
-    b, s, h, d = q.shape
-    hk, per = k.shape[2], 16 // q.element_size()
+    code = _CODES[q.dtype]
+    per = 4 if code == 2 else 8
     dq, dk = q.new_empty((b, s, h, d)), k.new_empty((b, s, hk, d))
     dwq = dwk = partial = None
     qa = ka = (0, 0, 0, 0)
     if q_weight is not None:
         dwq, dwk = q_weight.new_empty((d,)), k_weight.new_empty((d,))
-        partial = cos.new_empty(_t().tcpxb_norm_rope_scratch_bytes(d) // 4)
+        partial = cos.new_empty(_entry("tcpxb_norm_rope_scratch_bytes")(d) // 4)
         q, *qa = _heads(q, per)
         k, *ka = _heads(k, per)
     cos, sin, q_weight, k_weight = _aligned(cos), _aligned(sin), _aligned(q_weight), _aligned(k_weight)
@@ -306,7 +311,7 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     dk_out, *dka = _heads(dk_out, per)
     _call("tcpxb_norm_rope_backward", dev, _NORM_ROPE.pack(*qa, *ka, _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), _ptr(positions), 0, 0,
                                                            *dqa, *dka, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk), _ptr(partial), b, s, h, hk, d,
-                                                           cos.shape[0], eps, _CODES[dq.dtype]))
+                                                           rows, eps, code))
     return dq, dk, dwq, dwk
 
 
@@ -339,28 +344,31 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     float32) turn the pairs (x[2i], x[2i + 1]); token t of a batch takes row t, or row `positions[b, t]`
     (int64).  A position outside the tables gives NaN.  Without weights there is no norm.  All in 32 bits,
     rounded once; outputs are contiguous."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or
+                                    (k_weight is not None and k_weight.requires_grad)):
         return _NormRopeFunction.apply(q, k, cos, sin, q_weight, k_weight, eps, positions)
     return _norm_rope_forward(q, k, cos, sin, q_weight, k_weight, eps, positions)
 
 
 # ----------------------------------------------------------------------- AdamW
+_data_ptr, _numel, _is_contiguous, _get_device = (getattr(torch.Tensor, n) for n in ("data_ptr", "numel", "is_contiguous", "get_device"))
+_dtype = operator.attrgetter("dtype")
+
+
 def _flat_list(name: str, ts: Sequence[torch.Tensor], numels: Sequence[int], dtype: torch.dtype, device: int) -> list:
     """The tensors' addresses; `device`: -1 stands for the CPU, where the arguments are all that can be checked."""
     if len(ts) != len(numels):
         raise ValueError(f"{len(numels)} tensors, but {len(ts)} {name}")
-    at = []
-    for i, t in enumerate(ts):
-        if t.dtype is not dtype:
-            raise TypeError(f"{name}[{i}] has to be {dtype}, got {t.dtype}")
-        if t.numel() != numels[i]:
-            raise ValueError(f"{name}[{i}] has {t.numel()} elements")
-        if not t.is_contiguous():
-            raise ValueError(f"{name}[{i}] has to be contiguous")
-        if t.get_device() != device:
-            raise ValueError(f"{name}[{i}] is on another device")
-        at.append(t.data_ptr())
-    return at
+    if set(map(_dtype, ts)) != {dtype}:
+        raise TypeError(f"{name} have to be {dtype}, got {set(map(_dtype, ts))}")
+    if list(map(_numel, ts)) != numels:
+        i = next(i for i, t in enumerate(ts) if t.numel() != numels[i])
+        raise ValueError(f"{name}[{i}] has {ts[i].numel()} elements, not {numels[i]}")
+    if not all(map(_is_contiguous, ts)):
+        raise ValueError(f"{name} have to be contiguous")
+    if set(map(_get_device, ts)) != {device}:
+        raise ValueError(f"{name} are on another device")
+    return list(map(_data_ptr, ts))
 
 
 def _table(*columns: Sequence[int]) -> ctypes.Array:
@@ -379,13 +387,13 @@ def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     dtype = grads[0].dtype
     if dtype not in _CODES:
         raise TypeError(f"gradients have to be bfloat16, float16 or float32, got {dtype}")
-    numels = [g.numel() for g in grads]
+    numels = list(map(_numel, grads))
     at = _flat_list("grads", grads, numels, dtype, grads[0].get_device())
     dev = _on_one_device(grads[0])
     none = [0] * len(grads)
     table = _table(none, at, none, none, none, none, none, none, numels)
     norm = grads[0].new_empty((), dtype=torch.float32)
-    scratch = grads[0].new_empty(_t().tcpxb_grad_norm_scratch_bytes(table, len(grads)), dtype=torch.uint8)
+    scratch = grads[0].new_empty(_entry("tcpxb_grad_norm_scratch_bytes")(table, len(grads)), dtype=torch.uint8)
     _call("tcpxb_grad_norm", dev, table, len(grads), _CODES[dtype], norm.data_ptr(), scratch.data_ptr())
     return norm
 
@@ -416,7 +424,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if (exp_avg_sq_scales is None) != (bits == 32):
         raise ValueError("8-bit states need the scales of both")
     count, device = len(params), params[0].get_device()
-    numels = [p.numel() for p in params]
+    numels = list(map(_numel, params))
     p_at = _flat_list("params", params, numels, dtype, device)
     g_at = _flat_list("grads", grads, numels, dtype, device)
     state = torch.float8_e4m3fn if bits == 8 else torch.float32
@@ -456,7 +464,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     compute = max_grad_norm is not None and norm is None
     if compute:
         norm = steps.new_empty((), dtype=torch.float32)
-    scratch = steps.new_empty(_t().tcpxb_adamw_scratch_bytes(table, count), dtype=torch.uint8)
+    scratch = steps.new_empty(_entry("tcpxb_adamw_scratch_bytes")(table, count), dtype=torch.uint8)
     _call("tcpxb_adamw_step", dev, table, count, _ADAMW.pack(lr, beta1, beta2, eps, weight_decay, _ptr(norm), max_grad_norm or 0.0, compute, bits,
                                                              _CODES[dtype], scratch.data_ptr()))
     return norm

@@ -259,6 +259,7 @@ def test_the_c_entry_refuses():
     import ctypes
     import train_abi as A
     from nccl_plugin_gpudirecttcpx_b200.ops import train as T
+    T._entry("tcpxb_train_last_error")  # sets the signatures
     lib = T._t()
     assert ctypes.sizeof(A.Adamw) == T._ADAMW.size
     t = (A.AdamwTensor * 1)(A.AdamwTensor(4096, 4096, 4096, 4096, None, None, None, 4096, 10))
