@@ -3,8 +3,10 @@
 The transport does not care what the gradients belong to; this model only has to
 produce the traffic pattern of a real step: 16 layers, d_model 2048, 32 query heads
 over 8 KV heads, SwiGLU FFN of 8192, vocabulary 128256, rotary embeddings, bf16,
-random initialisation.  Plain PyTorch on purpose (fused attention from
-torch.nn.functional); the code under test is the gradient all_reduce below it.
+random initialisation.  By default plain PyTorch (fused attention from
+torch.nn.functional); the code under test is the gradient all_reduce below it.  With
+`kernels` the decoder runs this package's own operators: norms of queries and keys with
+the position rotation in one pass, and attention forward and backward.
 """
 from __future__ import annotations
 
@@ -13,6 +15,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .. import ops
 
 
 @dataclass
@@ -26,6 +30,8 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     norm_eps: float = 1e-5
     tie_embeddings: bool = True
+    qk_norm: bool = False  # norm of every query and key head, before the rotation
+    kernels: bool = False  # ops.qk_norm_rope and ops.attention (CUDA, bfloat16 or float16)
 
     @staticmethod
     def tiny() -> "LlamaConfig":
@@ -67,12 +73,26 @@ class Attention(nn.Module):
         self.wk = nn.Linear(cfg.d_model, self.kv * self.d, bias=False)
         self.wv = nn.Linear(cfg.d_model, self.kv * self.d, bias=False)
         self.wo = nn.Linear(self.h * self.d, cfg.d_model, bias=False)
+        self.kernels, self.eps = cfg.kernels, cfg.norm_eps
+        self.q_norm = RMSNorm(self.d, cfg.norm_eps) if cfg.qk_norm else None
+        self.k_norm = RMSNorm(self.d, cfg.norm_eps) if cfg.qk_norm else None
+
+    def _forward_kernels(self, x, cos, sin):
+        B, S, _ = x.shape
+        q, k, v = (w(x).view(B, S, -1, self.d) for w in (self.wq, self.wk, self.wv))
+        weights = (None, None) if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
+        q, k = ops.qk_norm_rope(q, k, cos, sin, *weights, eps=self.eps)
+        return self.wo(ops.attention(q, k, v, causal=True).view(B, S, self.h * self.d))
 
     def forward(self, x, cos, sin):
+        if self.kernels:
+            return self._forward_kernels(x, cos, sin)
         B, S, _ = x.shape
         q = self.wq(x).view(B, S, self.h, self.d).transpose(1, 2)
         k = self.wk(x).view(B, S, self.kv, self.d).transpose(1, 2)
         v = self.wv(x).view(B, S, self.kv, self.d).transpose(1, 2)
+        if self.q_norm is not None:
+            q, k = self.q_norm(q), self.k_norm(k)
         q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         rep = self.h // self.kv
         k = k.repeat_interleave(rep, dim=1)
@@ -117,7 +137,8 @@ class LlamaDecoder(nn.Module):
     def forward(self, tokens, targets=None):
         B, S = tokens.shape
         x = self.embed(tokens)
-        cos, sin = rope_tables(S, self.cfg.d_model // self.cfg.n_heads, self.cfg.rope_theta, x.device, x.dtype)
+        # the kernels take the tables in 32 bits
+        cos, sin = rope_tables(S, self.cfg.d_model // self.cfg.n_heads, self.cfg.rope_theta, x.device, torch.float32 if self.cfg.kernels else x.dtype)
         for layer in self.layers:
             x = layer(x, cos, sin)
         logits = self.lm_head(self.norm(x))

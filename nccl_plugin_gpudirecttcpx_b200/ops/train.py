@@ -399,7 +399,7 @@ def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
-               exp_avg_sqs: Sequence[torch.Tensor], steps: torch.Tensor, *, lr: float, betas: tuple = (0.9, 0.999), eps: float = 1e-8,
+               exp_avg_sqs: Sequence[torch.Tensor], steps, *, lr: float, betas: tuple = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, max_grad_norm: Optional[float] = None, norm: Optional[torch.Tensor] = None,
                exp_avg_scales: Optional[Sequence[torch.Tensor]] = None, exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
                masters: Optional[Sequence[torch.Tensor]] = None) -> Optional[torch.Tensor]:
@@ -408,8 +408,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     `params` and `grads`: contiguous tensors of one type (bfloat16, float16, float32) on one device.
     States in 32 bits: `exp_avgs` and `exp_avg_sqs` are float32 tensors of the params' sizes.  In 8 bits:
     float8_e4m3fn tensors with `exp_avg_scales` and `exp_avg_sq_scales`, one float32 per 256 elements; a
-    state's value is code times scale, and `exp_avg_sqs` holds the root.  `steps` ([number of tensors],
-    int32) counts each tensor's updates and is advanced.  `max_grad_norm`: gradients are scaled by
+    state's value is code times scale, and `exp_avg_sqs` holds the root.  `steps` (an int32 tensor with an
+    entry for each of them, or a list of one-element ones) counts each tensor's updates and is advanced.  `max_grad_norm`: gradients are scaled by
     min(1, max_grad_norm / (norm + 1e-6)), where `norm` is theirs over all tensors (computed here and
     returned), or the given float32 device scalar, for lists that share one.  `masters`: float32 weights
     that are updated and rounded into 16-bit `params`.  Nothing is copied to or from the host: the call can
@@ -443,10 +443,17 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             raise ValueError("masters stand behind 16-bit params")
         master_at = _flat_list("masters", list(masters), numels, torch.float32, device)
         written += master_at
-    if steps.dtype is not torch.int32:
-        raise TypeError(f"steps has to be int32, got {steps.dtype}")
-    if steps.shape != (count,) or not steps.is_contiguous():
-        raise ValueError(f"steps has to be a contiguous [{count}], got {tuple(steps.shape)}")
+    if isinstance(steps, torch.Tensor):
+        if steps.dtype is not torch.int32:
+            raise TypeError(f"steps has to be int32, got {steps.dtype}")
+        if steps.shape != (count,) or not steps.is_contiguous() or steps.get_device() != device:
+            raise ValueError(f"steps has to be a contiguous [{count}] on the same device, got {tuple(steps.shape)}")
+        step_at = steps.data_ptr()
+        step_at = range(step_at, step_at + 4 * count, 4)
+    else:
+        step_at = _flat_list("steps", list(steps), [1] * count, torch.int32, device)
+        if len(set(step_at)) != count:
+            raise ValueError("a step counter is given twice")
     if 0 in numels:  # a tensor without elements has no address of its own
         written = [x for x, n in zip(written, numels * (len(written) // count)) if n]
     if len(set(written)) != len(written):
@@ -458,13 +465,12 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError(f"max_grad_norm has to be finite and not below zero, got {max_grad_norm}")
     if norm is not None and (norm.dtype is not torch.float32 or norm.numel() != 1 or max_grad_norm is None):
         raise ValueError("norm has to be one float32 value, given with max_grad_norm")
-    dev = _on_one_device(params[0], steps, norm)
-    step_at = steps.data_ptr()
-    table = _table(p_at, g_at, m_at, v_at, ms_at, vs_at, master_at, range(step_at, step_at + 4 * count, 4), numels)
+    dev = _on_one_device(params[0], norm)
+    table = _table(p_at, g_at, m_at, v_at, ms_at, vs_at, master_at, step_at, numels)
     compute = max_grad_norm is not None and norm is None
     if compute:
-        norm = steps.new_empty((), dtype=torch.float32)
-    scratch = steps.new_empty(_entry("tcpxb_adamw_scratch_bytes")(table, count), dtype=torch.uint8)
+        norm = params[0].new_empty((), dtype=torch.float32)
+    scratch = params[0].new_empty(_entry("tcpxb_adamw_scratch_bytes")(table, count), dtype=torch.uint8)
     _call("tcpxb_adamw_step", dev, table, count, _ADAMW.pack(lr, beta1, beta2, eps, weight_decay, _ptr(norm), max_grad_norm or 0.0, compute, bits,
                                                              _CODES[dtype], scratch.data_ptr()))
     return norm

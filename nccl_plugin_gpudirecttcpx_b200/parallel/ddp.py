@@ -13,7 +13,9 @@ NVLink fan-out kernels) from a DDP communication hook; the hook queues buckets o
 engine's own thread and stream (`all_reduce_async`), so backward keeps running while
 buckets are on the wire.  Model, optimizer and bucketing are stock
 PyTorch: Llama-style decoder, AdamW, DistributedDataParallel with 25 MB buckets
-overlapped with backward.  Synthetic uniform token ids, random-init weights.
+overlapped with backward.  `--kernels` runs the step on this package's own operators instead:
+head norms with rotation (`--qk-norm`), attention and AdamW (`--state-bits`, `--max-grad-norm`).
+Synthetic uniform token ids, random-init weights.
 Rank 0 prints one JSON line with the device-timed step time (max over ranks).
 """
 from __future__ import annotations
@@ -41,7 +43,16 @@ def parse_args(argv=None):
     ap.add_argument("--nthreads", type=int, default=4)
     ap.add_argument("--engine-buffer-kb", type=int, default=0,
                     help="--transport engine, several GPUs per node: size of the symmetric buffers (0 = bucket cap + largest parameter); larger buckets travel in pieces")
-    return ap.parse_args(argv)
+    ap.add_argument("--qk-norm", action="store_true", help="norms of queries and keys in the model")
+    ap.add_argument("--kernels", action="store_true", help="the package's own attention, head norms with rotation and AdamW (nccl backend)")
+    ap.add_argument("--state-bits", type=int, default=32, choices=[8, 32], help="--kernels: AdamW states")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="--kernels: gradients are clipped to this norm")
+    args = ap.parse_args(argv)
+    if args.kernels and args.backend != "nccl":
+        ap.error("--kernels needs GPUs (--backend nccl)")
+    if not args.kernels and (args.state_bits != 32 or args.max_grad_norm is not None):
+        ap.error("--state-bits and --max-grad-norm belong to --kernels")
+    return args
 
 
 def setup_env(args, rank: int) -> None:
@@ -186,6 +197,7 @@ def main(argv=None) -> int:
         dist.init_process_group("gloo")
     torch.manual_seed(1234)  # same initial weights everywhere
     cfg = LlamaConfig.tiny() if args.tiny else LlamaConfig()
+    cfg.qk_norm, cfg.kernels = args.qk_norm, args.kernels
     dtype = torch.bfloat16 if use_cuda else torch.float32
     model = LlamaDecoder(cfg).to(device=dev, dtype=dtype)
     ddp = DDP(model, device_ids=[local] if use_cuda else None, bucket_cap_mb=args.bucket_mb, gradient_as_bucket_view=True)
@@ -193,7 +205,11 @@ def main(argv=None) -> int:
     if args.transport == "engine":
         reducer = make_engine_reducer(args, dev, world, model)
         ddp.register_comm_hook(None, reducer.hook)
-    opt = torch.optim.AdamW(ddp.parameters(), lr=1e-4, weight_decay=0.1, fused=use_cuda)
+    if args.kernels:
+        from .. import ops
+        opt = ops.AdamW(ddp.parameters(), lr=1e-4, weight_decay=0.1, state_bits=args.state_bits, max_grad_norm=args.max_grad_norm)
+    else:
+        opt = torch.optim.AdamW(ddp.parameters(), lr=1e-4, weight_decay=0.1, fused=use_cuda)
     seq = min(args.seq_len, 64) if args.tiny else args.seq_len
     gen = torch.Generator(device=dev).manual_seed(99 + rank)
 
@@ -241,7 +257,7 @@ def main(argv=None) -> int:
             "grad_bytes_per_step": n_params * (2 if use_cuda else 4), "bucket_mb": args.bucket_mb,
             "micro_batch": args.micro_batch, "seq_len": seq, "loss_first": losses[0], "loss_last": losses[-1],
             "replicas_in_sync": in_sync, "dtype": str(dtype), "data": "synthetic uniform token ids, random init",
-            "engine_buckets": reducer.buckets if reducer else None,
+            "engine_buckets": reducer.buckets if reducer else None, "kernels": args.kernels, "qk_norm": args.qk_norm,
         }), flush=True)
     if reducer is not None:
         if use_cuda:
