@@ -77,6 +77,14 @@ template <int G> __device__ __forceinline__ float groupSum(float x) {
   return x;
 }
 
+template <int G> __device__ __forceinline__ void groupSums(float& x, float& y) {
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+    y += __shfl_xor_sync(0xffffffffu, y, o);
+  }
+}
+
 // A lane's eight elements as four pairs.
 template <class T> __device__ __forceinline__ void pairs(const Vec8<T>& v, float2 (&f)[4]) {
 #pragma unroll
@@ -160,18 +168,19 @@ template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads
 #pragma unroll
       for (int k = 0; k < 4; k++) f[k] = {f[k].x * c[k] + f[k].y * s[k], f[k].y * c[k] - f[k].x * s[k]};
       if (kNorm) {
-        float2 xh[4], g[4];
-        pairs(rawX[i], xh);
-        const float r = rsqrtf(groupSum<G>(sum(xh, xh)) * j.perD + j.eps);
+        float2 x[4], g[4];
+        pairs(rawX[i], x);
+#pragma unroll
+        for (int k = 0; k < 4; k++) g[k] = mul2(f[k], w[k]);
+        // both sums go through the shuffles side by side: sum(g xh) = r sum(g x)
+        float squares = sum(x, x), mix = sum(g, x);
+        groupSums<G>(squares, mix);
+        const float r = rsqrtf(squares * j.perD + j.eps), back = -r * r * (mix * j.perD) * r;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          xh[k] = mul2(xh[k], {r, r});
-          g[k] = mul2(f[k], w[k]);
-          if (live) dw[k] = fma2(f[k], xh[k], dw[k]);
+          if (live) dw[k] = fma2(f[k], mul2(x[k], {r, r}), dw[k]);
+          f[k] = fma2(x[k], {back, back}, mul2(g[k], {r, r}));
         }
-        const float mean = -groupSum<G>(sum(g, xh)) * j.perD;
-#pragma unroll
-        for (int k = 0; k < 4; k++) f[k] = mul2(fma2(xh[k], {mean, mean}, g[k]), {r, r});
       }
       if (live) store(dx + i * (32 / G) * j.d, f);
     }

@@ -9,7 +9,9 @@ option is a `ValueError`, a wrong type a `TypeError`.
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import itertools
 import math
 import operator
 import struct
@@ -371,10 +373,9 @@ def _flat_list(name: str, ts: Sequence[torch.Tensor], numels: Sequence[int], dty
     return list(map(_data_ptr, ts))
 
 
-def _table(*columns: Sequence[int]) -> ctypes.Array:
+def _table(*columns: Sequence[int]) -> bytes:
     """The C entry's list of tensors: rows of nine words, from lists of each word."""
-    rows = [x for row in zip(*columns) for x in row]
-    return (ctypes.c_int64 * len(rows))(*rows)
+    return array.array("q", itertools.chain.from_iterable(zip(*columns))).tobytes()
 
 
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
