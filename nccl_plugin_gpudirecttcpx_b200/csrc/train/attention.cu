@@ -67,6 +67,7 @@ struct Args {
   const int32_t* keyLengths;
   int32_t* status;
   int b, sq, sk, heads, kvHeads, d, causal;
+  int split;  // blocks of a cluster that share a tile of keys
   float scale;
 };
 
@@ -108,6 +109,21 @@ struct Shared {
 constexpr int kSharedBytes = 6144;
 static_assert(sizeof(Shared) <= kSharedBytes, "barriers and statistics");
 
+// Begins a block: the load warp has initialised the barriers and goes on to its loads, the others
+// wait for that and for the tensor memory, and get its address.
+template <int P> __device__ __forceinline__ uint32_t begin(int warp, uint32_t* tmem) {
+  constexpr int kThreads = Tiling<P>::kThreads;
+  if (warp == kLoadWarp) {
+    asm volatile("bar.arrive 2, %0;" ::"n"(kThreads) : "memory");
+    return 0;
+  }
+  if (warp == kMmaWarp) tmemAlloc(smemAddr(tmem), Tiling<P>::kTmem);
+  tcBefore();
+  asm volatile("bar.sync 2, %0;" ::"n"(kThreads) : "memory");
+  tcAfter();
+  return uniform(*tmem);
+}
+
 template <int P> __device__ __forceinline__ void finish(const Args& a, uint32_t tmem, volatile int* dead) {
   tcBefore();
   __syncthreads();
@@ -120,8 +136,8 @@ template <int P> __device__ __forceinline__ void finish(const Args& a, uint32_t 
   if (threadIdx.x / 32 == kMmaWarp) tmemFree(tmem, Tiling<P>::kTmem);
 }
 
-// Eight 32-bit values as one 16-byte store; by zero they are zeros, whatever they were.
-template <class T> __device__ __forceinline__ void storeRow8(T* p, const uint32_t* r, float by) {
+// Eight 32-bit values as 16 bytes; by zero they are zeros, whatever they were.
+template <class T> __device__ __forceinline__ uint4 rounded8(const uint32_t* r, float by) {
   uint4 x = {};
   if (by != 0.f) {
     x.x = pack2<T>(__uint_as_float(r[0]) * by, __uint_as_float(r[1]) * by);
@@ -129,19 +145,38 @@ template <class T> __device__ __forceinline__ void storeRow8(T* p, const uint32_
     x.z = pack2<T>(__uint_as_float(r[4]) * by, __uint_as_float(r[5]) * by);
     x.w = pack2<T>(__uint_as_float(r[6]) * by, __uint_as_float(r[7]) * by);
   }
-  *reinterpret_cast<uint4*>(p) = x;
+  return x;
 }
-// Columns [begin, end) of the thread's accumulator row, times `by`; all threads of the warp come here.
-template <class T> __device__ __forceinline__ void storeRow(T* row, bool live, uint32_t tmem, int begin, int end, int d, float by, bool any) {
-  for (int c = begin; c < end && c < d; c += 32) {
+// A warp's 32 accumulator rows, kCols of their columns from `begin` on, times each lane's `by`, to
+// memory: row r goes to out + r * stride, where r < rows.  They are turned in `stage` (32 rows of
+// kCols 16-bit elements, a tile that is no longer needed), so that a row's lanes write side by
+// side; rows straight out of the lanes took 2000 to 4000 cycles of a block's end.
+template <class T, int kCols>
+__device__ __forceinline__ void storeRows(T* out, int64_t stride, int rows, uint32_t tmem, int begin, int d, float by, bool any, uint32_t stage) {
+  constexpr int kChunks = kCols / 8;  // of 16 bytes in a row
+  const int lane = threadIdx.x % 32;
+  // the chunks of a row change places by its number: eight lanes never meet in a bank
+  const auto place = [](int row, int c) { return uint32_t(row * kChunks + (c ^ (kChunks == 4 ? row / 2 % 4 : row % 8))) * 16; };
+#pragma unroll
+  for (int c = 0; c < kCols; c += 32) {
     uint32_t r[32] = {};
     if (any) {
-      tmemLoad32(tmem + c, r);
+      tmemLoad32(tmem + begin + c, r);
       tmemWaitLoad();
     }
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (live && c + i < d) storeRow8(row + c + i, r + i, by);
+    for (int i = 0; i < 4; i++) {
+      const uint4 x = rounded8<T>(r + i * 8, by);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + place(lane, c / 8 + i)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kChunks; i++) {
+    const int row = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(stage + place(row, c)) : "memory");
+    if (row < rows && begin + c * 8 < d) *reinterpret_cast<uint4*>(out + row * stride + begin + c * 8) = x;
   }
 }
 
@@ -177,17 +212,21 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
   for (int t = 0; t < 2; t++) n[t] = q0 + t * kTile < a.sq ? colTiles<P>(seenBy(a, min(q0 + t * kTile + kTile, a.sq) - 1, keys)) : 0;
   const int most = max(n[0], n[1]);
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < F::kBars; i++) barInit(bar(i), i >= F::kPFull && i < F::kOFull ? 4 : 1);
-    sh.dead = 0;
-    fenceBarInit();
+  const auto loadPair = [&](int i) {  // number i of K_0, V_0, K_1, ...
+    const int slot = i % F::kSlots;
+    barExpect(bar(F::kFull + slot), F::kTileBytes);
+    loadTile<P, kCols>(ring + slot * F::kTileBytes, i & 1 ? &a.v : &a.k, bar(F::kFull + slot), i / 2 * kCols, kv, b);
+  };
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < F::kBars; i++) barInit(bar(i), i >= F::kPFull && i < F::kOFull ? 4 : 1);
+      sh.dead = 0;
+      fenceBarInit();
+      fenceAsyncShared();
+    }
+    __syncwarp();
   }
-  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), L::kTmem);
-  tcBefore();
-  __syncthreads();
-  tcAfter();
-  const uint32_t tmem = uniform(sh.tmem);
-
+  const uint32_t tmem = begin<P>(warp, &sh.tmem);
   if (warp == kLoadWarp) {
     L::other();
     if (lane == 0) {
@@ -195,12 +234,11 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
         if (n[t]) {
           barExpect(bar(F::kQFull + t), F::kQBytes);
           loadTile<P, kTile>(tile0 + t * F::kQBytes, &a.q, bar(F::kQFull + t), q0 + t * kTile, h, b);
+          if (t == 0 || !n[0]) loadPair(0);
         }
-      for (int i = 0; i < 2 * most; i++) {
-        const int slot = i % F::kSlots, turn = i / F::kSlots;
-        if (turn) barWait(bar(F::kEmpty + slot), (turn - 1) & 1, dead);
-        barExpect(bar(F::kFull + slot), F::kTileBytes);
-        loadTile<P, kCols>(ring + slot * F::kTileBytes, i & 1 ? &a.v : &a.k, bar(F::kFull + slot), i / 2 * kCols, kv, b);
+      for (int i = 1; i < 2 * most; i++) {
+        if (i >= F::kSlots) barWait(bar(F::kEmpty + i % F::kSlots), (i / F::kSlots - 1) & 1, dead);
+        loadPair(i);
       }
     }
     __syncwarp();
@@ -312,10 +350,11 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
     }
     const float sum = sum2.x + sum2.y;
     const bool live = i < a.sq;
-    const long long at = (((long long)b * a.sq + i) * a.heads + h) * a.d;
     // a row that sees nothing is zero, whatever its tile holds
     const float by = seen > 0 ? 1.f / sum : 0.f;
-    if (q0 + t * kTile < a.sq) storeRow(static_cast<T*>(a.o) + at, live, o, 0, kMaxD, a.d, by, n[t] > 0);
+    const int i0 = i - lane;  // the warp's first row
+    storeRows<T, L::kHeadCols>(static_cast<T*>(a.o) + (((long long)b * a.sq + i0) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - i0, o, 0, a.d, by,
+                               n[t] > 0, tile0 + t * F::kQBytes + warp % 4 * (F::kQBytes / 4));
     if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
   } else {
     L::other();
@@ -356,31 +395,40 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
   const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
   const int keys = keysOf(a, b), n = colTiles<P>(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < F::kBars; i++) barInit(bar(i), i == F::kDsFull ? kComputeWarps : 1);
-    *dead = 0;
-    fenceBarInit();
+  const auto loadKeys = [&](int j) {
+    const int ks = j % F::kKSlots;
+    barExpect(bar(F::kKFull + ks), F::kTileBytes);
+    loadTile<P, kCols>(kRing + ks * F::kTileBytes, &a.k, bar(F::kKFull + ks), j * kCols, kv, b);
+  };
+  const auto loadValues = [&](int j) {
+    const int vs = j % F::kVSlots;
+    barExpect(bar(F::kVFull + vs), F::kTileBytes);
+    loadTile<P, kCols>(vRing + vs * F::kTileBytes, &a.v, bar(F::kVFull + vs), j * kCols, kv, b);
+  };
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < F::kBars; i++) barInit(bar(i), i == F::kDsFull ? kComputeWarps : 1);
+      *dead = 0;
+      fenceBarInit();
+      fenceAsyncShared();
+    }
+    __syncwarp();
   }
-  if (warp == kMmaWarp) tmemAlloc(smemAddr(tmemAt), L::kTmem);
-  tcBefore();
-  __syncthreads();
-  tcAfter();
-  const uint32_t tmem = uniform(*tmemAt), dp = tmem + 2 * kCols, dq = tmem + 3 * kCols;
+  const uint32_t tmem = begin<P>(warp, tmemAt), dp = tmem + 2 * kCols, dq = tmem + 3 * kCols;
 
   if (warp == kLoadWarp) {
     L::other();
     if (lane == 0 && n) {
       barExpect(bar(F::kQFull), 2 * F::kQBytes);
       loadTile<P, kTile>(qTile, &a.q, bar(F::kQFull), q0, h, b);
+      loadKeys(0);
       loadTile<P, kTile>(doTile, &a.dout, bar(F::kQFull), q0, h, b);
-      for (int j = 0; j < n; j++) {
-        const int ks = j % F::kKSlots, vs = j % F::kVSlots;
-        if (j >= F::kKSlots) barWait(bar(F::kKEmpty + ks), (j / F::kKSlots - 1) & 1, dead);
-        barExpect(bar(F::kKFull + ks), F::kTileBytes);
-        loadTile<P, kCols>(kRing + ks * F::kTileBytes, &a.k, bar(F::kKFull + ks), j * kCols, kv, b);
-        if (j >= F::kVSlots) barWait(bar(F::kVEmpty + vs), (j / F::kVSlots - 1) & 1, dead);
-        barExpect(bar(F::kVFull + vs), F::kTileBytes);
-        loadTile<P, kCols>(vRing + vs * F::kTileBytes, &a.v, bar(F::kVFull + vs), j * kCols, kv, b);
+      loadValues(0);
+      for (int j = 1; j < n; j++) {
+        if (j >= F::kKSlots) barWait(bar(F::kKEmpty + j % F::kKSlots), (j / F::kKSlots - 1) & 1, dead);
+        loadKeys(j);
+        if (j >= F::kVSlots) barWait(bar(F::kVEmpty + j % F::kVSlots), (j / F::kVSlots - 1) & 1, dead);
+        loadValues(j);
       }
     }
     __syncwarp();
@@ -432,8 +480,9 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
     const int half = warp / 4, row = warp % 4 * 32 + lane, i = q0 + row;
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool live = i < a.sq;
-    const long long at = (((long long)b * a.sq + i) * a.heads + h) * a.d, stat = ((long long)b * a.heads + h) * a.sq + i;
+    const long long stat = ((long long)b * a.heads + h) * a.sq + i;
     const float c = a.scale * kLog2e;
+    const long long at = (((long long)b * a.sq + i) * a.heads + h) * a.d;
     if (half == 0) {
       float sum = 0.f;
       if (live && n > 1) {
@@ -478,15 +527,15 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
 #pragma unroll
         for (int k = 0; k < kHalf; k++)
           if (k < left) sum += __uint_as_float(x[k]) * __uint_as_float(y[k]);
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // everybody has read the zeros
+        // both halves' parts, always in the same order
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         if (half) deltas[row] = sum;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (!half) {
           sum += deltas[row];
           if (live) a.delta[stat] = sum;
+          deltas[row] = sum;
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (!half) deltas[row] = sum;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         delta = deltas[row];
       }
@@ -514,7 +563,8 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       barWait(bar(F::kDone), 0, dead);
       tcAfter();
     }
-    storeRow(static_cast<T*>(a.dq) + at, live, dq + lanes, half * L::kHeadCols / 2, (half + 1) * L::kHeadCols / 2, a.d, seen > 0 ? a.scale : 0.f, n > 0);
+    storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dq) + (((long long)b * a.sq + i - lane) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - (i - lane),
+                                   dq + lanes, half * L::kHeadCols / 2, a.d, seen > 0 ? a.scale : 0.f, n > 0, qTile + warp * (F::kQBytes / 8));
   } else {
     L::other();
   }
@@ -526,9 +576,48 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
 // its group:  S^T = K Q^T, dP^T = V dout^T, then dv += P^T dout and dk += dS^T Q.  While the warps
 // make P, the matrix units do the last tile's dk and this one's dP; while they make dS, dv and
 // the next scores.
+// Where that gives too few blocks, a cluster of two to eight shares the keys: each goes through a
+// part of the query tiles, leaves its 32-bit sums in shared memory, and adds up an equal part of
+// the rows over the cluster, always in the order of the blocks.
+__device__ __forceinline__ void clusterSync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Where 16-byte piece c of a row lies: pieces change places within 128 bytes, so that neither a
+// column of rows nor the pieces of a row meet in a bank.
+template <int kCols> __device__ __forceinline__ uint32_t pieceAt(uint32_t base, int row, int c) { return base + (row * (kCols / 4) + (c ^ row % 8)) * 16; }
+// Half of the thread's accumulator row into shared memory.
+template <int kCols> __device__ __forceinline__ void leaveRow(uint32_t base, int row, uint32_t tmem, int begin, bool any) {
+#pragma unroll
+  for (int c = 0; c < kCols / 2; c += 32) {
+    uint32_t r[32] = {};
+    if (any) {
+      tmemLoad32(tmem + begin + c, r);
+      tmemWaitLoad();
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(pieceAt<kCols>(base, row, (begin + c + i) / 4)), "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]),
+                   "r"(r[i + 3])
+                   : "memory");
+  }
+}
+// Adds eight elements of a row that block `rank` of the cluster has left.
+template <int kCols> __device__ __forceinline__ void addRow8(uint32_t base, int row, int c, int rank, float (&sum)[8]) {
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    uint32_t at;
+    float x[4];
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(pieceAt<kCols>(base, row, c * 2 + k)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at) : "memory");
+#pragma unroll
+    for (int u = 0; u < 4; u++) sum[k * 4 + u] += x[u];
+  }
+}
+
 template <class T, int P> struct Keys {
   static constexpr int kStages = P == 2 ? 2 : 4;
   static constexpr uint32_t kTileBytes = Tiling<P>::kColTile, kKBytes = Tiling<P>::kRowTile;
+  static_assert(2 * kStages * kTileBytes >= 2 * kTile * Tiling<P>::kHeadCols * 4, "the sums of a shared tile fit the ring");
   static constexpr size_t kShared = kSharedBytes + 1024 + 2 * kKBytes + 2 * kStages * kTileBytes;
   enum { kKvFull = 0, kFull = 1, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kDpFull, kPFull, kDsFull, kDone, kBars };
 };
@@ -544,22 +633,24 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
-  const int j0 = blockIdx.z * kTile, kv = blockIdx.x, b = blockIdx.y, group = a.heads / a.kvHeads;
+  const int j0 = blockIdx.z * kTile, kv = blockIdx.x / a.split, rank = blockIdx.x % a.split, b = blockIdx.y, group = a.heads / a.kvHeads;
   const int keys = keysOf(a, b);
   const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kCols : 0;  // first query tile that sees a key of this one
-  const int each = j0 < keys ? max(0, colTiles<P>(a.sq) - first) : 0, n = each * group;
+  const int each = j0 < keys ? max(0, colTiles<P>(a.sq) - first) : 0, all = each * group;
+  // this block's part of the tiles
+  const int begun = int((long long)all * rank / a.split), n = int((long long)all * (rank + 1) / a.split) - begun;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < F::kBars; i++)
-      barInit(bar(i), i == F::kPFull || i == F::kDsFull ? kComputeWarps : i >= F::kFull && i < F::kEmpty ? 33 : 1);
-    sh.dead = 0;
-    fenceBarInit();
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < F::kBars; i++)
+        barInit(bar(i), i == F::kPFull || i == F::kDsFull ? kComputeWarps : i >= F::kFull && i < F::kEmpty ? 33 : 1);
+      sh.dead = 0;
+      fenceBarInit();
+      fenceAsyncShared();
+    }
+    __syncwarp();
   }
-  if (warp == kMmaWarp) tmemAlloc(smemAddr(&sh.tmem), L::kTmem);
-  tcBefore();
-  __syncthreads();
-  tcAfter();
-  const uint32_t tmem = uniform(sh.tmem), s = tmem, dp = tmem + kCols, dv = tmem + 2 * kCols, dk = dv + L::kHeadCols;
+  const uint32_t tmem = begin<P>(warp, &sh.tmem), s = tmem, dp = tmem + kCols, dv = tmem + 2 * kCols, dk = dv + L::kHeadCols;
 
   if (warp == kLoadWarp) {
     L::other();
@@ -568,7 +659,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       loadTile<P, kTile>(kTileAt, &a.k, bar(F::kKvFull), j0, kv, b);
       loadTile<P, kTile>(vTileAt, &a.v, bar(F::kKvFull), j0, kv, b);
     }
-    for (int it = 0, h = kv * group, qt = 0; it < n; it++) {
+    for (int it = 0, h = kv * group + (n ? begun / each : 0), qt = n ? begun % each : 0; it < n; it++) {
       const int st = it % F::kStages, turn = it / F::kStages, q0 = (first + qt) * kCols;
       const long long stat = ((long long)b * a.heads + h) * a.sq;
       float l[kCols / 32], d[kCols / 32];
@@ -640,7 +731,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
     // every statistic went to every thread, and reading them took as long as the exponentials.)
     constexpr int kBlocks8 = kHalf / 8, kRegs = kHalf / 2;
     const int row0 = warp % 4 * 32 + lane / 4, col0 = lane % 4 * 2;
-    for (int it = 0, qt = 0; it < n; it++) {
+    for (int it = 0, qt = n ? begun % each : 0; it < n; it++) {
       const int st = it % F::kStages, q0 = (first + qt) * kCols;
       if (++qt == each) qt = 0;
       const float* l = sh.stats[st][0] + half * kHalf + col0;
@@ -724,12 +815,36 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       barWait(bar(F::kDone), 0, dead);
       tcAfter();
     }
-    const bool live = j < a.sk;
-    const long long at = (((long long)b * a.sk + j) * a.kvHeads + kv) * a.d;
-    storeRow(static_cast<T*>(a.dv) + at, live, dv + lanes, half * L::kHeadCols / 2, (half + 1) * L::kHeadCols / 2, a.d, counts ? 1.f : 0.f, n > 0);
-    storeRow(static_cast<T*>(a.dk) + at, live, dk + lanes, half * L::kHeadCols / 2, (half + 1) * L::kHeadCols / 2, a.d, counts ? a.scale : 0.f, n > 0);
+    if (a.split == 1) {
+      const int jw = j - lane;  // the warp's first row
+      const long long at = (((long long)b * a.sk + jw) * a.kvHeads + kv) * a.d;
+      const int64_t stride = (int64_t)a.kvHeads * a.d;
+      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dv) + at, stride, a.sk - jw, dv + lanes, half * L::kHeadCols / 2, a.d, counts ? 1.f : 0.f, n > 0,
+                                     vTileAt + warp * (F::kKBytes / 8));
+      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dk) + at, stride, a.sk - jw, dk + lanes, half * L::kHeadCols / 2, a.d, counts ? a.scale : 0.f, n > 0,
+                                     kTileAt + warp * (F::kKBytes / 8));
+    } else {
+      // the tiles of the ring are done with: dv, then dk, in 32 bits
+      leaveRow<L::kHeadCols>(ring, row, dv + lanes, half * L::kHeadCols / 2, n > 0);
+      leaveRow<L::kHeadCols>(ring + kTile * L::kHeadCols * 4, row, dk + lanes, half * L::kHeadCols / 2, n > 0);
+    }
   } else {
     L::other();
+  }
+  if (a.split > 1) {
+    clusterSync();
+    if (warp < kComputeWarps) {
+      const int rows = kTile / a.split, row0 = rank * rows, chunks = a.d / 8, count = 2 * rows * chunks;
+      for (int i = threadIdx.x; i < count; i += kComputeWarps * 32) {
+        const int which = i / (rows * chunks), row = row0 + i / chunks % rows, c = i % chunks, j = j0 + row;
+        float sum[8] = {};
+        for (int r = 0; r < a.split; r++) addRow8<L::kHeadCols>(ring + which * kTile * L::kHeadCols * 4, row, c, r, sum);
+        if (j >= a.sk) continue;
+        T* out = static_cast<T*>(which ? a.dk : a.dv) + (((long long)b * a.sk + j) * a.kvHeads + kv) * a.d + c * 8;
+        *reinterpret_cast<uint4*>(out) = rounded8<T>(reinterpret_cast<const uint32_t*>(sum), j >= keys ? 0.f : which ? a.scale : 1.f);
+      }
+    }
+    clusterSync();  // nobody leaves while its sums are read
   }
   finish<P>(a, tmem, dead);
 }
@@ -802,7 +917,7 @@ int makeArgs(const tcpxbAttention& a, bool backward, int rows, Args* x) {
 }
 
 // Once for each kernel and device the block's shared memory is allowed; more than 64 devices would only ask again.
-template <void (*kKernel)(Args)> int launch(dim3 grid, int threads, size_t shared, const Args& a, int device, cudaStream_t s, const char* what) {
+template <void (*kKernel)(Args)> int launch(dim3 grid, int threads, size_t shared, const Args& a, int device, cudaStream_t s, const char* what, unsigned cluster = 1) {
   static std::atomic<uint64_t> allowed{0};
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   if (!(allowed.load(std::memory_order_relaxed) & bit)) {
@@ -810,7 +925,20 @@ template <void (*kKernel)(Args)> int launch(dim3 grid, int threads, size_t share
     if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  kKernel<<<grid, threads, shared, s>>>(a);
+  if (cluster == 1) {
+    kKernel<<<grid, threads, shared, s>>>(a);
+  } else {
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = cluster, attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid, config.blockDim = dim3(threads), config.dynamicSmemBytes = shared, config.stream = s;
+    config.attrs = &attribute, config.numAttrs = 1;
+    if (const cudaError_t e = cudaLaunchKernelEx(&config, kKernel, a); e != cudaSuccess) {
+      cudaGetLastError();
+      return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    }
+  }
   return launched(what);
 }
 
@@ -831,7 +959,18 @@ template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaSt
                                                  "attention backward, queries"))
       return rc;
   if (!a.b || !a.sk) return TCPXB_T_OK;
-  return launch<keyKernel<T, P>>(dim3(a.kv_heads, a.b, (a.sk + kTile - 1) / kTile), Tiling<P>::kThreads, Keys<T, P>::kShared, x, device, s, "attention backward, keys");
+  // A cluster where all blocks find room at the same time, with at least four tiles for each.  2 x 512
+  // tokens, 16/4 heads of 64, causal: 32 tiles in one block 31.6 us, 8 in each of four 16.2 us; 1000 tokens,
+  // 8/1 heads of 128: 99.7 us, in fours 37.1 us, in eights 28.7 us.  Where blocks come in several rounds a
+  // cluster's overhead, about six tiles of 64 queries, is lost (512 blocks 163 us, in fours 211 us), and
+  // eights do not pack: 256 of their blocks take 24.5 us for the first example.
+  const long long tilesOfKeys = (a.sk + kTile - 1) / kTile, blocks = tilesOfKeys * a.kv_heads * a.b;
+  const long long tilesOfQueries = (long long)(a.sq + Tiling<P>::kCols - 1) / Tiling<P>::kCols * (a.heads / a.kv_heads);
+  const auto fits = [&](int split) { return blocks * split <= (split == 8 ? 148 : 148 * Tiling<P>::kBlocks) && tilesOfQueries / split >= 4; };
+  x.split = 1;
+  while (x.split < 8 && fits(2 * x.split)) x.split *= 2;
+  return launch<keyKernel<T, P>>(dim3(a.kv_heads * x.split, a.b, unsigned(tilesOfKeys)), Tiling<P>::kThreads, Keys<T, P>::kShared, x, device, s,
+                                 "attention backward, keys", unsigned(x.split));
 }
 
 int dispatch(const tcpxbAttention* a, bool backward, void* stream) {

@@ -281,3 +281,14 @@ def test_the_c_entry_refuses():
         assert lib.tcpxb_attention_forward(args(**kw), None) == -1, kw
         assert lib.tcpxb_train_last_error()
     assert lib.tcpxb_attention_backward(args(), None) == -1
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,s,h,hk,d", [(1, 300, 16, 1, 64), (2, 513, 8, 2, 64), (1, 1000, 8, 1, 128), (1, 130, 12, 2, 40), (1, 600, 6, 2, 96)])
+def test_shared_keys_are_summed_over_clusters(b, s, h, hk, d, causal):
+    """Few blocks with many tiles each: two, four and eight blocks share a tile of keys; lengths leave some without work."""
+    q, k, v, dout = inputs(b, s, s, h, hk, d, BF16, seed=s)
+    first = check(q, k, v, dout, causal)
+    assert all(torch.equal(x, y) for x, y in zip(first, check(q, k, v, dout, causal)))
+    check(q, k, v, dout, causal, torch.full((b,), s // 3, dtype=torch.int32, device="cuda"))
