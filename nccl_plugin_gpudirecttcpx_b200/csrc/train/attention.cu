@@ -180,6 +180,51 @@ __device__ __forceinline__ void storeRows(T* out, int64_t stride, int rows, uint
   }
 }
 
+// A cluster of `split` blocks can share a tile of rows, each with a part of what the rows are summed
+// over: at the end every block leaves its 32-bit sums in shared memory and adds up an equal part of
+// the rows, always in the order of the blocks.
+__device__ __forceinline__ void clusterSync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Where 16-byte piece c of a row lies: pieces change places within 128 bytes, so that neither a
+// column of rows nor the pieces of a row meet in a bank.
+template <int kCols> __device__ __forceinline__ uint32_t pieceAt(uint32_t base, int row, int c) { return base + (row * (kCols / 4) + (c ^ row % 8)) * 16; }
+// A value that block `rank` of the cluster has at `at` in its shared memory.
+__device__ __forceinline__ float remote(uint32_t at, int rank) {
+  float x;
+  asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+// kPart columns of the thread's accumulator row into shared memory.
+template <int kCols, int kPart> __device__ __forceinline__ void leaveRow(uint32_t base, int row, uint32_t tmem, int begin, bool any) {
+#pragma unroll
+  for (int c = 0; c < kPart; c += 32) {
+    uint32_t r[32] = {};
+    if (any) {
+      tmemLoad32(tmem + begin + c, r);
+      tmemWaitLoad();
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(pieceAt<kCols>(base, row, (begin + c + i) / 4)), "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]),
+                   "r"(r[i + 3])
+                   : "memory");
+  }
+}
+// Adds eight elements of a row that block `rank` of the cluster has left, times `by`.
+template <int kCols> __device__ __forceinline__ void addRow8(uint32_t base, int row, int c, int rank, float by, float (&sum)[8]) {
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    uint32_t at;
+    float x[4];
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(pieceAt<kCols>(base, row, c * 2 + k)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at) : "memory");
+#pragma unroll
+    for (int u = 0; u < 4; u++) sum[k * 4 + u] += x[u] * by;
+  }
+}
+
 // ------------------------------------------------------------------ forward
 // A block owns two tiles of queries; four warps do the softmax of each.  While one tile's scores
 // are turned into probabilities, the matrix units work for the other one: out += P V of the
@@ -190,32 +235,36 @@ template <class T, int P> struct Forward {
   static constexpr int kSlots = P == 2 ? 4 : 8;  // tiles of keys and values in turn
   static constexpr uint32_t kTileBytes = Tiling<P>::kColTile, kQBytes = Tiling<P>::kRowTile;
   static constexpr size_t kShared = kSharedBytes + 1024 + 2 * kQBytes + kSlots * kTileBytes;
+  static_assert(kSlots * kTileBytes >= 2 * kTile * Tiling<P>::kHeadCols * 4, "the sums of shared tiles fit the ring");
   enum { kQFull = 0, kFull = 2, kEmpty = kFull + kSlots, kSFull = kEmpty + kSlots, kPFull = kSFull + 2, kOFull = kPFull + 2, kBars = kOFull + 2 };
 };
 
-template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) forwardKernel(const __grid_constant__ Args a) {
+template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) forwardKernel(const __grid_constant__ Args a) {
   using F = Forward<T, P>;
   using L = Tiling<P>;
   constexpr int kCols = L::kCols;
   static_assert(F::kBars <= 32, "barriers");
   extern __shared__ char raw[];
+  const int split = kSplit ? a.split : 1;
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const uint32_t tile0 = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, ring = tile0 + 2 * F::kQBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   // the longest blocks first, over all heads and batches: with a causal mask the last queries see the most keys
-  const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * 2 * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
+  const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * 2 * kTile, h = blockIdx.x / split, rank = blockIdx.x % split, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
   const int keys = keysOf(a, b);
-  int n[2];
+  int all[2], n[2];  // tiles of keys that a tile of queries sees, and those of this block's part
 #pragma unroll
-  for (int t = 0; t < 2; t++) n[t] = q0 + t * kTile < a.sq ? colTiles<P>(seenBy(a, min(q0 + t * kTile + kTile, a.sq) - 1, keys)) : 0;
-  const int most = max(n[0], n[1]);
+  for (int t = 0; t < 2; t++) all[t] = q0 + t * kTile < a.sq ? colTiles<P>(seenBy(a, min(q0 + t * kTile + kTile, a.sq) - 1, keys)) : 0;
+  const int every = max(all[0], all[1]), begun = int((long long)every * rank / split), most = int((long long)every * (rank + 1) / split) - begun;
+#pragma unroll
+  for (int t = 0; t < 2; t++) n[t] = min(max(all[t] - begun, 0), most);
 
   const auto loadPair = [&](int i) {  // number i of K_0, V_0, K_1, ...
     const int slot = i % F::kSlots;
     barExpect(bar(F::kFull + slot), F::kTileBytes);
-    loadTile<P, kCols>(ring + slot * F::kTileBytes, i & 1 ? &a.v : &a.k, bar(F::kFull + slot), i / 2 * kCols, kv, b);
+    loadTile<P, kCols>(ring + slot * F::kTileBytes, i & 1 ? &a.v : &a.k, bar(F::kFull + slot), (begun + i / 2) * kCols, kv, b);
   };
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -253,7 +302,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       if (j < most) barWait(bar(F::kFull + ik % F::kSlots), ik / F::kSlots & 1, dead);
       if (j) {
         barWait(bar(F::kFull + iv % F::kSlots), iv / F::kSlots & 1, dead);
-        if (j * kCols > keys && keys < a.sk) clearRows<P>(vTileAt, keys - (j - 1) * kCols);
+        if ((begun + j) * kCols > keys && keys < a.sk) clearRows<P>(vTileAt, keys - (begun + j - 1) * kCols);
       }
       for (int t = 0; t < 2; t++) {
         const uint32_t s = tmem + t * kCols, o = tmem + 2 * kCols + t * L::kHeadCols;
@@ -297,8 +346,8 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       uint32_t x[kCols];
       tmemLoad<kCols>(s, x);
       tmemWaitLoad();
-      if (j >= whole) {
-        const int left = seen - j * kCols;
+      if (begun + j >= whole) {
+        const int left = seen - (begun + j) * kCols;
 #pragma unroll
         for (int k = 0; k < kCols; k++) x[k] = k < left ? x[k] : 0xff800000u;
       }
@@ -350,14 +399,51 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
     }
     const float sum = sum2.x + sum2.y;
     const bool live = i < a.sq;
-    // a row that sees nothing is zero, whatever its tile holds
-    const float by = seen > 0 ? 1.f / sum : 0.f;
-    const int i0 = i - lane;  // the warp's first row
-    storeRows<T, L::kHeadCols>(static_cast<T*>(a.o) + (((long long)b * a.sq + i0) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - i0, o, 0, a.d, by,
-                               n[t] > 0, tile0 + t * F::kQBytes + warp % 4 * (F::kQBytes / 4));
-    if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
+    if constexpr (kSplit) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the other tile of queries reads the ring to its own end
+      leaveRow<L::kHeadCols, L::kHeadCols>(ring + t * kTile * L::kHeadCols * 4, row, o, 0, n[t] > 0);
+      sh.stats[t][0][row] = top, sh.stats[t][1][row] = sum;
+    } else {
+      // a row that sees nothing is zero, whatever its tile holds
+      const float by = seen > 0 ? 1.f / sum : 0.f;
+      const int i0 = i - lane;  // the warp's first row
+      storeRows<T, L::kHeadCols>(static_cast<T*>(a.o) + (((long long)b * a.sq + i0) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - i0, o, 0, a.d, by,
+                                 n[t] > 0, tile0 + t * F::kQBytes + warp % 4 * (F::kQBytes / 4));
+      if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
+    }
   } else {
     L::other();
+  }
+  if constexpr (kSplit) {
+    clusterSync();
+    if (warp < kComputeWarps) {
+      const float c = a.scale * kLog2e;
+      const int rows = 2 * kTile / split, chunks = a.d / 8, count = rows * chunks;
+      for (int k = threadIdx.x; k < count; k += kComputeWarps * 32) {
+        const int r = rank * rows + k / chunks, t = r / kTile, row = r % kTile, chunk = k % chunks, i = q0 + r;
+        // the blocks' sums are for maxima of their own
+        float tops[8], sums[8], top = -INFINITY, sum = 0.f, o[8] = {};
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+          if (u < split) {
+            tops[u] = remote(smemAddr(&sh.stats[t][0][row]), u), sums[u] = remote(smemAddr(&sh.stats[t][1][row]), u);
+            top = fmaxf(top, tops[u]);
+          }
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+          if (u < split && sums[u] != 0.f) {
+            const float by = exp2Fast((tops[u] - top) * c);
+            sum += sums[u] * by;
+            addRow8<L::kHeadCols>(ring + t * kTile * L::kHeadCols * 4, row, chunk, u, by, o);
+          }
+        if (i >= a.sq) continue;
+        const bool sees = seenBy(a, i, keys) > 0;
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (((long long)b * a.sq + i) * a.heads + h) * a.d + chunk * 8) =
+            rounded8<T>(reinterpret_cast<const uint32_t*>(o), sees ? 1.f / sum : 0.f);
+        if (chunk == 0) a.lse[((long long)b * a.heads + h) * a.sq + i] = sees ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
+      }
+    }
+    clusterSync();  // nobody leaves while its sums are read
   }
   finish<P>(a, tmem, dead);
 }
@@ -373,17 +459,19 @@ template <class T, int P> struct Queries {
   static constexpr int kKSlots = P == 2 ? 3 : 5, kVSlots = P == 2 ? 2 : 3;
   static constexpr uint32_t kTileBytes = Tiling<P>::kColTile, kQBytes = Tiling<P>::kRowTile;
   static constexpr size_t kShared = 1024 + 1024 + 2 * kQBytes + (kKSlots + kVSlots) * kTileBytes;
+  static_assert(kKSlots * kTileBytes >= kTile * Tiling<P>::kHeadCols * 4, "the sums of a shared tile fit the ring of keys");
   enum { kQFull = 0, kKFull = 1, kVFull = kKFull + kKSlots, kKEmpty = kVFull + kVSlots, kVEmpty = kKEmpty + kKSlots, kSFull = kVEmpty + kVSlots,
          kDpFull = kSFull + 2, kDsFull, kDone, kBars };
 };
 
 // A score that the row or key does not count for leaves exactly zero.
-template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) queryKernel(const __grid_constant__ Args a) {
+template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) queryKernel(const __grid_constant__ Args a) {
   using F = Queries<T, P>;
   using L = Tiling<P>;
   constexpr int kCols = L::kCols, kHalf = L::kHalf;
   static_assert(F::kBars <= 32, "barriers");
   extern __shared__ char raw[];
+  const int split = kSplit ? a.split : 1;
   uint64_t* bars = reinterpret_cast<uint64_t*>(raw);
   uint32_t* tmemAt = reinterpret_cast<uint32_t*>(raw + 256);
   volatile int* dead = reinterpret_cast<int*>(raw + 264);
@@ -392,18 +480,20 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
                  vRing = kRing + F::kKSlots * F::kTileBytes;
   const auto bar = [&](int i) { return smemAddr(bars) + 8 * i; };
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
-  const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * kTile, h = blockIdx.x, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
-  const int keys = keysOf(a, b), n = colTiles<P>(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
+  const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * kTile, h = blockIdx.x / split, rank = blockIdx.x % split, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
+  // tiles of keys that the queries see, and this block's part of them
+  const int keys = keysOf(a, b), all = colTiles<P>(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
+  const int begun = int((long long)all * rank / split), n = int((long long)all * (rank + 1) / split) - begun;
 
   const auto loadKeys = [&](int j) {
     const int ks = j % F::kKSlots;
     barExpect(bar(F::kKFull + ks), F::kTileBytes);
-    loadTile<P, kCols>(kRing + ks * F::kTileBytes, &a.k, bar(F::kKFull + ks), j * kCols, kv, b);
+    loadTile<P, kCols>(kRing + ks * F::kTileBytes, &a.k, bar(F::kKFull + ks), (begun + j) * kCols, kv, b);
   };
   const auto loadValues = [&](int j) {
     const int vs = j % F::kVSlots;
     barExpect(bar(F::kVFull + vs), F::kTileBytes);
-    loadTile<P, kCols>(vRing + vs * F::kTileBytes, &a.v, bar(F::kVFull + vs), j * kCols, kv, b);
+    loadTile<P, kCols>(vRing + vs * F::kTileBytes, &a.v, bar(F::kVFull + vs), (begun + j) * kCols, kv, b);
   };
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -441,7 +531,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       const int ks = j % F::kKSlots;
       const uint32_t kTileAt = kRing + ks * F::kTileBytes;
       barWait(bar(F::kKFull + ks), j / F::kKSlots & 1, dead);
-      if ((j + 1) * kCols > keys && keys < a.sk) clearRows<P>(kTileAt, keys - j * kCols);
+      if ((begun + j + 1) * kCols > keys && keys < a.sk) clearRows<P>(kTileAt, keys - (begun + j) * kCols);
       if (leader) {
         mmaTiles<P>(tmem + (j & 1) * kCols, qTile, kTileAt, scores, steps);
         mmaCommit(bar(F::kSFull + (j & 1)));
@@ -485,7 +575,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
     const long long at = (((long long)b * a.sq + i) * a.heads + h) * a.d;
     if (half == 0) {
       float sum = 0.f;
-      if (live && n > 1) {
+      if (live && all > 1) {
         const T *o = static_cast<const T*>(a.out) + at, *g = static_cast<const T*>(a.doutPtr) + b * a.doutB + i * a.doutS + h * a.doutH;
         for (int k = 0; k < a.d; k += 8) {
           float x[8], y[8];
@@ -495,7 +585,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
           for (int u = 0; u < 8; u++) sum += x[u] * y[u];
         }
       }
-      if (live && n != 1) a.delta[stat] = sum;
+      if (live && all != 1 && rank == 0) a.delta[stat] = sum;
       deltas[row] = sum;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -521,8 +611,8 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       uint32_t y[kHalf], ds[kHalf / 2];
       tmemLoad<kHalf>(dp + half * kHalf + lanes, y);
       tmemWaitLoad();
-      const int left = seen - j * kCols - half * kHalf;
-      if (n == 1) {
+      const int left = seen - (begun + j) * kCols - half * kHalf;
+      if (all == 1) {
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < kHalf; k++)
@@ -551,7 +641,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
           ds[k / 2] = pack2<T>(g.x, g.y);
         }
       };
-      if (j < whole) gradients(std::false_type());
+      if (begun + j < whole) gradients(std::false_type());
       else gradients(std::true_type());
       tmemStore<kHalf / 2>(s, ds);
       tmemWaitStore();
@@ -563,10 +653,28 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       barWait(bar(F::kDone), 0, dead);
       tcAfter();
     }
-    storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dq) + (((long long)b * a.sq + i - lane) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - (i - lane),
-                                   dq + lanes, half * L::kHeadCols / 2, a.d, seen > 0 ? a.scale : 0.f, n > 0, qTile + warp * (F::kQBytes / 8));
+    if constexpr (kSplit)
+      leaveRow<L::kHeadCols, L::kHeadCols / 2>(kRing, row, dq + lanes, half * L::kHeadCols / 2, n > 0);
+    else
+      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dq) + (((long long)b * a.sq + i - lane) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - (i - lane),
+                                     dq + lanes, half * L::kHeadCols / 2, a.d, seen > 0 ? a.scale : 0.f, n > 0, qTile + warp * (F::kQBytes / 8));
   } else {
     L::other();
+  }
+  if constexpr (kSplit) {
+    clusterSync();
+    if (warp < kComputeWarps) {
+      const int rows = kTile / split, chunks = a.d / 8, count = rows * chunks;
+      for (int k = threadIdx.x; k < count; k += kComputeWarps * 32) {
+        const int row = rank * rows + k / chunks, chunk = k % chunks, i = q0 + row;
+        float sum[8] = {};
+        for (int r = 0; r < split; r++) addRow8<L::kHeadCols>(kRing, row, chunk, r, 1.f, sum);
+        if (i < a.sq)
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.dq) + (((long long)b * a.sq + i) * a.heads + h) * a.d + chunk * 8) =
+              rounded8<T>(reinterpret_cast<const uint32_t*>(sum), seenBy(a, i, keys) > 0 ? a.scale : 0.f);
+      }
+    }
+    clusterSync();  // nobody leaves while its sums are read
   }
   finish<P>(a, tmem, dead);
 }
@@ -576,44 +684,6 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
 // its group:  S^T = K Q^T, dP^T = V dout^T, then dv += P^T dout and dk += dS^T Q.  While the warps
 // make P, the matrix units do the last tile's dk and this one's dP; while they make dS, dv and
 // the next scores.
-// Where that gives too few blocks, a cluster of two to eight shares the keys: each goes through a
-// part of the query tiles, leaves its 32-bit sums in shared memory, and adds up an equal part of
-// the rows over the cluster, always in the order of the blocks.
-__device__ __forceinline__ void clusterSync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Where 16-byte piece c of a row lies: pieces change places within 128 bytes, so that neither a
-// column of rows nor the pieces of a row meet in a bank.
-template <int kCols> __device__ __forceinline__ uint32_t pieceAt(uint32_t base, int row, int c) { return base + (row * (kCols / 4) + (c ^ row % 8)) * 16; }
-// Half of the thread's accumulator row into shared memory.
-template <int kCols> __device__ __forceinline__ void leaveRow(uint32_t base, int row, uint32_t tmem, int begin, bool any) {
-#pragma unroll
-  for (int c = 0; c < kCols / 2; c += 32) {
-    uint32_t r[32] = {};
-    if (any) {
-      tmemLoad32(tmem + begin + c, r);
-      tmemWaitLoad();
-    }
-#pragma unroll
-    for (int i = 0; i < 32; i += 4)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(pieceAt<kCols>(base, row, (begin + c + i) / 4)), "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]),
-                   "r"(r[i + 3])
-                   : "memory");
-  }
-}
-// Adds eight elements of a row that block `rank` of the cluster has left.
-template <int kCols> __device__ __forceinline__ void addRow8(uint32_t base, int row, int c, int rank, float (&sum)[8]) {
-#pragma unroll
-  for (int k = 0; k < 2; k++) {
-    uint32_t at;
-    float x[4];
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(pieceAt<kCols>(base, row, c * 2 + k)), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at) : "memory");
-#pragma unroll
-    for (int u = 0; u < 4; u++) sum[k * 4 + u] += x[u];
-  }
-}
-
 template <class T, int P> struct Keys {
   static constexpr int kStages = P == 2 ? 2 : 4;
   static constexpr uint32_t kTileBytes = Tiling<P>::kColTile, kKBytes = Tiling<P>::kRowTile;
@@ -622,23 +692,24 @@ template <class T, int P> struct Keys {
   enum { kKvFull = 0, kFull = 1, kEmpty = kFull + kStages, kSFull = kEmpty + kStages, kDpFull, kPFull, kDsFull, kDone, kBars };
 };
 
-template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) keyKernel(const __grid_constant__ Args a) {
+template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<P>::kThreads, Tiling<P>::kBlocks) keyKernel(const __grid_constant__ Args a) {
   using F = Keys<T, P>;
   using L = Tiling<P>;
   constexpr int kCols = L::kCols, kHalf = L::kHalf;
   static_assert(F::kBars <= 32 && F::kStages <= 4, "barriers");
   extern __shared__ char raw[];
+  const int split = kSplit ? a.split : 1;
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const uint32_t kTileAt = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, vTileAt = kTileAt + F::kKBytes, ring = vTileAt + F::kKBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
   volatile int* dead = &sh.dead;
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
-  const int j0 = blockIdx.z * kTile, kv = blockIdx.x / a.split, rank = blockIdx.x % a.split, b = blockIdx.y, group = a.heads / a.kvHeads;
+  const int j0 = blockIdx.z * kTile, kv = blockIdx.x / split, rank = blockIdx.x % split, b = blockIdx.y, group = a.heads / a.kvHeads;
   const int keys = keysOf(a, b);
   const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kCols : 0;  // first query tile that sees a key of this one
   const int each = j0 < keys ? max(0, colTiles<P>(a.sq) - first) : 0, all = each * group;
   // this block's part of the tiles
-  const int begun = int((long long)all * rank / a.split), n = int((long long)all * (rank + 1) / a.split) - begun;
+  const int begun = int((long long)all * rank / split), n = int((long long)all * (rank + 1) / split) - begun;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -815,7 +886,7 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
       barWait(bar(F::kDone), 0, dead);
       tcAfter();
     }
-    if (a.split == 1) {
+    if constexpr (!kSplit) {
       const int jw = j - lane;  // the warp's first row
       const long long at = (((long long)b * a.sk + jw) * a.kvHeads + kv) * a.d;
       const int64_t stride = (int64_t)a.kvHeads * a.d;
@@ -825,20 +896,20 @@ template <class T, int P> __global__ void __launch_bounds__(Tiling<P>::kThreads,
                                      kTileAt + warp * (F::kKBytes / 8));
     } else {
       // the tiles of the ring are done with: dv, then dk, in 32 bits
-      leaveRow<L::kHeadCols>(ring, row, dv + lanes, half * L::kHeadCols / 2, n > 0);
-      leaveRow<L::kHeadCols>(ring + kTile * L::kHeadCols * 4, row, dk + lanes, half * L::kHeadCols / 2, n > 0);
+      leaveRow<L::kHeadCols, L::kHeadCols / 2>(ring, row, dv + lanes, half * L::kHeadCols / 2, n > 0);
+      leaveRow<L::kHeadCols, L::kHeadCols / 2>(ring + kTile * L::kHeadCols * 4, row, dk + lanes, half * L::kHeadCols / 2, n > 0);
     }
   } else {
     L::other();
   }
-  if (a.split > 1) {
+  if constexpr (kSplit) {
     clusterSync();
     if (warp < kComputeWarps) {
-      const int rows = kTile / a.split, row0 = rank * rows, chunks = a.d / 8, count = 2 * rows * chunks;
+      const int rows = kTile / split, row0 = rank * rows, chunks = a.d / 8, count = 2 * rows * chunks;
       for (int i = threadIdx.x; i < count; i += kComputeWarps * 32) {
         const int which = i / (rows * chunks), row = row0 + i / chunks % rows, c = i % chunks, j = j0 + row;
         float sum[8] = {};
-        for (int r = 0; r < a.split; r++) addRow8<L::kHeadCols>(ring + which * kTile * L::kHeadCols * 4, row, c, r, sum);
+        for (int r = 0; r < split; r++) addRow8<L::kHeadCols>(ring + which * kTile * L::kHeadCols * 4, row, c, r, 1.f, sum);
         if (j >= a.sk) continue;
         T* out = static_cast<T*>(which ? a.dk : a.dv) + (((long long)b * a.sk + j) * a.kvHeads + kv) * a.d + c * 8;
         *reinterpret_cast<uint4*>(out) = rounded8<T>(reinterpret_cast<const uint32_t*>(sum), j >= keys ? 0.f : which ? a.scale : 1.f);
@@ -917,28 +988,32 @@ int makeArgs(const tcpxbAttention& a, bool backward, int rows, Args* x) {
 }
 
 // Once for each kernel and device the block's shared memory is allowed; more than 64 devices would only ask again.
-template <void (*kKernel)(Args)> int launch(dim3 grid, int threads, size_t shared, const Args& a, int device, cudaStream_t s, const char* what, unsigned cluster = 1) {
+template <void (*kKernel)(Args)> int allow(size_t shared, int device, const char* what) {
   static std::atomic<uint64_t> allowed{0};
   const uint64_t bit = device < 64 ? 1ull << device : 0;
-  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-    const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
-    if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    allowed.fetch_or(bit, std::memory_order_relaxed);
-  }
-  if (cluster == 1) {
+  if (allowed.load(std::memory_order_relaxed) & bit) return TCPXB_T_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+  if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return TCPXB_T_OK;
+}
+
+// The kernel, or its form for clusters where `a.split` blocks share a tile.
+template <void (*kKernel)(Args), void (*kClusters)(Args)>
+int launch(dim3 grid, int threads, size_t shared, const Args& a, int device, cudaStream_t s, const char* what) {
+  if (a.split == 1) {
+    if (const int rc = allow<kKernel>(shared, device, what)) return rc;
     kKernel<<<grid, threads, shared, s>>>(a);
-  } else {
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = cluster, attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = grid, config.blockDim = dim3(threads), config.dynamicSmemBytes = shared, config.stream = s;
-    config.attrs = &attribute, config.numAttrs = 1;
-    if (const cudaError_t e = cudaLaunchKernelEx(&config, kKernel, a); e != cudaSuccess) {
-      cudaGetLastError();
-      return fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    }
+    return launched(what);
   }
+  if (const int rc = allow<kClusters>(shared, device, what)) return rc;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = unsigned(a.split), attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid, config.blockDim = dim3(threads), config.dynamicSmemBytes = shared, config.stream = s;
+  config.attrs = &attribute, config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kClusters, a);
   return launched(what);
 }
 
@@ -950,27 +1025,35 @@ template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaSt
   if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "attention: %s", cudaGetErrorString(e));
   Args x;
   if (const int rc = makeArgs(a, backward, Tiling<P>::kCols, &x)) return rc;
+  constexpr int kCols = Tiling<P>::kCols;
+  // A cluster where all blocks find room at the same time, with at least four (gradients of keys) or eight
+  // tiles for each.  2 x 512 tokens, 16/4 heads of 64, causal, gradients of keys: 32 tiles in one block 31.6 us, 8 in each of four
+  // 16.2 us; 1000 tokens, 8/1 heads of 128: 99.7 us, in fours 37.1 us, in eights 28.7 us.  Where blocks come
+  // in several rounds a cluster's overhead, about six tiles of 64, is lost (512 blocks 163 us, in fours
+  // 211 us), and eights do not pack: 256 of their blocks take 24.5 us for the first example.
+  const auto splitFor = [](long long blocks, long long tiles, int least) {
+    int split = 1;
+    while (split < 8 && blocks * split * 2 <= (split == 4 ? 148 : 148 * Tiling<P>::kBlocks) && tiles / (split * 2) >= least) split *= 2;
+    return split;
+  };
+  const long long tilesOfKeys = (a.sk + kTile - 1) / kTile, colsOfKeys = (a.sk + kCols - 1) / kCols;
+  const long long tilesOfQueries = (a.sq + kTile - 1) / kTile, pairsOfQueries = (tilesOfQueries + 1) / 2;
   if (!backward) {
     if (!a.b || !a.sq) return TCPXB_T_OK;
-    return launch<forwardKernel<T, P>>(dim3(a.heads, a.b, (a.sq + 2 * kTile - 1) / (2 * kTile)), Tiling<P>::kThreads, Forward<T, P>::kShared, x, device, s, "attention forward");
+    x.split = splitFor(pairsOfQueries * a.heads * a.b, colsOfKeys, 8);
+    return launch<forwardKernel<T, P, false>, forwardKernel<T, P, true>>(dim3(a.heads * x.split, a.b, unsigned(pairsOfQueries)), Tiling<P>::kThreads, Forward<T, P>::kShared, x, device, s,
+                                       "attention forward");
   }
-  if (a.b && a.sq)
-    if (const int rc = launch<queryKernel<T, P>>(dim3(a.heads, a.b, (a.sq + kTile - 1) / kTile), Tiling<P>::kThreads, Queries<T, P>::kShared, x, device, s,
-                                                 "attention backward, queries"))
+  if (a.b && a.sq) {
+    x.split = splitFor(tilesOfQueries * a.heads * a.b, colsOfKeys, 8);
+    if (const int rc = launch<queryKernel<T, P, false>, queryKernel<T, P, true>>(dim3(a.heads * x.split, a.b, unsigned(tilesOfQueries)), Tiling<P>::kThreads, Queries<T, P>::kShared, x,
+                                                 device, s, "attention backward, queries"))
       return rc;
+  }
   if (!a.b || !a.sk) return TCPXB_T_OK;
-  // A cluster where all blocks find room at the same time, with at least four tiles for each.  2 x 512
-  // tokens, 16/4 heads of 64, causal: 32 tiles in one block 31.6 us, 8 in each of four 16.2 us; 1000 tokens,
-  // 8/1 heads of 128: 99.7 us, in fours 37.1 us, in eights 28.7 us.  Where blocks come in several rounds a
-  // cluster's overhead, about six tiles of 64 queries, is lost (512 blocks 163 us, in fours 211 us), and
-  // eights do not pack: 256 of their blocks take 24.5 us for the first example.
-  const long long tilesOfKeys = (a.sk + kTile - 1) / kTile, blocks = tilesOfKeys * a.kv_heads * a.b;
-  const long long tilesOfQueries = (long long)(a.sq + Tiling<P>::kCols - 1) / Tiling<P>::kCols * (a.heads / a.kv_heads);
-  const auto fits = [&](int split) { return blocks * split <= (split == 8 ? 148 : 148 * Tiling<P>::kBlocks) && tilesOfQueries / split >= 4; };
-  x.split = 1;
-  while (x.split < 8 && fits(2 * x.split)) x.split *= 2;
-  return launch<keyKernel<T, P>>(dim3(a.kv_heads * x.split, a.b, unsigned(tilesOfKeys)), Tiling<P>::kThreads, Keys<T, P>::kShared, x, device, s,
-                                 "attention backward, keys", unsigned(x.split));
+  x.split = splitFor(tilesOfKeys * a.kv_heads * a.b, (long long)(a.sq + kCols - 1) / kCols * (a.heads / a.kv_heads), 4);
+  return launch<keyKernel<T, P, false>, keyKernel<T, P, true>>(dim3(a.kv_heads * x.split, a.b, unsigned(tilesOfKeys)), Tiling<P>::kThreads, Keys<T, P>::kShared, x, device, s,
+                                 "attention backward, keys");
 }
 
 int dispatch(const tcpxbAttention* a, bool backward, void* stream) {

@@ -286,9 +286,30 @@ def test_the_c_entry_refuses():
 @gpu
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("b,s,h,hk,d", [(1, 300, 16, 1, 64), (2, 513, 8, 2, 64), (1, 1000, 8, 1, 128), (1, 130, 12, 2, 40), (1, 600, 6, 2, 96)])
-def test_shared_keys_are_summed_over_clusters(b, s, h, hk, d, causal):
-    """Few blocks with many tiles each: two, four and eight blocks share a tile of keys; lengths leave some without work."""
+def test_shared_tiles_are_summed_over_clusters(b, s, h, hk, d, causal):
+    """Few blocks with many tiles each: two, four and eight blocks share a tile; lengths leave some without work."""
     q, k, v, dout = inputs(b, s, s, h, hk, d, BF16, seed=s)
     first = check(q, k, v, dout, causal)
     assert all(torch.equal(x, y) for x, y in zip(first, check(q, k, v, dout, causal)))
     check(q, k, v, dout, causal, torch.full((b,), s // 3, dtype=torch.int32, device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d", [(1, 1, 4000, 2, 1, 64), (2, 300, 1500, 2, 2, 128), (1, 257, 2100, 1, 1, 64), (1, 20, 3001, 8, 2, 72), (1, 2500, 40, 2, 1, 64)])
+def test_long_rows_of_few_queries(b, sq, sk, h, hk, d, dtype):
+    """The keys of a row are split over a cluster, whose parts have maxima of their own; some parts are empty."""
+    q, k, v, dout = inputs(b, sq, sk, h, hk, d, dtype, seed=sk)
+    check(q, k, v, dout)
+    check(q, k, v, dout, True)
+    lens = torch.tensor([sk // 5, 3][:b], dtype=torch.int32, device="cuda")
+    check(q, k, v, dout, False, lens)
+    check(q, k, v, dout, True, torch.zeros_like(lens))
+    # maxima that rise and fall from part to part
+    k[..., 0] = torch.linspace(-20, 20, sk, device="cuda").to(dtype)[None, :, None]
+    q[..., 0] = 4.0
+    check(q, k, v, dout)
+    k[..., 0] = k[..., 0].flip(1)
+    check(q, k, v, dout)
+    k[:, sk // 2] = math.nan
+    assert ops.attention_forward(q, k, v)[0].isnan().all()

@@ -4,7 +4,13 @@ Tolerances are counted from roundings, element by element.  `half` is half a ste
 to the value: what one rounding to it can be off.  Roundings to the type are: each operand that a kernel
 feeds to the matrix units (probabilities, score gradients) and each result.  Everything else is 32-bit:
 a sum of n products is off by at most n 2^-24 of the sum of magnitudes, and the kernels add in pieces,
-so n + 8 covers the scaling and the exponential beside it."""
+so n + 8 covers the scaling and the exponential beside it.
+
+Under its normal range a type's steps are all of one size, so an operand is also off by up to half of
+its smallest step (`least / 2`), whatever its value: in fp16 that is 2^-25, and a probability of 2^-26
+becomes zero.  Such an error enters a product with the other operand's magnitude, summed over the row
+(the forward pass's unnormalised probabilities are at least as large as the normalised ones, as their
+sum is at least one)."""
 import torch
 
 F32 = 2.0 ** -24
@@ -28,6 +34,7 @@ def attention(q, k, v, dout, causal=False, lengths=None, scale=None):
     dtype, (b, sq, h, d), (sk, hk) = q.dtype, q.shape, k.shape[1:3]
     scale = d ** -0.5 if scale is None else scale
     u = half(dtype)
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     ok = visible(b, sq, sk, causal, lengths).to(q.device)
     at = torch.arange(sk, device=q.device)
     live = (at < lengths.to(q.device)[:, None] if lengths is not None else at.expand(b, sk) >= 0)[:, None, :, None]
@@ -49,20 +56,21 @@ def attention(q, k, v, dout, causal=False, lengths=None, scale=None):
     n = max(sq, sk) + 8
     out = p @ v
     mag = p @ v.abs()
-    eout = u * out.abs() + (u + n * F32) * mag + (p * ep) @ v.abs()
+    under = (p > 0) * (least / 2)
+    eout = u * out.abs() + (u + n * F32) * mag + (p * ep + under) @ v.abs()
     tol = {"out": eout, "lse": rowes.squeeze(-1) + (sk + 16) * F32 + 4 * F32 * lse.abs().nan_to_num(posinf=0.0)}
     dp = dout @ v.mT
     delta = (dout * out).sum(-1, keepdim=True)
     ds = p * (dp - delta)
     edelta = (dout.abs() * eout).sum(-1, keepdim=True) + (d + 8) * F32 * (dout * out).abs().sum(-1, keepdim=True)
     edp = (d + 8) * F32 * (dout.abs() @ v.abs().mT)
-    eds = ds.abs() * (u + ep) + p * (1 + u) * (edelta + edp)
+    eds = ds.abs() * (u + ep) + p * (1 + u) * (edelta + edp) + under
     dq = scale * (ds @ k)
     edq = u * dq.abs() + scale * ((eds + n * F32 * ds.abs()) @ k.abs())
     dk, dv = scale * (ds.mT @ q), p.mT @ dout
     group = (h // hk) * n * F32
     edk = scale * ((eds + group * ds.abs()).mT @ q.abs())
-    edv = (p * (u + ep + group)).mT @ dout.abs()
+    edv = (p * (u + ep + group) + under).mT @ dout.abs()
 
     def shared(x):
         return x.unflatten(1, (hk, h // hk)).sum(2)
@@ -71,8 +79,7 @@ def attention(q, k, v, dout, causal=False, lengths=None, scale=None):
     vals = {"out": out, "dq": dq, "dk": dk, "dv": dv}
     tol.update(dq=edq, dk=shared(edk) + u * dk.abs(), dv=shared(edv) + u * dv.abs())
     # values under the type's normal range are off by a step of its smallest
-    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
-    got = {name: (x.transpose(1, 2), tol[name].transpose(1, 2) * 1.001 + tiny) for name, x in vals.items()}
+    got = {name: (x.transpose(1, 2), tol[name].transpose(1, 2) * 1.001 + least) for name, x in vals.items()}
     got["lse"] = lse, tol["lse"] * 1.001 + 1e-30
     return got
 
