@@ -110,8 +110,11 @@ struct Step {
   float beta1, beta2, rest1, rest2, eps, keep, stepSize, rootCorrection, coef;
   __device__ __forceinline__ void operator()(float2& p, float2 g, float2& m, float2& v, float2& root) const {
     g = mul2(g, {coef, coef});
-    m = add2(mul2(m, {beta1, beta1}), mul2(g, {rest1, rest1}));
-    v = add2(mul2(v, {beta2, beta2}), mul2(mul2(g, {rest2, rest2}), g));
+    // sums one by one: a packed sum would be contracted with its product, which rounds otherwise
+    const float2 m1 = mul2(m, {beta1, beta1}), m2 = mul2(g, {rest1, rest1});
+    m = {__fadd_rn(m1.x, m2.x), __fadd_rn(m1.y, m2.y)};
+    const float2 v1 = mul2(v, {beta2, beta2}), v2 = mul2(mul2(g, {rest2, rest2}), g);
+    v = {__fadd_rn(v1.x, v2.x), __fadd_rn(v1.y, v2.y)};
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.x) : "f"(v.x));
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.y) : "f"(v.y));
     float2 below = fma2(root, {rootCorrection, rootCorrection}, {eps, eps});
@@ -231,7 +234,7 @@ __device__ __forceinline__ float warpTop(float x) {
 }
 // About 220 instructions a block, of which 64 are the step itself: at this count issue and memory
 // take the same time, so the rest is kept short (the warp's maximum is one instruction, the four
-// divisions of a block are done by four lanes at once).
+// factors of a block are taken by four lanes at once).
 template <bool kVector, class T, class W>
 __device__ __forceinline__ void stepBlock(const Raw<T, W>& r, const tcpxbAdamwTensor& t, const Step& step, long long b, long long end, float& mScale, float& vScale) {
   const int lane = threadIdx.x % 32;
@@ -257,7 +260,7 @@ __device__ __forceinline__ void stepBlock(const Raw<T, W>& r, const tcpxbAdamwTe
   // lanes 0 and 1 take the factors to codes, 2 and 3 the scales, of m and of the root.  Below 1e-30
   // a block is held as zeros: the factor would leave the range.
   const float top = lane & 1 ? topV : topM;
-  float ratio = lane & 2 ? top / kE4m3Max : kE4m3Max / top;
+  float ratio = lane & 2 ? top * (1.f / kE4m3Max) : kE4m3Max * __frcp_rn(top);
   if (!(top >= 1e-30f)) ratio = 0.f;
   const float toM = __shfl_sync(0xffffffffu, ratio, 0), toV = __shfl_sync(0xffffffffu, ratio, 1);
 #pragma unroll
