@@ -474,4 +474,6 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     scratch = params[0].new_empty(_entry("tcpxb_adamw_scratch_bytes")(table, count), dtype=torch.uint8)
     _call("tcpxb_adamw_step", dev, table, count, _ADAMW.pack(lr, beta1, beta2, eps, weight_decay, _ptr(norm), max_grad_norm or 0.0, compute, bits,
                                                              _CODES[dtype], scratch.data_ptr()))
+    if not torch.is_inference_mode_enabled():
+        torch.autograd.graph.increment_version(params)  # autograd learns of the update, as of any other in place
     return norm

@@ -131,6 +131,17 @@ def test_first_steps_and_single_values():
 
 
 @gpu
+def test_autograd_learns_of_the_update():
+    s = tensors([300], F32, seed=10)
+    w = s["params"][0].requires_grad_()
+    loss = (w * w).sum()
+    with torch.no_grad():
+        ops.adamw_step(**s, **HOW)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_zero_gradients_keep_everything_finite(bits):
     s = tensors([1000], BF16, bits, seed=5, steps=0)

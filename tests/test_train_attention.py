@@ -170,6 +170,15 @@ def test_gradients_where_only_some_are_wanted():
 
 
 @gpu
+def test_status_stays_zero():
+    status = ops.status_buffer()
+    q, k, v, dout = inputs(2, 300, 300, 8, 2, 64, BF16, seed=13)
+    out, lse = ops.attention_forward(q, k, v, causal=True, status=status)
+    ops.attention_backward(dout, q, k, v, out, lse, causal=True, status=status)
+    assert not status.any()
+
+
+@gpu
 @pytest.mark.parametrize("b,sq,sk", [(0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 0)])
 def test_nothing_to_do(b, sq, sk):
     q, k, v, dout = inputs(b, sq, sk, 4, 2, 64, BF16)
@@ -242,6 +251,7 @@ def test_refusals():
         (ValueError, lambda: ops.attention(q, k, v, scale=-1.0)),
         (TypeError, lambda: ops.attention(q, k, v, key_lengths=torch.ones(2, dtype=torch.int64))),
         (ValueError, lambda: ops.attention(q, k, v, key_lengths=torch.ones(3, dtype=torch.int32))),
+        (ValueError, lambda: ops.attention_forward(q, k, v, status=torch.zeros(4))),
         (ValueError, lambda: ops.attention(q, k, v)),  # not on a GPU
     ]
     lse = torch.zeros(2, 4, 5)
