@@ -124,17 +124,6 @@ struct Step {
   }
 };
 
-// Eight elements of a lane, as pairs, and as they lie in memory.
-template <class T> __device__ __forceinline__ void pairs(const Vec8<T>& x, float2 (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) f[i] = {toFloat(x.x[2 * i]), toFloat(x.x[2 * i + 1])};
-}
-template <class T> __device__ __forceinline__ Vec8<T> rounded(const float2 (&f)[4]) {
-  Vec8<T> x;
-#pragma unroll
-  for (int i = 0; i < 4; i++) x.x[2 * i] = fromFloat<T>(f[i].x), x.x[2 * i + 1] = fromFloat<T>(f[i].y);
-  return x;
-}
 struct alignas(8) Codes { __nv_fp8x2_storage_t c[4]; };
 __device__ __forceinline__ void decode(const Codes& x, float scale, float2 (&f)[4]) {
 #pragma unroll

@@ -578,11 +578,12 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
       if (live && all > 1) {
         const T *o = static_cast<const T*>(a.out) + at, *g = static_cast<const T*>(a.doutPtr) + b * a.doutB + i * a.doutS + h * a.doutH;
         for (int k = 0; k < a.d; k += 8) {
-          float x[8], y[8];
-          load8(o + k, x);
-          load8(g + k, y);
+          float2 x[4], y[4], part = {0.f, 0.f};
+          pairs(*reinterpret_cast<const Vec8<T>*>(o + k), x);
+          pairs(*reinterpret_cast<const Vec8<T>*>(g + k), y);
 #pragma unroll
-          for (int u = 0; u < 8; u++) sum += x[u] * y[u];
+          for (int u = 0; u < 4; u++) part = fma2(x[u], y[u], part);
+          sum += part.x + part.y;
         }
       }
       if (live && all != 1 && rank == 0) a.delta[stat] = sum;

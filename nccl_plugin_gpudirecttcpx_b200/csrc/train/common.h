@@ -12,10 +12,6 @@ int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 // The last launch's status, as a return value.
 int launched(const char* what);
 
-template <class T> struct Pair;
-template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
-template <> struct Pair<__half> { using type = __half2; };
-
 __device__ __forceinline__ float toFloat(float x) { return x; }
 __device__ __forceinline__ float toFloat(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float toFloat(__half x) { return __half2float(x); }
@@ -26,18 +22,6 @@ template <> __device__ __forceinline__ __half fromFloat<__half>(float x) { retur
 
 // Eight elements on a 16-byte boundary (fp32: 32 bytes as two such vectors).
 template <class T> struct alignas(16) Vec8 { T x[8]; };
-
-template <class T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; i++) f[i] = toFloat(v.x[i]);
-}
-template <class T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  Vec8<T> v;
-#pragma unroll
-  for (int i = 0; i < 8; i++) v.x[i] = fromFloat<T>(f[i]);
-  *reinterpret_cast<Vec8<T>*>(p) = v;
-}
 
 // Two 32-bit operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -62,6 +46,41 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+template <class T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// A lane's eight elements as four pairs, and back, rounded; two 16-bit elements share a register.
+__device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) { return {__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)}; }
+__device__ __forceinline__ float2 unpack2(uint32_t x, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+template <class T> __device__ __forceinline__ void pairs(const Vec8<T>& v, float2 (&f)[4]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 w = *reinterpret_cast<const uint4*>(&v);
+    f[0] = unpack2(w.x, T()), f[1] = unpack2(w.y, T()), f[2] = unpack2(w.z, T()), f[3] = unpack2(w.w, T());
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = {v.x[2 * i], v.x[2 * i + 1]};
+  }
+}
+template <class T> __device__ __forceinline__ Vec8<T> rounded(const float2 (&f)[4]) {
+  Vec8<T> v;
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(&v) = {pack2<T>(f[0].x, f[0].y), pack2<T>(f[1].x, f[1].y), pack2<T>(f[2].x, f[2].y), pack2<T>(f[3].x, f[3].y)};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v.x[2 * i] = f[i].x, v.x[2 * i + 1] = f[i].y;
+  }
+  return v;
+}
+
 inline bool headsOk(const tcpxbHeads& h, int elemBytes) {
   const int64_t per = 16 / elemBytes;
   return h.ptr && reinterpret_cast<uintptr_t>(h.ptr) % 16 == 0 && h.stride_b % per == 0 && h.stride_s % per == 0 && h.stride_h % per == 0;

@@ -85,17 +85,7 @@ template <int G> __device__ __forceinline__ void groupSums(float& x, float& y) {
   }
 }
 
-// A lane's eight elements as four pairs.
-template <class T> __device__ __forceinline__ void pairs(const Vec8<T>& v, float2 (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) f[i] = {toFloat(v.x[2 * i]), toFloat(v.x[2 * i + 1])};
-}
-template <class T> __device__ __forceinline__ void store(T* p, const float2 (&f)[4]) {
-  Vec8<T> v;
-#pragma unroll
-  for (int i = 0; i < 4; i++) v.x[2 * i] = fromFloat<T>(f[i].x), v.x[2 * i + 1] = fromFloat<T>(f[i].y);
-  *reinterpret_cast<Vec8<T>*>(p) = v;
-}
+template <class T> __device__ __forceinline__ void store(T* p, const float2 (&f)[4]) { *reinterpret_cast<Vec8<T>*>(p) = rounded<T>(f); }
 __device__ __forceinline__ float sum(const float2 (&a)[4], const float2 (&b)[4]) {
   float2 s = mul2(a[0], b[0]);
 #pragma unroll
