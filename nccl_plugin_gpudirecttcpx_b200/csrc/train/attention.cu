@@ -20,7 +20,12 @@
 // Head sizes above 64 take score tiles of 128 columns and one block on an SM: all of its tensor
 // memory.  Up to 64 the products are half as long while the exponentials stay, so what counts is
 // to keep the other units busy: tiles of 64 columns, half the tensor memory, two blocks on an SM
-// that fill each other's waits, and each other's beginnings and ends.
+// that fill each other's waits, and each other's beginnings and ends.  Shared memory lets no more
+// blocks onto an SM than its tensor memory serves, whichever of these kernels they are of, so an
+// allocation never waits for a block of another cluster.
+//
+// A product that overwrites scores whose 16-bit form the product before it still reads is issued
+// behind that one without a wait: the matrix instructions of a block run in the order of issue.
 //
 // Probabilities and score gradients are rounded to the inputs' type because the matrix units take
 // operands of one type; sums, statistics and everything else are 32-bit.
@@ -46,13 +51,13 @@ template <int P> struct Tiling {
   static constexpr int kHeadCols = P * 64;         // of a sum over scores
   static constexpr uint32_t kRowTile = P * kPanelBytes, kColTile = P * kCols * 128;
   // With one block the compute warps take registers from the others, for which two idle warps
-  // complete a third warpgroup: 2 x 128 x 208 + 128 x 80 is less than the 384 x 168 of the launch.
+  // complete a third warpgroup: 2 x 128 x 216 + 128 x 72 are the 384 x 168 of the launch.
   static constexpr int kThreads = P == 1 ? 320 : 384;
   static __device__ __forceinline__ void compute() {
-    if constexpr (P == 2) moreRegisters<208>();
+    if constexpr (P == 2) moreRegisters<216>();
   }
   static __device__ __forceinline__ void other() {
-    if constexpr (P == 2) fewerRegisters<80>();
+    if constexpr (P == 2) fewerRegisters<72>();
   }
 };
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
