@@ -8,6 +8,7 @@ and g++.  Outputs land in `nccl_plugin_gpudirecttcpx_b200/_lib/`:
 
   libtcpxb_kernels.so   device kernels behind a C ABI (needs nvcc)
   libtcpxb_train.so     the training step's operators behind a C ABI (needs nvcc)
+  tcpxb_train_torch.so  their Python module: torch tensors to the C ABI (needs CUDA and torch headers)
   libnccl-net.so        the NCCL net plugin: host core + kernels + engine (needs nvcc)
   libtcpxb_host.so      host core + engine with no CUDA: device calls go to a stand-in
                         device in host memory (g++ only; used by CPU tests)
@@ -128,7 +129,7 @@ def build_cuda(verbose: bool = False) -> list[Path]:
     tlib = OUT / "libtcpxb_train.so"
     if _stale(tlib, tobjs, 0.0):
         _run([nvcc, "-shared", "-o", str(tlib)] + [str(o) for o in tobjs] + ["-cudart", "static"])
-    outs = [klib, tlib]
+    outs = [klib, tlib, _build_torch_module(nvcc, tlib, hdr, verbose)]
     core = _sources("core", ".cc") + _sources("plugin", ".cc") + _sources("engine", ".cc")
     if core:
         cobjs = _compile(core, "full", ["g++"], CXX_FLAGS + ["-I", _cuda_include(nvcc)], hdr, verbose)
@@ -146,6 +147,24 @@ def build_cuda(verbose: bool = False) -> list[Path]:
                                         f"-l:{plug.name}", "-Wl,-rpath,$ORIGIN", "-ldl", "-pthread"])
         outs.append(daemon)
     return outs
+
+
+def _build_torch_module(nvcc: str, tlib: Path, hdr: float, verbose: bool) -> Path:
+    """The module that ops/train.py calls, against the torch that runs this."""
+    import sysconfig
+
+    import torch
+    home = Path(torch.__file__).parent
+    inc = [str(home / "include"), str(home / "include/torch/csrc/api/include"), sysconfig.get_paths()["include"], _cuda_include(nvcc)]
+    flags = CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=tcpxb_train_torch", "-Wno-unused-parameter"]
+    for d in inc:
+        flags += ["-isystem", d]
+    objs = _compile(_sources("bind", ".cc"), "torch", ["g++"], flags, hdr, verbose)
+    mod = OUT / "tcpxb_train_torch.so"
+    if _stale(mod, objs + [tlib], 0.0):
+        _run(["g++", "-shared", "-o", str(mod)] + [str(o) for o in objs] + ["-L", str(OUT), f"-l:{tlib.name}", "-Wl,-rpath,$ORIGIN", "-L", str(home / "lib"),
+             "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
+    return mod
 
 
 def _cuda_include(nvcc: str) -> str:

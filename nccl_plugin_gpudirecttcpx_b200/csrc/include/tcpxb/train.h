@@ -51,6 +51,7 @@ typedef struct tcpxbAttention {
   int32_t b, sq, sk, heads, kv_heads, d;  // d: a multiple of 8, at most 128
   float scale;            // above zero
   int32_t causal, dtype;
+  int32_t device;         // that the tensors are on; becomes the calling thread's
   int32_t* status;        // a word on the device, or null: 3 (TCPXB_ST_TIMEOUT) where a bounded wait ran out
 } tcpxbAttention;
 
@@ -72,7 +73,7 @@ typedef struct tcpxbNormRope {
   int32_t b, s, heads, kv_heads, d;  // d: a multiple of 8, at most 256
   int32_t positions;
   float eps;
-  int32_t dtype;
+  int32_t dtype, device;
 } tcpxbNormRope;
 
 size_t tcpxb_norm_rope_scratch_bytes(int d);
@@ -97,7 +98,7 @@ typedef struct tcpxbAdamw {
   float* grad_norm;        // device scalar: gradients are scaled by min(1, max_norm / (grad_norm + 1e-6)); null: not clipped
   float max_norm;
   int32_t compute_norm;    // write *grad_norm first, as tcpxb_grad_norm would
-  int32_t state_bits, dtype;
+  int32_t state_bits, dtype, device;
   void* scratch;           // tcpxb_adamw_scratch_bytes()
 } tcpxbAdamw;
 
@@ -106,7 +107,7 @@ int tcpxb_adamw_step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdam
 
 // *norm = sqrt(sum of squares over all gradients (`g`, `n` of each tensor)).
 size_t tcpxb_grad_norm_scratch_bytes(const tcpxbAdamwTensor* tensors, int count);
-int tcpxb_grad_norm(const tcpxbAdamwTensor* tensors, int count, int dtype, float* norm, void* scratch, void* stream);
+int tcpxb_grad_norm(const tcpxbAdamwTensor* tensors, int count, int dtype, int device, float* norm, void* scratch, void* stream);
 
 #ifdef __cplusplus
 }

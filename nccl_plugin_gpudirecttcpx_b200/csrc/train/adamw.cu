@@ -525,6 +525,7 @@ extern "C" int tcpxb_adamw_step(const tcpxbAdamwTensor* tensors, int count, cons
     return fail(TCPXB_T_INVALID, "the arguments, the scratch or the norm are null");
   if (a->state_bits != 8 && a->state_bits != 32) return fail(TCPXB_T_INVALID, "states have 8 or 32 bits, not %d", a->state_bits);
   if (const int rc = check(tensors, count, a->dtype, true, a->state_bits)) return rc;
+  if (const int rc = use(a->device)) return rc;
   auto s = static_cast<cudaStream_t>(stream);
   if (a->dtype == TCPXB_T_BF16) return step<__nv_bfloat16>(tensors, count, *a, s);
   if (a->dtype == TCPXB_T_F16) return step<__half>(tensors, count, *a, s);
@@ -533,9 +534,10 @@ extern "C" int tcpxb_adamw_step(const tcpxbAdamwTensor* tensors, int count, cons
 
 extern "C" size_t tcpxb_grad_norm_scratch_bytes(const tcpxbAdamwTensor* tensors, int count) { return partialBytes(tensors, count); }
 
-extern "C" int tcpxb_grad_norm(const tcpxbAdamwTensor* tensors, int count, int dtype, float* norm, void* scratch, void* stream) {
+extern "C" int tcpxb_grad_norm(const tcpxbAdamwTensor* tensors, int count, int dtype, int device, float* norm, void* scratch, void* stream) {
   if (!norm || !scratch) return fail(TCPXB_T_INVALID, "null argument");
   if (const int rc = check(tensors, count, dtype, false, 32)) return rc;
+  if (const int rc = use(device)) return rc;
   auto s = static_cast<cudaStream_t>(stream);
   auto* partial = static_cast<double*>(scratch);
   if (dtype == TCPXB_T_BF16) return gradNorm<__nv_bfloat16>(tensors, count, norm, partial, s);

@@ -1024,11 +1024,8 @@ int launch(dim3 grid, int threads, size_t shared, const Args& a, int device, cud
 }
 
 template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaStream_t s) {
-  // a thread that only autograd has used so far knows its device but has no context yet, which the driver's call needs
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaSetDevice(device);
-  if (e != cudaSuccess) return fail(TCPXB_T_CUDA, "attention: %s", cudaGetErrorString(e));
+  if (const int rc = use(a.device)) return rc;
+  const int device = a.device;
   Args x;
   if (const int rc = makeArgs(a, backward, Tiling<P>::kCols, &x)) return rc;
   constexpr int kCols = Tiling<P>::kCols;

@@ -9,6 +9,9 @@
 namespace tcpxb_train {
 
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+// Makes the tensors' device the thread's.  A thread that only autograd has used so far has a device but
+// no context, which the driver's calls need; this gives it both.
+int use(int device);
 // The last launch's status, as a return value.
 int launched(const char* what);
 

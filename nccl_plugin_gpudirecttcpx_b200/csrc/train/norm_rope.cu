@@ -284,6 +284,7 @@ template <class T> int byWidth(const tcpxbNormRope& a, bool backward, cudaStream
 
 int dispatch(const tcpxbNormRope* a, bool backward, void* stream) {
   if (const int rc = check(a, backward)) return rc;
+  if (const int rc = use(a->device)) return rc;
   auto s = static_cast<cudaStream_t>(stream);
   if (a->dtype == TCPXB_T_BF16) return byWidth<__nv_bfloat16>(*a, backward, s);
   if (a->dtype == TCPXB_T_F16) return byWidth<__half>(*a, backward, s);

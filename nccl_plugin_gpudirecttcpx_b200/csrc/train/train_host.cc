@@ -19,6 +19,11 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+int use(int device) {
+  const cudaError_t e = cudaSetDevice(device);
+  return e == cudaSuccess ? TCPXB_T_OK : fail(TCPXB_T_CUDA, "device %d: %s", device, cudaGetErrorString(e));
+}
+
 int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TCPXB_T_OK : fail(TCPXB_T_CUDA, "%s: %s", what, cudaGetErrorString(e));

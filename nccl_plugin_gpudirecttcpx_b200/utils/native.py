@@ -44,6 +44,27 @@ def load(name: str, build: bool = True) -> ctypes.CDLL:
         return lib
 
 
+def module(name: str):
+    """Imports `_lib/<name>.so`, a Python module, building the native tree first when it is absent."""
+    import importlib.util
+    import sys
+
+    with _lock:
+        if name in sys.modules:
+            return sys.modules[name]
+        path = lib_path(name + ".so")
+        if not path.exists() and os.environ.get("TCPXB_NO_AUTOBUILD") != "1":
+            from .. import _build
+            _build.build_all()
+        if not path.exists():
+            raise NativeLibraryMissing(f"{path} is missing; run `python -m nccl_plugin_gpudirecttcpx_b200._build`")
+        spec = importlib.util.spec_from_file_location(name, path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        sys.modules[name] = mod
+        return mod
+
+
 def plugin_path() -> Path:
     """Path of the NCCL net plugin (`libnccl-net.so`), for NCCL_NET_PLUGIN."""
     return lib_path("libnccl-net.so")

@@ -269,10 +269,7 @@ def test_refusals():
 def test_the_c_entry_refuses():
     import ctypes
     import train_abi as A
-    from nccl_plugin_gpudirecttcpx_b200.ops import train as T
-    T._entry("tcpxb_train_last_error")  # sets the signatures
-    lib = T._t()
-    assert ctypes.sizeof(A.Adamw) == T._ADAMW.size
+    lib = A.library()
     t = (A.AdamwTensor * 1)(A.AdamwTensor(4096, 4096, 4096, 4096, None, None, None, 4096, 10))
     good = dict(lr=1e-3, beta1=0.9, beta2=0.9, eps=1e-8, weight_decay=0.0, state_bits=32, dtype=1, scratch=4096)
     assert lib.tcpxb_adamw_step(t, 1, None, None) == -1 and lib.tcpxb_adamw_step(None, 1, ctypes.byref(A.Adamw(**good)), None) == -1
@@ -282,4 +279,4 @@ def test_the_c_entry_refuses():
         u = (A.AdamwTensor * 1)(A.AdamwTensor(4096, 4096, 4096, 4096, None, None, None, 4096, 10))
         setattr(u[0], field, x)
         assert lib.tcpxb_adamw_step(u, 1, ctypes.byref(A.Adamw(**good)), None) == -1, field
-    assert lib.tcpxb_grad_norm(t, 1, 1, None, 4096, None) == -1
+    assert lib.tcpxb_grad_norm(t, 1, 1, 0, None, 4096, None) == -1

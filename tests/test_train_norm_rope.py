@@ -197,10 +197,7 @@ def test_refusals():
 def test_the_c_entry_refuses():
     import ctypes
     import train_abi as A
-    from nccl_plugin_gpudirecttcpx_b200.ops import train as T
-    T._entry("tcpxb_train_last_error")  # sets the signatures
-    lib = T._t()
-    assert ctypes.sizeof(A.NormRope) == T._NORM_ROPE.size
+    lib = A.library()
     assert lib.tcpxb_norm_rope_forward(None, None) == -1
 
     def args(**kw):

@@ -1,6 +1,8 @@
 """The argument structs of csrc/include/tcpxb/train.h, for calls of the C entries themselves."""
 import ctypes
 
+from nccl_plugin_gpudirecttcpx_b200.utils import native
+
 _vp, _i32, _i64, _f32, _f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 
@@ -14,12 +16,12 @@ def _all(kind, names):
 
 class Attention(ctypes.Structure):
     _fields_ = (_heads("q", "k", "v") + _all(_vp, "out lse") + _heads("dout") + _all(_vp, "dq dk dv delta key_lengths") +
-                _all(_i32, "b sq sk heads kv_heads d") + [("scale", _f32)] + _all(_i32, "causal dtype") + [("status", _vp)])
+                _all(_i32, "b sq sk heads kv_heads d") + [("scale", _f32)] + _all(_i32, "causal dtype device") + [("status", _vp)])
 
 
 class NormRope(ctypes.Structure):
     _fields_ = (_heads("q", "k") + _all(_vp, "wq wk cos sin pos q_out k_out") + _heads("dq_out", "dk_out") + _all(_vp, "dq dk dwq dwk partial") +
-                _all(_i32, "b s heads kv_heads d positions") + [("eps", _f32), ("dtype", _i32)])
+                _all(_i32, "b s heads kv_heads d positions") + [("eps", _f32)] + _all(_i32, "dtype device"))
 
 
 class AdamwTensor(ctypes.Structure):
@@ -28,4 +30,13 @@ class AdamwTensor(ctypes.Structure):
 
 class Adamw(ctypes.Structure):
     _fields_ = (_all(_f64, "lr beta1 beta2 eps weight_decay") + [("grad_norm", _vp), ("max_norm", _f32)] +
-                _all(_i32, "compute_norm state_bits dtype") + [("scratch", _vp)])
+                _all(_i32, "compute_norm state_bits dtype device") + [("scratch", _vp)])
+
+
+def library():
+    lib = native.load("libtcpxb_train.so")
+    lib.tcpxb_train_last_error.restype = ctypes.c_char_p
+    for name, *args in (("attention_forward", _vp, _vp), ("attention_backward", _vp, _vp), ("norm_rope_forward", _vp, _vp), ("norm_rope_backward", _vp, _vp),
+                        ("adamw_step", _vp, _i32, _vp, _vp), ("grad_norm", _vp, _i32, _i32, _i32, _vp, _vp, _vp)):
+        getattr(lib, "tcpxb_" + name).argtypes = args
+    return lib
