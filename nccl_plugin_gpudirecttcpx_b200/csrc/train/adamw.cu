@@ -239,9 +239,9 @@ __device__ __forceinline__ void stepBlock(const Raw<T, W>& r, const tcpxbAdamwTe
   for (int i = 0; i < 4; i++) {
     vv[i] = mul2(vv[i], vv[i]);
     step(pp[i], gg[i], mm[i], vv[i], root[i]);
-    topM = fmaxf(topM, fmaxf(fabsf(mm[i].x), fabsf(mm[i].y)));
-    topV = fmaxf(topV, fmaxf(root[i].x, root[i].y));
-    least = fminf(least, fminf(root[i].x, root[i].y));
+    topM = max3(topM, fabsf(mm[i].x), fabsf(mm[i].y));
+    topV = max3(topV, root[i].x, root[i].y);
+    least = min3(least, root[i].x, root[i].y);
   }
   put<kVector>(static_cast<T*>(t.p), e, end, rounded<T>(pp));
   if constexpr (!std::is_same_v<T, W>) put<kVector>(t.master, e, end, rounded<float>(pp));
@@ -336,13 +336,14 @@ template <class T, class W> __device__ __forceinline__ void stepBlocks(char* sha
   }
 }
 
-// What a CTA works on: elements [begin, end) of a tensor.
+// What a CTA works on: elements [begin, end) of a tensor.  The step goes through the list backwards: the
+// gradients that the norm has read last are still in the L2.
 template <class L> struct Chunk {
   int tensor;
   long long begin, end;
-  __device__ __forceinline__ explicit Chunk(const L& l) {
-    tensor = tensorOf(l, blockIdx.x);
-    begin = (long long)(blockIdx.x - (tensor ? l.end[tensor - 1] : 0)) * l.chunk;
+  __device__ __forceinline__ Chunk(const L& l, unsigned chunk) {
+    tensor = tensorOf(l, chunk);
+    begin = (long long)(chunk - (tensor ? l.end[tensor - 1] : 0)) * l.chunk;
     end = min((long long)l.t[tensor].n, begin + l.chunk);
   }
 };
@@ -354,7 +355,7 @@ __device__ __forceinline__ Step stepOf(const tcpxbAdamw& a, int tensor) {
 __device__ __forceinline__ bool inVectors(const tcpxbAdamwTensor& t) { return aligned(t.p) && aligned(t.g) && aligned(t.m) && aligned(t.v) && aligned(t.master); }
 
 template <class T, class L> __global__ void __launch_bounds__(kThreads, 4) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
-  const Chunk<L> c(l);
+  const Chunk<L> c(l, gridDim.x - 1 - blockIdx.x);
   const tcpxbAdamwTensor t = l.t[c.tensor];
   const Step step = stepOf(a, l.first + c.tensor);
   const long long whole = inVectors(t) ? c.begin + (c.end - c.begin) / 8 * 8 : c.begin;
@@ -364,14 +365,14 @@ template <class T, class L> __global__ void __launch_bounds__(kThreads, 4) stepK
 
 template <class T, class W, class L> __global__ void __launch_bounds__(kSmallWarps * 32, sizeof(W) == 2 ? 8 : 4) stepSmallKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
   __shared__ alignas(16) char shared[kSmallWarps * kStages * 32 * sizeof(Raw<T, W>)];
-  const Chunk<L> c(l);
+  const Chunk<L> c(l, gridDim.x - 1 - blockIdx.x);
   const tcpxbAdamwTensor t = l.t[c.tensor];
   const Step step = stepOf(a, l.first + c.tensor);
   stepBlocks<T, W>(shared, t, step, c.begin, c.end, inVectors(t));
 }
 
 template <class T, class L> __global__ void __launch_bounds__(kThreads) squaresKernel(const __grid_constant__ L l, double* partial) {
-  const Chunk<L> c(l);
+  const Chunk<L> c(l, blockIdx.x);
   const long long begin = c.begin, end = c.end;
   const T* g = static_cast<const T*>(l.t[c.tensor].g);
   // eight squares in 32 bits, those sums in 64: what rounding is left averages out

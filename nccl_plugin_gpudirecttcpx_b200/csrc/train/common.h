@@ -26,6 +26,16 @@ template <> __device__ __forceinline__ __half fromFloat<__half>(float x) { retur
 // Eight elements on a 16-byte boundary (fp32: 32 bytes as two such vectors).
 template <class T> struct alignas(16) Vec8 { T x[8]; };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Two 32-bit operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
