@@ -10,7 +10,7 @@
 // 22 bytes an element.
 //
 // 8-bit states: a block of 256 elements is held by one warp, eight elements a lane, so the
-// block's largest magnitude is five shuffles.  m is held as e4m3 times a 32-bit scale.  Of v the
+// block's largest magnitude is one instruction.  m is held as e4m3 times a 32-bit scale.  Of v the
 // root is held: it spans half the exponents, and e4m3 reaches 2^-18 of a block's largest root,
 // 2^-36 of its largest v.  A root above zero stays above zero (it is rounded up to the smallest
 // code), so an element whose m survives never meets a denominator of eps alone.
@@ -24,17 +24,13 @@ namespace tcpxb_train {
 namespace {
 
 constexpr int kThreads = 256;
-// Elements of a CTA: short chunks while they do not fill the GPU a few times, else longer ones,
-// which begin and end less often (323 M weights with 8-bit states: 1.61 ms in chunks of 8192).
-constexpr int kShortChunk = 8192, kLongChunk = 32768;
-constexpr long long kManyElements = 148ll * 8 * 4 * kShortChunk;
+constexpr int kChunk = 8192;  // elements of a CTA (32768: 1213 us instead of 1167 us for 323 M weights with clipping)
 constexpr float kE4m3Max = 448.f, kLeastCode = 0.001953125f;  // the largest code, and 2^-9, the smallest above zero
 
 template <int N> struct List {
   tcpxbAdamwTensor t[N];
   unsigned end[N];  // chunks up to and with tensor i
   int count, first;  // `first`: number of t[0] in the caller's list
-  int chunk;
 };
 // Two sizes of the same launch: a short list does not pay for copying 30 KB of parameters.
 using Short = List<24>;
@@ -72,13 +68,19 @@ __device__ __forceinline__ double blockSum(double x) {
 
 __device__ __forceinline__ float rootOfSum(const double* partial, long long n) {
   double sum = 0;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) sum += partial[i];
+  for (long long i0 = threadIdx.x; i0 < n; i0 += 8 * blockDim.x) {
+    double x[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = i0 + k * blockDim.x < n ? partial[i0 + k * blockDim.x] : 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) sum += x[k];
+  }
   return float(sqrt(blockSum(sum)));
 }
 
 // Counts every tensor's step and takes what depends on it, in 64 bits: 1 - b^t cancels.  The first
 // list's launch also takes the norm out of `partials` sums, where it is computed here.
-template <class L> __global__ void __launch_bounds__(512) prepareKernel(const __grid_constant__ L l, const tcpxbAdamw a, const double* partial, long long partials) {
+template <class L> __global__ void __launch_bounds__(1024) prepareKernel(const __grid_constant__ L l, const tcpxbAdamw a, const double* partial, long long partials) {
   auto* s = static_cast<Scratch*>(a.scratch);
   if (l.first == 0) {
     float norm = 0.f;
@@ -280,7 +282,7 @@ template <int kBytes> __device__ __forceinline__ void copyAsync(void* to, const 
 // first block and written after the last: one in between waits for the stores to its neighbours
 // (0.94 ms).
 constexpr int kSmallWarps = 4, kStages = 4;
-static_assert(kLongChunk / TCPXB_ADAMW_BLOCK / kSmallWarps <= 32, "a lane holds the scales of one block of its warp");
+static_assert(kChunk / TCPXB_ADAMW_BLOCK / kSmallWarps <= 32, "a lane holds the scales of one block of its warp");
 
 template <class T, class W> __device__ __forceinline__ void stepBlocks(char* shared, const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end, bool vectors) {
   using Share = Raw<T, W>;
@@ -343,8 +345,8 @@ template <class L> struct Chunk {
   long long begin, end;
   __device__ __forceinline__ Chunk(const L& l, unsigned chunk) {
     tensor = tensorOf(l, chunk);
-    begin = (long long)(chunk - (tensor ? l.end[tensor - 1] : 0)) * l.chunk;
-    end = min((long long)l.t[tensor].n, begin + l.chunk);
+    begin = (long long)(chunk - (tensor ? l.end[tensor - 1] : 0)) * kChunk;
+    end = min((long long)l.t[tensor].n, begin + kChunk);
   }
 };
 __device__ __forceinline__ Step stepOf(const tcpxbAdamw& a, int tensor) {
@@ -413,33 +415,24 @@ __global__ void __launch_bounds__(1024) normKernel(const double* partial, long l
   if (threadIdx.x == 0) *norm = x;
 }
 
-int chunkOf(const tcpxbAdamwTensor* tensors, int count) {
-  long long all = 0;
-  for (int i = 0; i < count; i++) all += tensors[i].n;
-  return all < kManyElements ? kShortChunk : kLongChunk;
-}
-long long chunksOf(const tcpxbAdamwTensor& t, int chunk) { return (t.n + chunk - 1) / chunk; }
+long long chunksOf(const tcpxbAdamwTensor& t) { return (t.n + kChunk - 1) / kChunk; }
 size_t ratesBytes(int count) { return sizeof(Scratch) + sizeof(Rates) * size_t(count); }
 size_t partialBytes(const tcpxbAdamwTensor* tensors, int count) {
   long long chunks = 0;
-  if (tensors) {
-    const int chunk = chunkOf(tensors, count);
-    for (int i = 0; i < count; i++) chunks += chunksOf(tensors[i], chunk);
-  }
+  for (int i = 0; tensors && i < count; i++) chunks += chunksOf(tensors[i]);
   return sizeof(double) * size_t(chunks + 1);
 }
 
 // Calls f(list, chunks) for the tensors in lists of at most N, leaving out those without elements.
 template <class L, int N, class F> int inLists(const tcpxbAdamwTensor* tensors, int count, F f) {
   static thread_local L l;
-  l.chunk = chunkOf(tensors, count);
   for (int first = 0; first < count;) {
     long long chunks = 0;
     l.count = 0, l.first = first;
     int i = first;
-    for (; i < count && l.count < N && chunks + chunksOf(tensors[i], l.chunk) < (1ll << 31); i++) {
+    for (; i < count && l.count < N && chunks + chunksOf(tensors[i]) < (1ll << 31); i++) {
       l.t[l.count] = tensors[i];
-      chunks += chunksOf(tensors[i], l.chunk);
+      chunks += chunksOf(tensors[i]);
       l.end[l.count++] = unsigned(chunks);
     }
     if (const int rc = f(l, chunks)) return rc;
@@ -495,7 +488,7 @@ template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tc
   }
   return inLists(tensors, count, [&](const auto& l, long long chunks) {
     using L = std::decay_t<decltype(l)>;
-    prepareKernel<<<1, partials > 128 ? 512 : l.count <= 128 ? 128 : 384, 0, s>>>(l, a, partial, partials);
+    prepareKernel<<<1, partials > 1024 ? 1024 : partials > 128 || l.count > 128 ? 384 : 128, 0, s>>>(l, a, partial, partials);
     if (const int rc = launched("adamw, rates")) return rc;
     if (!chunks) return int(TCPXB_T_OK);
     if (a.state_bits == 8 && masters) stepSmallKernel<T, float, L><<<unsigned(chunks), kSmallWarps * 32, 0, s>>>(l, a);

@@ -75,9 +75,6 @@ __device__ __forceinline__ void tmaLoad(uint32_t dst, const CUtensorMap* map, ui
       "l"(map), "r"(bar), "r"(col), "r"(row), "r"(head), "r"(batch)
       : "memory");
 }
-// Fetches a map's descriptor ahead of its first load.
-__device__ __forceinline__ void prefetchMap(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
-
 // Moves registers between the block's warpgroups: out of the shares of those that load and issue.
 template <int N> __device__ __forceinline__ void moreRegisters() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewerRegisters() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
