@@ -81,6 +81,8 @@ __device__ __forceinline__ float rootOfSum(const double* partial, long long n) {
 // Counts every tensor's step and takes what depends on it, in 64 bits: 1 - b^t cancels.  The first
 // list's launch also takes the norm out of `partials` sums, where it is computed here.
 template <class L> __global__ void __launch_bounds__(1024) prepareKernel(const __grid_constant__ L l, const tcpxbAdamw a, const double* partial, long long partials) {
+  waitForPrevious();
+  letNextStart();
   auto* s = static_cast<Scratch*>(a.scratch);
   if (l.first == 0) {
     float norm = 0.f;
@@ -357,6 +359,7 @@ __device__ __forceinline__ Step stepOf(const tcpxbAdamw& a, int tensor) {
 __device__ __forceinline__ bool inVectors(const tcpxbAdamwTensor& t) { return aligned(t.p) && aligned(t.g) && aligned(t.m) && aligned(t.v) && aligned(t.master); }
 
 template <class T, class L> __global__ void __launch_bounds__(kThreads, 4) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
+  waitForPrevious();
   const Chunk<L> c(l, gridDim.x - 1 - blockIdx.x);
   const tcpxbAdamwTensor t = l.t[c.tensor];
   const Step step = stepOf(a, l.first + c.tensor);
@@ -366,6 +369,7 @@ template <class T, class L> __global__ void __launch_bounds__(kThreads, 4) stepK
 }
 
 template <class T, class W, class L> __global__ void __launch_bounds__(kSmallWarps * 32, sizeof(W) == 2 ? 8 : 4) stepSmallKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
+  waitForPrevious();
   __shared__ alignas(16) char shared[kSmallWarps * kStages * 32 * sizeof(Raw<T, W>)];
   const Chunk<L> c(l, gridDim.x - 1 - blockIdx.x);
   const tcpxbAdamwTensor t = l.t[c.tensor];
@@ -374,6 +378,7 @@ template <class T, class W, class L> __global__ void __launch_bounds__(kSmallWar
 }
 
 template <class T, class L> __global__ void __launch_bounds__(kThreads) squaresKernel(const __grid_constant__ L l, double* partial) {
+  letNextStart();
   const Chunk<L> c(l, blockIdx.x);
   const long long begin = c.begin, end = c.end;
   const T* g = static_cast<const T*>(l.t[c.tensor].g);
@@ -411,6 +416,7 @@ template <class T, class L> __global__ void __launch_bounds__(kThreads) squaresK
 }
 
 __global__ void __launch_bounds__(1024) normKernel(const double* partial, long long n, float* norm) {
+  waitForPrevious();
   const float x = rootOfSum(partial, n);
   if (threadIdx.x == 0) *norm = x;
 }
@@ -488,21 +494,18 @@ template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tc
   }
   return inLists(tensors, count, [&](const auto& l, long long chunks) {
     using L = std::decay_t<decltype(l)>;
-    prepareKernel<<<1, partials > 1024 ? 1024 : partials > 128 || l.count > 128 ? 384 : 128, 0, s>>>(l, a, partial, partials);
-    if (const int rc = launched("adamw, rates")) return rc;
+    const int threads = partials > 1024 ? 1024 : partials > 128 || l.count > 128 ? 384 : 128;
+    if (const int rc = launchBehind(partials || l.first, prepareKernel<L>, 1, threads, 0, s, "adamw, rates", l, a, static_cast<const double*>(partial), partials)) return rc;
     if (!chunks) return int(TCPXB_T_OK);
-    if (a.state_bits == 8 && masters) stepSmallKernel<T, float, L><<<unsigned(chunks), kSmallWarps * 32, 0, s>>>(l, a);
-    else if (a.state_bits == 8) stepSmallKernel<T, T, L><<<unsigned(chunks), kSmallWarps * 32, 0, s>>>(l, a);
-    else stepKernel<T, L><<<unsigned(chunks), kThreads, 0, s>>>(l, a);
-    return launched("adamw");
+    if (a.state_bits == 32) return launchBehind(true, stepKernel<T, L>, unsigned(chunks), kThreads, 0, s, "adamw", l, a);
+    return launchBehind(true, masters ? stepSmallKernel<T, float, L> : stepSmallKernel<T, T, L>, unsigned(chunks), kSmallWarps * 32, 0, s, "adamw", l, a);
   });
 }
 
 template <class T> int gradNorm(const tcpxbAdamwTensor* tensors, int count, float* out, double* partial, cudaStream_t s) {
   long long done = 0;
   if (const int rc = squares<T>(tensors, count, partial, &done, s)) return rc;
-  normKernel<<<1, 1024, 0, s>>>(partial, done, out);
-  return launched("gradient norm, sum");
+  return launchBehind(done > 0, normKernel, 1, 1024, 0, s, "gradient norm, sum", static_cast<const double*>(partial), done, out);
 }
 
 }  // namespace

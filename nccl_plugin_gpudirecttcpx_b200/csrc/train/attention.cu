@@ -510,6 +510,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, tmemAt), dp = tmem + 2 * kCols, dq = tmem + 3 * kCols;
+  letNextStart();  // all blocks have their tensor memory
 
   if (warp == kLoadWarp) {
     L::other();
@@ -728,6 +729,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, &sh.tmem), s = tmem, dp = tmem + kCols, dv = tmem + 2 * kCols, dk = dv + L::kHeadCols;
+  waitForPrevious();  // for delta
 
   if (warp == kLoadWarp) {
     L::other();
@@ -1004,22 +1006,25 @@ template <void (*kKernel)(Args)> int allow(size_t shared, int device, const char
   return TCPXB_T_OK;
 }
 
-// The kernel, or its form for clusters where `a.split` blocks share a tile.
+// The kernel, or its form for clusters where `a.split` blocks share a tile; `behind` another kernel of this call.
 template <void (*kKernel)(Args), void (*kClusters)(Args)>
-int launch(dim3 grid, int threads, size_t shared, const Args& a, int device, cudaStream_t s, const char* what) {
-  if (a.split == 1) {
-    if (const int rc = allow<kKernel>(shared, device, what)) return rc;
-    kKernel<<<grid, threads, shared, s>>>(a);
-    return launched(what);
-  }
-  if (const int rc = allow<kClusters>(shared, device, what)) return rc;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = unsigned(a.split), attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+int launch(bool behind, dim3 grid, int threads, size_t shared, const Args& a, int device, cudaStream_t s, const char* what) {
+  if (const int rc = a.split == 1 ? allow<kKernel>(shared, device, what) : allow<kClusters>(shared, device, what)) return rc;
+  cudaLaunchAttribute attributes[2];
   cudaLaunchConfig_t config = {};
   config.gridDim = grid, config.blockDim = dim3(threads), config.dynamicSmemBytes = shared, config.stream = s;
-  config.attrs = &attribute, config.numAttrs = 1;
-  cudaLaunchKernelEx(&config, kClusters, a);
+  config.attrs = attributes, config.numAttrs = 0;
+  if (a.split > 1) {
+    cudaLaunchAttribute& x = attributes[config.numAttrs++];
+    x.id = cudaLaunchAttributeClusterDimension;
+    x.val.clusterDim.x = unsigned(a.split), x.val.clusterDim.y = x.val.clusterDim.z = 1;
+  }
+  if (behind) {
+    cudaLaunchAttribute& x = attributes[config.numAttrs++];
+    x.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    x.val.programmaticStreamSerializationAllowed = 1;
+  }
+  cudaLaunchKernelEx(&config, a.split == 1 ? kKernel : kClusters, a);
   return launched(what);
 }
 
@@ -1044,18 +1049,18 @@ template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaSt
   if (!backward) {
     if (!a.b || !a.sq) return TCPXB_T_OK;
     x.split = splitFor(pairsOfQueries * a.heads * a.b, colsOfKeys, 8);
-    return launch<forwardKernel<T, P, false>, forwardKernel<T, P, true>>(dim3(a.heads * x.split, a.b, unsigned(pairsOfQueries)), Tiling<P>::kThreads, Forward<T, P>::kShared, x, device, s,
+    return launch<forwardKernel<T, P, false>, forwardKernel<T, P, true>>(false, dim3(a.heads * x.split, a.b, unsigned(pairsOfQueries)), Tiling<P>::kThreads, Forward<T, P>::kShared, x, device, s,
                                        "attention forward");
   }
   if (a.b && a.sq) {
     x.split = splitFor(tilesOfQueries * a.heads * a.b, colsOfKeys, 8);
-    if (const int rc = launch<queryKernel<T, P, false>, queryKernel<T, P, true>>(dim3(a.heads * x.split, a.b, unsigned(tilesOfQueries)), Tiling<P>::kThreads, Queries<T, P>::kShared, x,
+    if (const int rc = launch<queryKernel<T, P, false>, queryKernel<T, P, true>>(false, dim3(a.heads * x.split, a.b, unsigned(tilesOfQueries)), Tiling<P>::kThreads, Queries<T, P>::kShared, x,
                                                  device, s, "attention backward, queries"))
       return rc;
   }
   if (!a.b || !a.sk) return TCPXB_T_OK;
   x.split = splitFor(tilesOfKeys * a.kv_heads * a.b, (long long)(a.sq + kCols - 1) / kCols * (a.heads / a.kv_heads), 4);
-  return launch<keyKernel<T, P, false>, keyKernel<T, P, true>>(dim3(a.kv_heads * x.split, a.b, unsigned(tilesOfKeys)), Tiling<P>::kThreads, Keys<T, P>::kShared, x, device, s,
+  return launch<keyKernel<T, P, false>, keyKernel<T, P, true>>(a.b && a.sq, dim3(a.kv_heads * x.split, a.b, unsigned(tilesOfKeys)), Tiling<P>::kThreads, Keys<T, P>::kShared, x, device, s,
                                  "attention backward, keys");
 }
 

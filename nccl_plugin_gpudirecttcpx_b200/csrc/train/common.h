@@ -94,6 +94,23 @@ template <class T> __device__ __forceinline__ Vec8<T> rounded(const float2 (&f)[
   return v;
 }
 
+// A kernel behind another one of the same call may be set up while that one ends, and waits here until
+// all of its writes are there.  It may be set up once all blocks of the one before have called
+// letNextStart(), or have ended: then it takes the room that they leave.  A call's first kernel is
+// launched in the ordinary way: what stands before it in the stream is not ours to judge.
+__device__ __forceinline__ void waitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void letNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <class K, class... A> int launchBehind(bool own, K* kernel, dim3 grid, int threads, size_t shared, cudaStream_t s, const char* what, const A&... args) {
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid, config.blockDim = dim3(threads), config.dynamicSmemBytes = shared, config.stream = s;
+  config.attrs = &attribute, config.numAttrs = own ? 1 : 0;
+  cudaLaunchKernelEx(&config, kernel, args...);
+  return launched(what);
+}
+
 inline bool headsOk(const tcpxbHeads& h, int elemBytes) {
   const int64_t per = 16 / elemBytes;
   return h.ptr && reinterpret_cast<uintptr_t>(h.ptr) % 16 == 0 && h.stride_b % per == 0 && h.stride_s % per == 0 && h.stride_h % per == 0;

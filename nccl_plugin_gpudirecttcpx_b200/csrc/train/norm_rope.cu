@@ -130,6 +130,7 @@ template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads
 
 // A few rows of a block's dw are in its lanes at the end: of queries in the first qBlocks, else of keys.
 template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads, 2) backwardKernel(const __grid_constant__ Job j) {
+  letNextStart();
   const bool keys = blockIdx.x >= j.qBlocks;
   const Side& side = j.side[keys];
   const unsigned block = blockIdx.x - (keys ? j.qBlocks : 0), blocks = keys ? j.kBlocks : j.qBlocks;
@@ -199,6 +200,7 @@ template <class T, int G, bool kNorm> __global__ void __launch_bounds__(kThreads
 // dw: the blocks' partial sums.  A block has 32 columns of one weight, and 32 warps that each take
 // every 32nd row.
 template <class T> __global__ void __launch_bounds__(1024) weightKernel(const __grid_constant__ Job j, T* dwq, T* dwk) {
+  waitForPrevious();
   __shared__ float sums[32][33];
   const int x = threadIdx.x % 32, y = threadIdx.x / 32, i = blockIdx.x * 32 + x;
   const unsigned first = blockIdx.y ? j.qBlocks : 0, end = blockIdx.y ? j.qBlocks + j.kBlocks : j.qBlocks;
@@ -270,8 +272,8 @@ template <class T, int G> int run(const tcpxbNormRope& a, bool backward, cudaStr
     else backwardKernel<T, G, false><<<j.qBlocks + j.kBlocks, kThreads, 0, s>>>(j);
     if (const int rc = launched("norm and rotation, backward")) return rc;
   }
-  if (a.wq) weightKernel<T><<<dim3((a.d + 31) / 32, 2), 1024, 0, s>>>(j, static_cast<T*>(a.dwq), static_cast<T*>(a.dwk));
-  return launched("norm and rotation, weights");
+  if (!a.wq) return TCPXB_T_OK;
+  return launchBehind(tokens > 0, weightKernel<T>, dim3((a.d + 31) / 32, 2), 1024, 0, s, "norm and rotation, weights", j, static_cast<T*>(a.dwq), static_cast<T*>(a.dwk));
 }
 
 template <class T> int byWidth(const tcpxbNormRope& a, bool backward, cudaStream_t s) {
