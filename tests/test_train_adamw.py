@@ -215,6 +215,38 @@ def test_same_bits_every_time_and_in_a_graph(bits):
             assert torch.equal(a.view(torch.uint8) if a.dim() else a, c.view(torch.uint8) if c.dim() else c)
 
 
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_of_several_lists_one_after_another(bits):
+    """Kernels that are set up while the one before them ends: gradients written right before a step, steps and norms
+    behind one another without a pause, eager and in a graph, against the same with a pause after every call."""
+    sizes = [(i * 61) % 900 for i in range(800)] + [300000]
+    paused, eager, graph = (tensors(sizes, BF16, bits, seed=14) for _ in range(3))
+    sources = [tensors(sizes, BF16, bits, seed=s)["grads"] for s in (15, 16, 17)]
+
+    def run(s, pause):
+        norms = []
+        for grads in sources:
+            torch._foreach_copy_(s["grads"], grads)
+            pause()
+            norms.append(ops.adamw_step(**s, **HOW, max_grad_norm=0.3))
+            pause()
+            norms.append(ops.grad_norm(s["grads"]))
+            pause()
+        return norms
+
+    wanted = run(paused, torch.cuda.synchronize)
+    norms = [run(eager, lambda: None)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        norms.append(run(graph, lambda: None))
+    g.replay()
+    for other, found in zip((eager, graph), norms):
+        assert all(torch.equal(a, b) for a, b in zip(wanted, found))
+        for n in paused:
+            assert all(torch.equal(a.reshape(-1).view(torch.uint8), b.reshape(-1).view(torch.uint8)) for a, b in zip(paused[n], other[n]))
+
+
 def test_refusals():
     def call(change=(), **kw):
         s = tensors([10, 300], BF16, device="cpu")
