@@ -34,6 +34,12 @@ void onDevice(std::optional<c10::cuda::CUDAGuard>& guard, const Tensor& first, s
   TORCH_CHECK_VALUE(ok, "all tensors have to be on one CUDA device");
   guard.emplace(first.device());
 }
+// A dual tensor of forward mode does not require gradients, so autograd's functions are passed by for it: its
+// tangent would be lost without a word, which reads as a derivative of zero.
+void noTangent(std::initializer_list<const Maybe*> tensors) {
+  for (const Maybe* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->has_value() || !(*t)->_fw_grad(0).defined(), "forward-mode derivatives are not provided: gradients are taken backwards");
+}
 void* streamOf(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 Tensor make(const Tensor& like, at::IntArrayRef sizes, ScalarType type) { return at::empty(sizes, like.options().dtype(type).requires_grad(false)); }
@@ -104,7 +110,8 @@ tcpxbAttention describe(Tensor& q, Tensor& k, Tensor& v, const Sizes& s, bool ca
 std::tuple<Tensor, Tensor> attentionForward(Tensor q, Tensor k, Tensor v, bool causal, std::optional<double> scale, Maybe lengths, Maybe status) {
   const Sizes s = checkAttention(q, k, v, scale, lengths, status);
   std::optional<c10::cuda::CUDAGuard> guard;
-  const Maybe mk = k, mv = v;
+  const Maybe mq = q, mk = k, mv = v;
+  noTangent({&mq, &mk, &mv});
   onDevice(guard, q, {&mk, &mv, &lengths, &status});
   Tensor out = make(q, {s.b, s.sq, s.h, s.d}), lse = make(q, {s.b, s.h, s.sq}, at::kFloat);
   tcpxbAttention a = describe(q, k, v, s, causal, lengths, status);
@@ -123,7 +130,8 @@ std::tuple<Tensor, Tensor, Tensor> attentionBackward(Tensor dout, Tensor q, Tens
   TORCH_CHECK_VALUE(lse.dim() == 3 && lse.size(0) == s.b && lse.size(1) == s.h && lse.size(2) == s.sq, "lse has to be [batch, heads, queries], got ", lse.sizes());
   TORCH_CHECK_TYPE(lse.scalar_type() == at::kFloat, "lse has to be float32, got ", lse.scalar_type());
   std::optional<c10::cuda::CUDAGuard> guard;
-  const Maybe mk = k, mv = v, mdout = dout, mout = out, mlse = lse;
+  const Maybe mq = q, mk = k, mv = v, mdout = dout, mout = out, mlse = lse;
+  noTangent({&mq, &mk, &mv, &mdout, &mout, &mlse});
   onDevice(guard, q, {&mk, &mv, &mdout, &mout, &mlse, &lengths, &status});
   Tensor dq = make(q, {s.b, s.sq, s.h, s.d}), dk = make(q, {s.b, s.sk, s.hk, s.d}), dv = make(q, {s.b, s.sk, s.hk, s.d});
   Tensor delta = make(q, {s.b, s.h, s.sq}, at::kFloat);
@@ -183,7 +191,8 @@ void describe(tcpxbNormRope& a, Tensor& cos, Tensor& sin, Maybe& wq, Maybe& wk, 
 std::tuple<Tensor, Tensor> normRopeForward(Tensor q, Tensor k, Tensor cos, Tensor sin, Maybe wq, Maybe wk, double eps, Maybe positions) {
   tcpxbNormRope a = checkNormRope(q, k, cos, sin, wq, wk, eps, positions);
   std::optional<c10::cuda::CUDAGuard> guard;
-  const Maybe mk = k, mcos = cos, msin = sin;
+  const Maybe mq = q, mk = k, mcos = cos, msin = sin;
+  noTangent({&mq, &mk, &mcos, &msin, &wq, &wk});
   onDevice(guard, q, {&mk, &mcos, &msin, &wq, &wk, &positions});
   Tensor qOut = make(q, q.sizes()), kOut = make(k, k.sizes());
   describe(a, cos, sin, wq, wk, positions);
@@ -201,7 +210,8 @@ std::tuple<Tensor, Tensor, Maybe, Maybe> normRopeBackward(Tensor dqOut, Tensor d
     TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name, " has to be ", x.scalar_type(), ", got ", t.scalar_type());
   }
   std::optional<c10::cuda::CUDAGuard> guard;
-  const Maybe mk = k, mcos = cos, msin = sin, mdq = dqOut, mdk = dkOut;
+  const Maybe mq = q, mk = k, mcos = cos, msin = sin, mdq = dqOut, mdk = dkOut;
+  noTangent({&mq, &mk, &mcos, &msin, &mdq, &mdk, &wq, &wk});
   onDevice(guard, q, {&mk, &mcos, &msin, &mdq, &mdk, &wq, &wk, &positions});
   Tensor dq = make(q, q.sizes()), dk = make(k, k.sizes()), partial;
   Maybe dwq, dwk;

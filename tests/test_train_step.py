@@ -255,3 +255,25 @@ def test_optimizer_refusals():
     p.grad = torch.zeros(3)
     with pytest.raises(ValueError):  # not on a GPU
         opt.step()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_is_refused(device):
+    """A dual tensor requires no gradient; its tangent is not dropped without a word, through `make_dual` or `torch.func.jvp`."""
+    import torch.autograd.forward_ad as fwd
+    q, k, v = (torch.randn(1, 6, 2, 16, device=device).to(BF16) for _ in range(3))
+    cos, sin = torch.randn(6, 8, device=device), torch.randn(6, 8, device=device)
+    w = torch.ones(16, device=device, dtype=BF16)
+    lse = torch.zeros(1, 2, 6, device=device)
+    calls = [(lambda x: ops.attention(x, k, v), q), (lambda x: ops.attention(q, x, v), k), (lambda x: ops.attention(q, k, x), v),
+             (lambda x: ops.attention_forward(x, k, v)[0], q), (lambda x: ops.attention_backward(x, q, k, v, q, lse)[0], q),
+             (lambda x: ops.qk_norm_rope(x, k, cos, sin)[0], q), (lambda x: ops.qk_norm_rope(q, k, x, sin)[0], cos),
+             (lambda x: ops.qk_norm_rope(q, k, cos, sin, x, w)[0], w), (lambda x: ops.qk_norm_rope_backward(x, k, q, k, cos, sin)[0], q)]
+    for call, x in calls:
+        with fwd.dual_level():
+            # autograd's own refusal, of a tensor that has both, comes behind the forward pass
+            for y in (x,) if device == "cpu" else (x, x.clone().requires_grad_()):
+                with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|jvp"):
+                    call(fwd.make_dual(y, torch.ones_like(x)))
+        with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|jvp"):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
