@@ -107,24 +107,50 @@ template <class L> __global__ void __launch_bounds__(1024) prepareKernel(const _
 
 // Two elements.  m and v are taken in the formula's order, every product and sum rounded by
 // itself: 8-bit codes then fall as those of any plain 32-bit computation do.  The root and the
-// quotient are the approximate ones (2 units in the last place of 32 bits, a v under 2^-126 counts
-// as zero): they touch the weight's own step, and the exact ones would make the 8-bit kernel wait
-// for arithmetic.
+// quotient are the approximate ones (2 units in the last place of 32 bits): they touch the weight's
+// own step, and the exact ones would make the 8-bit kernel wait for arithmetic.  The fastest ones also
+// take a v under 2^-126 for zero.  Next to an `eps` of 2^-39 or more times the root's correction a root
+// under 2^-63 is nothing.  Under that (`eps` zero, or far below the usual ones) it may be all of the
+// denominator, and a denominator's reciprocal may leave the range, as it does for a huge `eps`: kernels
+// of their own (kWide) take roots of any v, and quotients.  (Both forms in one kernel: 1176 us instead of
+// 1161 us for 323 M weights with clipping.)
+template <bool kAll> __device__ __forceinline__ float2 roots(float2 v) {
+  float2 r;
+  if constexpr (kAll) {
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+  } else {
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+  }
+  return r;
+}
+constexpr float kLeastNormal = 0x1p-126f;
+
 struct Step {
   float beta1, beta2, rest1, rest2, eps, keep, stepSize, rootCorrection, coef;
-  __device__ __forceinline__ void operator()(float2& p, float2 g, float2& m, float2& v, float2& root) const {
+  __device__ __forceinline__ void moments(float2 g, float2& m, float2& v) const {
     g = mul2(g, {coef, coef});
     // sums one by one: a packed sum would be contracted with its product, which rounds otherwise
     const float2 m1 = mul2(m, {beta1, beta1}), m2 = mul2(g, {rest1, rest1});
     m = {__fadd_rn(m1.x, m2.x), __fadd_rn(m1.y, m2.y)};
     const float2 v1 = mul2(v, {beta2, beta2}), v2 = mul2(mul2(g, {rest2, rest2}), g);
     v = {__fadd_rn(v1.x, v2.x), __fadd_rn(v1.y, v2.y)};
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.x) : "f"(v.x));
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.y) : "f"(v.y));
+  }
+  template <bool kWide> __device__ __forceinline__ void weights(float2& p, float2 m, float2 root) const {
     float2 below = fma2(root, {rootCorrection, rootCorrection}, {eps, eps});
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(below.x) : "f"(below.x));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(below.y) : "f"(below.y));
-    p = fma2(p, {keep, keep}, mul2(mul2(m, {-stepSize, -stepSize}), below));
+    const float2 move = mul2(m, {-stepSize, -stepSize});
+    if constexpr (kWide) {
+      p = fma2(p, {keep, keep}, {__fdiv_rn(move.x, below.x), __fdiv_rn(move.y, below.y)});
+    } else {
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(below.x) : "f"(below.x));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(below.y) : "f"(below.y));
+      p = fma2(p, {keep, keep}, mul2(move, below));
+    }
+  }
+  template <bool kWide> __device__ __forceinline__ void pair(float2& p, float2 g, float2& m, float2& v) const {
+    moments(g, m, v);
+    weights<kWide>(p, m, roots<kWide>(v));
   }
 };
 
@@ -164,20 +190,20 @@ template <bool kVector, class V, class T> __device__ __forceinline__ void put(T*
 template <class T> __device__ __forceinline__ bool aligned(const T* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // 32-bit states, whole vectors: a thread has two runs of eight elements in flight, 96 bytes each.
-template <class T> __device__ __forceinline__ void stepVectors(const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end) {
+template <class T, bool kWide> __device__ __forceinline__ void stepVectors(const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end) {
   T* p = static_cast<T*>(t.p);
   const T* g = static_cast<const T*>(t.g);
   float *m = static_cast<float*>(t.m), *v = static_cast<float*>(t.v);
 #pragma unroll 2
   for (long long e = begin + threadIdx.x * 8; e < end; e += kThreads * 8) {
-    float2 pp[4], gg[4], mm[4], vv[4], root;
+    float2 pp[4], gg[4], mm[4], vv[4];
     if (t.master) pairs(*reinterpret_cast<const Vec8<float>*>(t.master + e), pp);
     else pairs(*reinterpret_cast<const Vec8<T>*>(p + e), pp);
     pairs(*reinterpret_cast<const Vec8<T>*>(g + e), gg);
     pairs(*reinterpret_cast<const Vec8<float>*>(m + e), mm);
     pairs(*reinterpret_cast<const Vec8<float>*>(v + e), vv);
 #pragma unroll
-    for (int i = 0; i < 4; i++) step(pp[i], gg[i], mm[i], vv[i], root);
+    for (int i = 0; i < 4; i++) step.pair<kWide>(pp[i], gg[i], mm[i], vv[i]);
     *reinterpret_cast<Vec8<float>*>(m + e) = rounded<float>(mm);
     *reinterpret_cast<Vec8<float>*>(v + e) = rounded<float>(vv);
     *reinterpret_cast<Vec8<T>*>(p + e) = rounded<T>(pp);
@@ -186,7 +212,7 @@ template <class T> __device__ __forceinline__ void stepVectors(const tcpxbAdamwT
 }
 
 // 32-bit states, any alignment and the ends: one element a lane, four in flight.
-template <class T> __device__ __forceinline__ void stepElements(const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end) {
+template <class T, bool kWide> __device__ __forceinline__ void stepElements(const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end) {
   T* p = static_cast<T*>(t.p);
   const T* g = static_cast<const T*>(t.g);
   float *m = static_cast<float*>(t.m), *v = static_cast<float*>(t.v);
@@ -199,8 +225,8 @@ template <class T> __device__ __forceinline__ void stepElements(const tcpxbAdamw
     }
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-      float2 w = {pp[i], pp[i + 1]}, m2 = {mm[i], mm[i + 1]}, v2 = {vv[i], vv[i + 1]}, root;
-      step(w, {gg[i], gg[i + 1]}, m2, v2, root);
+      float2 w = {pp[i], pp[i + 1]}, m2 = {mm[i], mm[i + 1]}, v2 = {vv[i], vv[i + 1]};
+      step.pair<kWide>(w, {gg[i], gg[i + 1]}, m2, v2);
       pp[i] = w.x, pp[i + 1] = w.y, mm[i] = m2.x, mm[i + 1] = m2.y, vv[i] = v2.x, vv[i + 1] = v2.y;
     }
 #pragma unroll
@@ -228,21 +254,35 @@ __device__ __forceinline__ float warpTop(float x) {
 // About 310 instructions a block, of which 64 are the step itself: at this count issue and memory
 // take about the same time, so the rest is kept short (the warp's maximum is one instruction, the four
 // factors of a block are taken by four lanes at once).
-template <bool kVector, class T, class W>
+template <bool kVector, bool kWide, class T, class W>
 __device__ __forceinline__ void stepBlock(const Raw<T, W>& r, const tcpxbAdamwTensor& t, const Step& step, long long b, long long end, float& mScale, float& vScale) {
   const int lane = threadIdx.x % 32;
   const long long e = b + lane * 8;
-  float2 pp[4], gg[4], mm[4], vv[4], root[4];
+  float2 pp[4], gg[4], mm[4], root[4];  // `root`: v until its root is taken
   pairs(r.w, pp);
   pairs(r.g, gg);
   decode(r.m, mScale, mm);
-  decode(r.v, vScale, vv);
+  decode(r.v, vScale, root);
   float topM = 0.f, topV = 0.f, least = INFINITY;
   // past the end everything is zero and stays so
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    vv[i] = mul2(vv[i], vv[i]);
-    step(pp[i], gg[i], mm[i], vv[i], root[i]);
+    root[i] = mul2(root[i], root[i]);
+    step.moments(gg[i], mm[i], root[i]);
+    least = min3(least, root[i].x, root[i].y);
+  }
+  if (kWide || least < kLeastNormal) {
+    // the root is a state, which no `eps` hides
+#pragma unroll
+    for (int i = 0; i < 4; i++) root[i] = roots<true>(root[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) root[i] = roots<false>(root[i]);
+  }
+  least = INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    step.weights<kWide>(pp[i], mm[i], root[i]);
     topM = max3(topM, fabsf(mm[i].x), fabsf(mm[i].y));
     topV = max3(topV, root[i].x, root[i].y);
     least = min3(least, root[i].x, root[i].y);
@@ -286,7 +326,7 @@ template <int kBytes> __device__ __forceinline__ void copyAsync(void* to, const 
 constexpr int kSmallWarps = 4, kStages = 4;
 static_assert(kChunk / TCPXB_ADAMW_BLOCK / kSmallWarps <= 32, "a lane holds the scales of one block of its warp");
 
-template <class T, class W> __device__ __forceinline__ void stepBlocks(char* shared, const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end, bool vectors) {
+template <class T, class W, bool kWide> __device__ __forceinline__ void stepBlocks(char* shared, const tcpxbAdamwTensor& t, const Step& step, long long begin, long long end, bool vectors) {
   using Share = Raw<T, W>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   Share* ring = reinterpret_cast<Share*>(shared) + warp * kStages * 32 + lane;  // kStages apart by 32
@@ -322,7 +362,7 @@ template <class T, class W> __device__ __forceinline__ void stepBlocks(char* sha
     const Share r = ring[k % kStages * 32];  // a lane reads what it copied itself
     copy(k + kStages - 1);
     float m = __shfl_sync(0xffffffffu, mScale, k), v = __shfl_sync(0xffffffffu, vScale, k);
-    stepBlock<true>(r, t, step, begin + (warp + kSmallWarps * k) * TCPXB_ADAMW_BLOCK, end, m, v);
+    stepBlock<true, kWide>(r, t, step, begin + (warp + kSmallWarps * k) * TCPXB_ADAMW_BLOCK, end, m, v);
     if (lane == k) mScale = m, vScale = v;
   }
 #pragma unroll 1
@@ -331,7 +371,7 @@ template <class T, class W> __device__ __forceinline__ void stepBlocks(char* sha
     const Share r = {get<false, Vec8<W>>(weights, e, end), get<false, Vec8<T>>(static_cast<const T*>(t.g), e, end),
                      get<false, Codes>(static_cast<const __nv_fp8_storage_t*>(t.m), e, end), get<false, Codes>(static_cast<const __nv_fp8_storage_t*>(t.v), e, end)};
     float m = __shfl_sync(0xffffffffu, mScale, k), v = __shfl_sync(0xffffffffu, vScale, k);
-    stepBlock<false>(r, t, step, b, end, m, v);
+    stepBlock<false, kWide>(r, t, step, b, end, m, v);
     if (lane == k) mScale = m, vScale = v;
   }
   if (warp + kSmallWarps * lane < blocks) {
@@ -358,23 +398,23 @@ __device__ __forceinline__ Step stepOf(const tcpxbAdamw& a, int tensor) {
 }
 __device__ __forceinline__ bool inVectors(const tcpxbAdamwTensor& t) { return aligned(t.p) && aligned(t.g) && aligned(t.m) && aligned(t.v) && aligned(t.master); }
 
-template <class T, class L> __global__ void __launch_bounds__(kThreads, 4) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
+template <class T, bool kWide, class L> __global__ void __launch_bounds__(kThreads, 4) stepKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
   waitForPrevious();
   const Chunk<L> c(l, gridDim.x - 1 - blockIdx.x);
   const tcpxbAdamwTensor t = l.t[c.tensor];
   const Step step = stepOf(a, l.first + c.tensor);
   const long long whole = inVectors(t) ? c.begin + (c.end - c.begin) / 8 * 8 : c.begin;
-  stepVectors<T>(t, step, c.begin, whole);
-  stepElements<T>(t, step, whole, c.end);
+  stepVectors<T, kWide>(t, step, c.begin, whole);
+  stepElements<T, kWide>(t, step, whole, c.end);
 }
 
-template <class T, class W, class L> __global__ void __launch_bounds__(kSmallWarps * 32, sizeof(W) == 2 ? 8 : 4) stepSmallKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
+template <class T, class W, bool kWide, class L> __global__ void __launch_bounds__(kSmallWarps * 32, sizeof(W) == 2 ? 8 : 4) stepSmallKernel(const __grid_constant__ L l, const tcpxbAdamw a) {
   waitForPrevious();
   __shared__ alignas(16) char shared[kSmallWarps * kStages * 32 * sizeof(Raw<T, W>)];
   const Chunk<L> c(l, gridDim.x - 1 - blockIdx.x);
   const tcpxbAdamwTensor t = l.t[c.tensor];
   const Step step = stepOf(a, l.first + c.tensor);
-  stepBlocks<T, W>(shared, t, step, c.begin, c.end, inVectors(t));
+  stepBlocks<T, W, kWide>(shared, t, step, c.begin, c.end, inVectors(t));
 }
 
 template <class T, class L> __global__ void __launch_bounds__(kThreads) squaresKernel(const __grid_constant__ L l, double* partial) {
@@ -484,7 +524,7 @@ template <class T> int squares(const tcpxbAdamwTensor* tensors, int count, doubl
   });
 }
 
-template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw& a, cudaStream_t s) {
+template <class T, bool kWide> int step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw& a, cudaStream_t s) {
   const bool masters = withMasters(tensors, count);
   double* partial = nullptr;
   long long partials = 0;
@@ -497,9 +537,14 @@ template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tc
     const int threads = partials > 1024 ? 1024 : partials > 128 || l.count > 128 ? 384 : 128;
     if (const int rc = launchBehind(partials || l.first, prepareKernel<L>, 1, threads, 0, s, "adamw, rates", l, a, static_cast<const double*>(partial), partials)) return rc;
     if (!chunks) return int(TCPXB_T_OK);
-    if (a.state_bits == 32) return launchBehind(true, stepKernel<T, L>, unsigned(chunks), kThreads, 0, s, "adamw", l, a);
-    return launchBehind(true, masters ? stepSmallKernel<T, float, L> : stepSmallKernel<T, T, L>, unsigned(chunks), kSmallWarps * 32, 0, s, "adamw", l, a);
+    if (a.state_bits == 32) return launchBehind(true, stepKernel<T, kWide, L>, unsigned(chunks), kThreads, 0, s, "adamw", l, a);
+    return launchBehind(true, masters ? stepSmallKernel<T, float, kWide, L> : stepSmallKernel<T, T, kWide, L>, unsigned(chunks), kSmallWarps * 32, 0, s, "adamw", l, a);
   });
+}
+
+template <class T> int step(const tcpxbAdamwTensor* tensors, int count, const tcpxbAdamw& a, cudaStream_t s) {
+  // the correction, 1 / sqrt(1 - b2^t), is largest in the first step; above 2^100 the reciprocal of `eps` would be flushed
+  return a.eps >= 0x1p-39 / sqrt(1 - a.beta2) && a.eps <= 0x1p100 ? step<T, false>(tensors, count, a, s) : step<T, true>(tensors, count, a, s);
 }
 
 template <class T> int gradNorm(const tcpxbAdamwTensor* tensors, int count, float* out, double* partial, cudaStream_t s) {

@@ -171,6 +171,31 @@ def test_small_roots_stay_above_zero_in_8_bits():
 
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-39, 1e-30, 1e-20, 1e-18, 1e-12, 1e-10, 1e33])
+def test_small_second_moments_and_extreme_eps(bits, eps):
+    """Second moments under the 32-bit normal range (1e-39 to 1e-35 here) are the denominator's own part where `eps` is
+    none: a first step is then about the learning rate, as the formula has it."""
+    s = tensors([700], F32, bits, seed=18, steps=0)
+    for n in ("exp_avgs", "exp_avg_sqs") + (("exp_avg_scales", "exp_avg_sq_scales") if bits == 8 else ()):
+        s[n][0].view(torch.uint8).zero_()
+    sign = s["grads"][0].sign()
+    s["grads"][0].copy_(sign * torch.logspace(-18, -16, 700, device="cuda"))
+    how = {**HOW, "betas": (0.9, 0.999), "eps": eps}
+    before = s["params"][0].clone()
+    step_and_check(s, how)
+    if eps <= 1e-30:
+        # lr times |g| / |g|, off by the moments' few roundings (a v of 1e-39 has steps of 1.4e-45); the rest is the decay
+        assert ((before * (1 - 1e-3) - s["params"][0]) / sign - 1e-2).abs().max() < 1e-6
+    if 0 < eps < 1:
+        # nothing has moved yet, nothing moves: zero over a denominator whose reciprocal is out of range is zero
+        for t in s["grads"] + s["exp_avgs"] + s["exp_avg_sqs"] + s.get("exp_avg_scales", []) + s.get("exp_avg_sq_scales", []):
+            t.view(torch.uint8).zero_()
+        step_and_check(s, how)
+        assert s["params"][0].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_bad_gradients_show(bits, bad):
     """They reach their own element (in 8 bits an infinity its block), and with clipping everything."""
