@@ -7,9 +7,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
-#include <unordered_set>
 #include <vector>
 
 #include "tcpxb/train.h"
@@ -243,6 +243,36 @@ template <class Size> void checkList(const char* name, const List& ts, size_t co
   }
 }
 
+// The memory of a call's tensors.  What is written may not share a byte with anything else: two blocks would
+// write the same elements, or read what another one has written, in an order that nothing gives.
+class Ranges {
+ public:
+  void reserve(size_t n) { all_.reserve(n); }
+  void* add(const Tensor& t, bool written) {
+    void* p = t.data_ptr();
+    const auto at = reinterpret_cast<uintptr_t>(p);
+    if (t.numel()) all_.push_back({at, at + t.nbytes(), written});
+    return p;
+  }
+  bool apart() {
+    std::sort(all_.begin(), all_.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t read = 0, write = 0;  // ends so far
+    for (const Range& r : all_) {
+      if (r.begin < (r.written ? std::max(read, write) : write)) return false;
+      uintptr_t& end = r.written ? write : read;
+      end = std::max(end, r.end);
+    }
+    return true;
+  }
+
+ private:
+  struct Range {
+    uintptr_t begin, end;
+    bool written;
+  };
+  std::vector<Range> all_;
+};
+
 Tensor gradNorm(const List& grads) {
   TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
   const auto type = grads[0].scalar_type();
@@ -282,29 +312,28 @@ Maybe adamwStep(const List& params, const List& grads, const List& ms, const Lis
     checkList("masters", *masters, count, at::kFloat, first, size);
   }
   std::vector<tcpxbAdamwTensor> table(count);
-  std::unordered_set<const void*> written;
-  size_t all = 0;
-  const auto write = [&](const Tensor& t) {
-    if (t.numel()) all++, written.insert(t.data_ptr());
-    return t.data_ptr();
-  };
+  Ranges ranges;
+  ranges.reserve(count * 8 + 2);
+  const auto write = [&](const Tensor& t) { return ranges.add(t, true); };
   if (THPVariable_Check(steps.ptr())) {
     const Tensor& t = THPVariable_Unpack(steps.ptr());
     TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, "steps has to be int32, got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.dim() == 1 && size_t(t.size(0)) == count && t.is_contiguous() && t.device() == first.device(), "steps has to be a contiguous [", count,
                       "] on the same device, got ", t.sizes());
-    for (size_t i = 0; i < count; i++) table[i].step = t.data_ptr<int32_t>() + i;
+    auto* first = static_cast<int32_t*>(write(t));
+    for (size_t i = 0; i < count; i++) table[i].step = first + i;
   } else {
     const List list = steps.cast<List>();
     checkList("steps", list, count, at::kInt, first, [](size_t) { return 1; });
     for (size_t i = 0; i < count; i++) table[i].step = static_cast<int32_t*>(write(list[i]));
   }
   for (size_t i = 0; i < count; i++) {
-    table[i].p = write(params[i]), table[i].g = grads[i].data_ptr(), table[i].m = write(ms[i]), table[i].v = write(vs[i]), table[i].n = params[i].numel();
+    table[i].p = write(params[i]), table[i].g = ranges.add(grads[i], false), table[i].m = write(ms[i]), table[i].v = write(vs[i]), table[i].n = params[i].numel();
     if (mScales) table[i].m_scale = static_cast<float*>(write((*mScales)[i])), table[i].v_scale = static_cast<float*>(write((*vScales)[i]));
     if (masters) table[i].master = static_cast<float*>(write((*masters)[i]));
   }
-  TORCH_CHECK_VALUE(written.size() == all, "a tensor is given twice");
+  if (norm) ranges.add(*norm, false);
+  TORCH_CHECK_VALUE(ranges.apart(), "a tensor that is written is given twice, or shares memory with another one");
   const auto good = [](double x) { return x >= 0 && x < INFINITY; };
   TORCH_CHECK_VALUE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && good(eps) && good(lr) && good(decay), "bad numbers: lr ", lr, ", betas (", beta1, ", ",
                     beta2, "), eps ", eps, ", weight_decay ", decay);

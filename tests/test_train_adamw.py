@@ -323,6 +323,34 @@ def test_refusals():
             ops.grad_norm(grads)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_that_share_memory_are_refused(bits):
+    """Views that overlap by an element, at their beginning, end or inside; a gradient, counter or norm that is also written."""
+    def refused(match="shares memory", **change):
+        s = tensors([300, 300], F32, bits, device="cpu")
+        s.update(change)
+        with pytest.raises(ValueError, match=match):
+            ops.adamw_step(**s, **{**HOW, **({"max_grad_norm": 1.0} if "norm" in change else {})})
+
+    buf = torch.zeros(1000)
+    codes = buf.to(tensors([1], F32, bits, device="cpu")["exp_avgs"][0].dtype)
+    for a, b in ((0, 299), (299, 0), (5, 5), (100, 399)):
+        refused(params=[buf[a:a + 300], buf[b:b + 300]])
+        refused(exp_avgs=[codes[a:a + 300], codes[b:b + 300]])
+        refused(exp_avgs=[codes[a:a + 300], torch.zeros_like(codes[:300])], exp_avg_sqs=[torch.zeros_like(codes[:300]), codes[b:b + 300]])
+        refused(params=[buf[a:a + 300], torch.zeros(300)], grads=[torch.zeros(300), buf[b:b + 300]])
+    refused(params=[buf[100:400], torch.zeros(300)], grads=[buf[:101], torch.zeros(300)], match="elements")
+    steps = torch.zeros(2, dtype=torch.int32)
+    refused(steps=[steps[0], steps[0]])
+    refused(steps=buf[:2].view(torch.int32), params=[buf[1:301], torch.zeros(300)])
+    refused(norm=buf[7], params=[buf[:300], torch.zeros(300)])
+    if bits == 8:
+        refused(exp_avg_scales=[buf[:2], buf[1:3]])
+        refused(exp_avg_scales=[buf[:2], buf[2:4]], exp_avg_sq_scales=[buf[4:6], buf[3:5]])
+    # side by side in one buffer, and one gradient for two tensors, are as good as any: only a GPU is missing
+    refused(match="CUDA", params=[buf[:300], buf[300:600]], grads=[buf[600:900]] * 2, steps=[steps[0], steps[1]], norm=buf[999])
+
+
 def test_the_c_entry_refuses():
     import ctypes
     import train_abi as A
