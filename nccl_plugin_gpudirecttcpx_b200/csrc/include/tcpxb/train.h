@@ -52,7 +52,8 @@ typedef struct tcpxbAttention {
   float scale;            // above zero
   int32_t causal, dtype;
   int32_t device;         // that the tensors are on; becomes the calling thread's
-  int32_t* status;        // a word on the device, or null: 3 (TCPXB_ST_TIMEOUT) where a bounded wait ran out
+  int32_t* status;        // a word on the device, or null: 3 (TCPXB_ST_TIMEOUT) where a bounded wait ran out.  The outputs are NaN then,
+                          // and those of calls that find a 3 there: rows that see nothing apart
 } tcpxbAttention;
 
 int tcpxb_attention_forward(const tcpxbAttention* a, void* stream);

@@ -129,6 +129,14 @@ template <int P> __device__ __forceinline__ uint32_t begin(int warp, uint32_t* t
   return uniform(*tmem);
 }
 
+// A block where a wait ran out computes on memory that nothing has filled.  The flag is set before any of that can
+// reach a sum, so the threads that store see it: their factors become NaN, and the outputs show it to a
+// caller who has no status word.  A row that sees nothing is right all the same.
+__device__ __forceinline__ float factor(bool sees, float by, volatile int* dead) { return !sees ? 0.f : *dead ? NAN : by; }
+// Whether the status already tells of a wait that ran out: the block then does no work, so that a grid
+// whose waits run out ends after the first of them, and what follows with the same status is void too.
+__device__ __forceinline__ int isVoid(const int32_t* status) { return status && *reinterpret_cast<const volatile int32_t*>(status) == kStatusTimeout; }
+
 template <int P> __device__ __forceinline__ void finish(const Args& a, uint32_t tmem, volatile int* dead) {
   tcBefore();
   __syncthreads();
@@ -201,14 +209,18 @@ __device__ __forceinline__ float remote(uint32_t at, int rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
   return x;
 }
-// kPart columns of the thread's accumulator row into shared memory.
-template <int kCols, int kPart> __device__ __forceinline__ void leaveRow(uint32_t base, int row, uint32_t tmem, int begin, bool any) {
+// kPart columns of the thread's accumulator row into shared memory; NaN where a wait ran out.
+template <int kCols, int kPart> __device__ __forceinline__ void leaveRow(uint32_t base, int row, uint32_t tmem, int begin, bool any, volatile int* dead) {
+  const float nothing = uniform(*dead) ? NAN : 0.f;  // the loads want the whole warp
 #pragma unroll
   for (int c = 0; c < kPart; c += 32) {
-    uint32_t r[32] = {};
-    if (any) {
+    uint32_t r[32];
+    if (any && nothing == 0.f) {
       tmemLoad32(tmem + begin + c, r);
       tmemWaitLoad();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) r[i] = __float_as_uint(nothing);
     }
 #pragma unroll
     for (int i = 0; i < 32; i += 4)
@@ -262,9 +274,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   int all[2], n[2];  // tiles of keys that a tile of queries sees, and those of this block's part
 #pragma unroll
   for (int t = 0; t < 2; t++) all[t] = q0 + t * kTile < a.sq ? colTiles<P>(seenBy(a, min(q0 + t * kTile + kTile, a.sq) - 1, keys)) : 0;
-  const int every = max(all[0], all[1]), begun = int((long long)every * rank / split), most = int((long long)every * (rank + 1) / split) - begun;
-#pragma unroll
-  for (int t = 0; t < 2; t++) n[t] = min(max(all[t] - begun, 0), most);
+  const int every = max(all[0], all[1]), begun = int((long long)every * rank / split);
 
   const auto loadPair = [&](int i) {  // number i of K_0, V_0, K_1, ...
     const int slot = i % F::kSlots;
@@ -274,13 +284,16 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   if (warp == kLoadWarp) {
     if (lane == 0) {
       for (int i = 0; i < F::kBars; i++) barInit(bar(i), i >= F::kPFull && i < F::kOFull ? 4 : 1);
-      sh.dead = 0;
+      sh.dead = isVoid(a.status);
       fenceBarInit();
       fenceAsyncShared();
     }
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, &sh.tmem);
+  const int most = uniform(*dead) ? 0 : int((long long)every * (rank + 1) / split) - begun;
+#pragma unroll
+  for (int t = 0; t < 2; t++) n[t] = min(max(all[t] - begun, 0), most);
   if (warp == kLoadWarp) {
     L::other();
     if (lane == 0) {
@@ -406,15 +419,15 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
     const bool live = i < a.sq;
     if constexpr (kSplit) {
       asm volatile("bar.sync 1, 256;" ::: "memory");  // the other tile of queries reads the ring to its own end
-      leaveRow<L::kHeadCols, L::kHeadCols>(ring + t * kTile * L::kHeadCols * 4, row, o, 0, n[t] > 0);
-      sh.stats[t][0][row] = top, sh.stats[t][1][row] = sum;
+      leaveRow<L::kHeadCols, L::kHeadCols>(ring + t * kTile * L::kHeadCols * 4, row, o, 0, n[t] > 0, dead);
+      sh.stats[t][0][row] = top, sh.stats[t][1][row] = *dead ? NAN : sum;
     } else {
       // a row that sees nothing is zero, whatever its tile holds
-      const float by = seen > 0 ? 1.f / sum : 0.f;
+      const float by = factor(seen > 0, 1.f / sum, dead);
       const int i0 = i - lane;  // the warp's first row
       storeRows<T, L::kHeadCols>(static_cast<T*>(a.o) + (((long long)b * a.sq + i0) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - i0, o, 0, a.d, by,
                                  n[t] > 0, tile0 + t * F::kQBytes + warp % 4 * (F::kQBytes / 4));
-      if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? (top * c + log2f(sum)) * kLn2 : -INFINITY;
+      if (live) a.lse[((long long)b * a.heads + h) * a.sq + i] = seen > 0 ? by == by ? (top * c + log2f(sum)) * kLn2 : by : -INFINITY;
     }
   } else {
     L::other();
@@ -488,7 +501,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * kTile, h = blockIdx.x / split, rank = blockIdx.x % split, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
   // tiles of keys that the queries see, and this block's part of them
   const int keys = keysOf(a, b), all = colTiles<P>(seenBy(a, min(q0 + kTile, a.sq) - 1, keys));
-  const int begun = int((long long)all * rank / split), n = int((long long)all * (rank + 1) / split) - begun;
+  const int begun = int((long long)all * rank / split);
 
   const auto loadKeys = [&](int j) {
     const int ks = j % F::kKSlots;
@@ -503,13 +516,14 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   if (warp == kLoadWarp) {
     if (lane == 0) {
       for (int i = 0; i < F::kBars; i++) barInit(bar(i), i == F::kDsFull ? kComputeWarps : 1);
-      *dead = 0;
+      *dead = isVoid(a.status);
       fenceBarInit();
       fenceAsyncShared();
     }
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, tmemAt), dp = tmem + 2 * kCols, dq = tmem + 3 * kCols;
+  const int n = uniform(*dead) ? 0 : int((long long)all * (rank + 1) / split) - begun;
   letNextStart();  // all blocks have their tensor memory
 
   if (warp == kLoadWarp) {
@@ -660,11 +674,12 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
       barWait(bar(F::kDone), 0, dead);
       tcAfter();
     }
+    if (*dead && half == 0 && seen > 0) a.delta[stat] = NAN;
     if constexpr (kSplit)
-      leaveRow<L::kHeadCols, L::kHeadCols / 2>(kRing, row, dq + lanes, half * L::kHeadCols / 2, n > 0);
+      leaveRow<L::kHeadCols, L::kHeadCols / 2>(kRing, row, dq + lanes, half * L::kHeadCols / 2, n > 0, dead);
     else
       storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dq) + (((long long)b * a.sq + i - lane) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - (i - lane),
-                                     dq + lanes, half * L::kHeadCols / 2, a.d, seen > 0 ? a.scale : 0.f, n > 0, qTile + warp * (F::kQBytes / 8));
+                                     dq + lanes, half * L::kHeadCols / 2, a.d, factor(seen > 0, a.scale, dead), n > 0, qTile + warp * (F::kQBytes / 8));
   } else {
     L::other();
   }
@@ -716,19 +731,20 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   const int first = a.causal ? max(0, j0 - (a.sk - a.sq)) / kCols : 0;  // first query tile that sees a key of this one
   const int each = j0 < keys ? max(0, colTiles<P>(a.sq) - first) : 0, all = each * group;
   // this block's part of the tiles
-  const int begun = int((long long)all * rank / split), n = int((long long)all * (rank + 1) / split) - begun;
+  const int begun = int((long long)all * rank / split);
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
       for (int i = 0; i < F::kBars; i++)
         barInit(bar(i), i == F::kPFull || i == F::kDsFull ? kComputeWarps : i >= F::kFull && i < F::kEmpty ? 33 : 1);
-      sh.dead = 0;
+      sh.dead = isVoid(a.status);
       fenceBarInit();
       fenceAsyncShared();
     }
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, &sh.tmem), s = tmem, dp = tmem + kCols, dv = tmem + 2 * kCols, dk = dv + L::kHeadCols;
+  const int n = uniform(*dead) ? 0 : int((long long)all * (rank + 1) / split) - begun;
   waitForPrevious();  // for delta
 
   if (warp == kLoadWarp) {
@@ -898,14 +914,14 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
       const int jw = j - lane;  // the warp's first row
       const long long at = (((long long)b * a.sk + jw) * a.kvHeads + kv) * a.d;
       const int64_t stride = (int64_t)a.kvHeads * a.d;
-      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dv) + at, stride, a.sk - jw, dv + lanes, half * L::kHeadCols / 2, a.d, counts ? 1.f : 0.f, n > 0,
+      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dv) + at, stride, a.sk - jw, dv + lanes, half * L::kHeadCols / 2, a.d, factor(counts, 1.f, dead), n > 0,
                                      vTileAt + warp * (F::kKBytes / 8));
-      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dk) + at, stride, a.sk - jw, dk + lanes, half * L::kHeadCols / 2, a.d, counts ? a.scale : 0.f, n > 0,
+      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dk) + at, stride, a.sk - jw, dk + lanes, half * L::kHeadCols / 2, a.d, factor(counts, a.scale, dead), n > 0,
                                      kTileAt + warp * (F::kKBytes / 8));
     } else {
       // the tiles of the ring are done with: dv, then dk, in 32 bits
-      leaveRow<L::kHeadCols, L::kHeadCols / 2>(ring, row, dv + lanes, half * L::kHeadCols / 2, n > 0);
-      leaveRow<L::kHeadCols, L::kHeadCols / 2>(ring + kTile * L::kHeadCols * 4, row, dk + lanes, half * L::kHeadCols / 2, n > 0);
+      leaveRow<L::kHeadCols, L::kHeadCols / 2>(ring, row, dv + lanes, half * L::kHeadCols / 2, n > 0, dead);
+      leaveRow<L::kHeadCols, L::kHeadCols / 2>(ring + kTile * L::kHeadCols * 4, row, dk + lanes, half * L::kHeadCols / 2, n > 0, dead);
     }
   } else {
     L::other();

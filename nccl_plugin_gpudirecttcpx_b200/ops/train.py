@@ -40,8 +40,8 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
     `key_lengths` ([batch], int32): keys at and behind a batch's length are not seen, whatever they
     hold.  A query that sees no key gets zeros.  `out` is contiguous; `lse` [batch, heads, queries]
     (float32) is the natural logarithm of each row's sum of exponentials, -inf for an empty row.
-    `status` (`ops.status_buffer()`): its first word becomes 3 where a wait inside the kernel ran out of
-    time and the outputs are void."""
+    Where a wait inside the kernel runs out of time, the rows that it concerns become NaN; with `status`
+    (`ops.status_buffer()`) its first word becomes 3, and calls that find a 3 there leave NaN."""
     return _m().attention_forward(q, k, v, causal, scale, key_lengths, status)
 
 

@@ -179,6 +179,35 @@ def test_status_stays_zero():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,causal", [
+    (1, 1, 1, 1, 1, 8, False), (2, 300, 300, 4, 2, 64, True), (2, 300, 300, 4, 2, 128, True), (1, 40, 3000, 2, 1, 64, False), (1, 40, 3000, 2, 1, 128, True),
+    (1, 700, 20, 8, 1, 40, False), (16, 513, 513, 8, 2, 64, True), (3, 150, 90, 4, 4, 96, True)])
+def test_void_outputs_are_nan(b, sq, sk, h, hk, d, causal, dtype):
+    """A status that tells of a wait that ran out makes what follows void: no work, NaN wherever a row sees something, the status
+    kept.  Blocks alone and in clusters, rows that see nothing, ends of tiles; with the status cleared all is as before."""
+    q, k, v, dout = inputs(b, sq, sk, h, hk, d, dtype, seed=14)
+    status = ops.status_buffer()
+    out, lse = ops.attention_forward(q, k, v, causal=causal, status=status)
+    want = out, lse, *ops.attention_backward(dout, q, k, v, out, lse, causal=causal, status=status)
+    kept = [t.clone() for t in (q, k, v, dout, out, lse)]
+    assert not status.any()
+    status[0] = 3
+    got = *ops.attention_forward(q, k, v, causal=causal, status=status), *ops.attention_backward(dout, q, k, v, out, lse, causal=causal, status=status)
+    sees = oracle.visible(b, sq, sk, causal, None).any(-1).cuda()  # [b, 1, sq]
+    assert got[1].isnan().eq(sees).all() and (got[1][~sees.expand_as(lse)] == -math.inf).all()
+    rows = sees.transpose(1, 2)[..., None]
+    for x in (got[0], got[2]):
+        assert x.isnan().eq(rows).all() and not x[~rows.expand_as(x)].any()
+    assert got[3].isnan().all() and got[4].isnan().all()
+    assert status.tolist() == [3] + [0] * (status.numel() - 1)
+    assert all(torch.equal(x, y) for x, y in zip(kept, (q, k, v, dout, out, lse)))
+    status.zero_()
+    got = *ops.attention_forward(q, k, v, causal=causal, status=status), *ops.attention_backward(dout, q, k, v, out, lse, causal=causal, status=status)
+    assert all(torch.equal(x, y) for x, y in zip(want, got)) and not status.any()
+
+
+@gpu
 @pytest.mark.parametrize("b,sq,sk", [(0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 0)])
 def test_nothing_to_do(b, sq, sk):
     q, k, v, dout = inputs(b, sq, sk, 4, 2, 64, BF16)
