@@ -108,7 +108,7 @@ template <int P> __device__ __forceinline__ void clearRows(uint32_t tile, int fi
 struct Shared {
   uint64_t bars[32];
   uint32_t tmem;
-  int dead;
+  int dead[2];  // a wait has run out; the block has its tensor memory
   alignas(16) float stats[4][2][kTile];  // lse and D of a stage's queries
 };
 constexpr int kSharedBytes = 6144;
@@ -266,7 +266,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const uint32_t tile0 = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, ring = tile0 + 2 * F::kQBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
-  volatile int* dead = &sh.dead;
+  volatile int* dead = sh.dead;
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   // the longest blocks first, over all heads and batches: with a causal mask the last queries see the most keys
   const int q0 = (int(gridDim.z) - 1 - int(blockIdx.z)) * 2 * kTile, h = blockIdx.x / split, rank = blockIdx.x % split, b = blockIdx.y, kv = h / (a.heads / a.kvHeads);
@@ -284,13 +284,14 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   if (warp == kLoadWarp) {
     if (lane == 0) {
       for (int i = 0; i < F::kBars; i++) barInit(bar(i), i >= F::kPFull && i < F::kOFull ? 4 : 1);
-      sh.dead = isVoid(a.status);
+      dead[0] = isVoid(a.status), dead[1] = 0;
       fenceBarInit();
       fenceAsyncShared();
     }
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, &sh.tmem);
+  if (warp == kMmaWarp) dead[1] = 1;
   const int most = uniform(*dead) ? 0 : int((long long)every * (rank + 1) / split) - begun;
 #pragma unroll
   for (int t = 0; t < 2; t++) n[t] = min(max(all[t] - begun, 0), most);
@@ -516,13 +517,14 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   if (warp == kLoadWarp) {
     if (lane == 0) {
       for (int i = 0; i < F::kBars; i++) barInit(bar(i), i == F::kDsFull ? kComputeWarps : 1);
-      *dead = isVoid(a.status);
+      dead[0] = isVoid(a.status), dead[1] = 0;
       fenceBarInit();
       fenceAsyncShared();
     }
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, tmemAt), dp = tmem + 2 * kCols, dq = tmem + 3 * kCols;
+  if (warp == kMmaWarp) dead[1] = 1;
   const int n = uniform(*dead) ? 0 : int((long long)all * (rank + 1) / split) - begun;
   letNextStart();  // all blocks have their tensor memory
 
@@ -724,7 +726,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const uint32_t kTileAt = (smemAddr(raw) + kSharedBytes + 1023) / 1024 * 1024, vTileAt = kTileAt + F::kKBytes, ring = vTileAt + F::kKBytes;
   const auto bar = [&](int i) { return smemAddr(sh.bars) + 8 * i; };
-  volatile int* dead = &sh.dead;
+  volatile int* dead = sh.dead;
   const int warp = uniform(int(threadIdx.x) / 32), lane = threadIdx.x % 32;
   const int j0 = blockIdx.z * kTile, kv = blockIdx.x / split, rank = blockIdx.x % split, b = blockIdx.y, group = a.heads / a.kvHeads;
   const int keys = keysOf(a, b);
@@ -737,13 +739,14 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
     if (lane == 0) {
       for (int i = 0; i < F::kBars; i++)
         barInit(bar(i), i == F::kPFull || i == F::kDsFull ? kComputeWarps : i >= F::kFull && i < F::kEmpty ? 33 : 1);
-      sh.dead = isVoid(a.status);
+      dead[0] = isVoid(a.status), dead[1] = 0;
       fenceBarInit();
       fenceAsyncShared();
     }
     __syncwarp();
   }
   const uint32_t tmem = begin<P>(warp, &sh.tmem), s = tmem, dp = tmem + kCols, dv = tmem + 2 * kCols, dk = dv + L::kHeadCols;
+  if (warp == kMmaWarp) dead[1] = 1;
   const int n = uniform(*dead) ? 0 : int((long long)all * (rank + 1) / split) - begun;
   waitForPrevious();  // for delta
 

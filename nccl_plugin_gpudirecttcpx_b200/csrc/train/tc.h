@@ -48,15 +48,17 @@ __device__ __forceinline__ uint64_t nowNs() {
 }
 // Waits for the phase of `parity` to end, two seconds at most.  After that `*dead` makes every wait
 // of the block return at once: its loops run to their end on whatever memory they own, and the
-// block reports a timeout.
+// block reports a timeout.  Until `dead[1]` tells that the block has its tensor memory the two seconds
+// do not begin: another kernel may hold that for any time, and the products do not start before.
 __device__ __forceinline__ void barWaitLong(uint32_t bar, uint32_t parity, volatile int* dead) {
 #pragma unroll 1
   for (int i = 0; i < 64; i++)
     if (barTry(bar, parity)) return;
-  const uint64_t began = nowNs();
+  uint64_t began = nowNs();
 #pragma unroll 1
   while (!barTry(bar, parity)) {
     if (*dead) return;
+    if (!dead[1]) began = nowNs();
     if (nowNs() - began > 2000000000ull) {
       *dead = 1;
       return;

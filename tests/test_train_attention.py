@@ -207,6 +207,58 @@ def test_void_outputs_are_nan(b, sq, sk, h, hk, d, causal, dtype):
     assert all(torch.equal(x, y) for x, y in zip(want, got)) and not status.any()
 
 
+HOLDER = r"""
+#include <cstdint>
+// Holds an SM's tensor memory for some time, beside whatever else finds room there.
+__global__ void hold(unsigned long long ns) {
+  __shared__ uint32_t at;
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"((uint32_t)__cvta_generic_to_shared(&at)) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  do {
+    __nanosleep(100000);
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  } while (t - t0 < ns);
+  __syncwarp();
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(at) : "memory");
+}
+extern "C" int run(int blocks, unsigned long long ns, void* stream) {
+  const int room = 118 << 10;  // one block on an SM, and room for one of attention's
+  if (cudaFuncSetAttribute(hold, cudaFuncAttributeMaxDynamicSharedMemorySize, room)) return 1;
+  hold<<<blocks, 32, room, (cudaStream_t)stream>>>(ns);
+  return cudaGetLastError();
+}
+"""
+
+
+@gpu
+def test_tensor_memory_that_another_kernel_holds(tmp_path):
+    """Blocks that get their tensor memory later than a wait may last: no wait runs out over it."""
+    import ctypes
+    import subprocess
+    import time
+    from nccl_plugin_gpudirecttcpx_b200 import _build
+    (tmp_path / "hold.cu").write_text(HOLDER)
+    subprocess.run([_build._nvcc(), *_build.NVCC_ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", tmp_path / "hold.so", tmp_path / "hold.cu"], check=True)
+    hold = ctypes.CDLL(str(tmp_path / "hold.so")).run
+    hold.argtypes = ctypes.c_int, ctypes.c_uint64, ctypes.c_void_p
+    q, k, v, dout = inputs(8, 900, 900, 8, 2, 64, BF16, seed=15)  # rings that wrap
+    status = ops.status_buffer()
+    out, lse = ops.attention_forward(q, k, v, status=status)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    assert hold(torch.cuda.get_device_properties(0).multi_processor_count, 2_600_000_000, side.cuda_stream) == 0
+    time.sleep(0.2)
+    began = time.time()
+    again = ops.attention_forward(q, k, v, status=status)
+    torch.cuda.current_stream().synchronize()
+    waited = time.time() - began
+    torch.cuda.synchronize()
+    assert not status.any() and torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    assert waited > 2.1  # else nothing was held
+
+
 @gpu
 @pytest.mark.parametrize("b,sq,sk", [(0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 0)])
 def test_nothing_to_do(b, sq, sk):
