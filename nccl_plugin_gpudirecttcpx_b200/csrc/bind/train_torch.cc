@@ -134,12 +134,13 @@ std::tuple<Tensor, Tensor, Tensor> attentionBackward(Tensor dout, Tensor q, Tens
   noTangent({&mq, &mk, &mv, &mdout, &mout, &mlse});
   onDevice(guard, q, {&mk, &mv, &mdout, &mout, &mlse, &lengths, &status});
   Tensor dq = make(q, {s.b, s.sq, s.h, s.d}), dk = make(q, {s.b, s.sk, s.hk, s.d}), dv = make(q, {s.b, s.sk, s.hk, s.d});
-  Tensor delta = make(q, {s.b, s.h, s.sq}, at::kFloat);
+  Tensor delta = make(q, {s.b, s.h, s.sq}, at::kFloat), bounds;
   out = aligned(out), lse = lse.contiguous();
   tcpxbAttention a = describe(q, k, v, s, causal, lengths, status);
   a.dout = heads(dout);
   a.out = out.data_ptr(), a.lse = lse.data_ptr<float>(), a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv = dv.data_ptr();
+  if (q.scalar_type() == at::kHalf) bounds = make(q, {s.b, s.hk, 64}, at::kFloat), a.bounds = bounds.data_ptr<float>();
   done(tcpxb_attention_backward(&a, streamOf(q)), "tcpxb_attention_backward");
   return {dq, dk, dv};
 }

@@ -54,6 +54,7 @@ typedef struct tcpxbAttention {
   int32_t device;         // that the tensors are on; becomes the calling thread's
   int32_t* status;        // a word on the device, or null: 3 (TCPXB_ST_TIMEOUT) where a bounded wait ran out.  The outputs are NaN then,
                           // and those of calls that find a 3 there: rows that see nothing apart
+  float* bounds;          // [b, kv_heads, 64] scratch, on an 8-byte boundary; backward of fp16 only, not read else
 } tcpxbAttention;
 
 int tcpxb_attention_forward(const tcpxbAttention* a, void* stream);

@@ -28,7 +28,9 @@
 // behind that one without a wait: the matrix instructions of a block run in the order of issue.
 //
 // Probabilities and score gradients are rounded to the inputs' type because the matrix units take
-// operands of one type; sums, statistics and everything else are 32-bit.
+// operands of one type; sums, statistics and everything else are 32-bit.  In float16, whose range ends at
+// 2^-24, the backward pass lifts both by powers of two and takes those out of the sums: see boundsKernel.
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <type_traits>
@@ -65,8 +67,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct Args {
   CUtensorMap q, k, v, dout;
   const void* out;
-  const void* doutPtr;
-  int64_t doutB, doutS, doutH;
+  const void *doutPtr, *vPtr;
+  int64_t doutB, doutS, doutH, vB, vS, vH;
+  const float2* bounds;
+  int parts;
   void *o, *dq, *dk, *dv;
   float *lse, *delta;
   const int32_t* keyLengths;
@@ -467,6 +471,84 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   finish<P>(a, tmem, dead);
 }
 
+// ------------------------------------------------------------------ backward, range of float16
+// A probability among thousands of keys times a gradient of 1e-4 is under float16's smallest step, and
+// dq and dk would be sums of zeros.  |dP_ij| and |D_i| are at most d max|dout| max|v| =: X, so the score
+// gradients stay under 2.01 X: multiplied by 2^e with 2^13 <= 2^e X < 2^14 none of them overflows, and
+// what still falls under the smallest step is 2^-38 of X.  It is exact and costs no instruction in the
+// loops (a sum becomes a multiply-add).  Probabilities, at most one, are lifted by 2^14 for dv.
+//
+// The maxima are taken over each key head's group and batch, over the rows that see a key and the keys
+// that can be seen; infinities and NaN are left out.  Up to kParts blocks share a key head's rows, about two
+// blocks to an SM in all, and each leaves the maxima of its own; a kernel that needs them takes them of all.
+// Memory-bound: every element of dout and v is read once, 14.8 us for 4 x 2048 tokens, 32/8 heads of 64 (42 MB; 17.6 us
+// with a few blocks more than find room at once), of 480 us both ways.
+constexpr int kParts = 32, kBoundsThreads = 1024;
+constexpr float kProbabilityLift = 14.f, kProbabilityDrop = 0x1p-14f;  // the exponent, and what takes it out again
+
+template <class T, int P> __global__ void __launch_bounds__(kBoundsThreads) boundsKernel(const __grid_constant__ Args a, float2* out) {
+  letNextStart();
+  constexpr int kWarps = kBoundsThreads / 32, kLanes = P * 8, kRows = kBoundsThreads / kLanes, kAhead = 4;
+  const int kv = blockIdx.y, b = blockIdx.z, part = blockIdx.x, group = a.heads / a.kvHeads, keys = keysOf(a, b);
+  const int col = int(threadIdx.x) % kLanes * 8;
+  // of tokens [first, end): those of this part, all heads of a token side by side
+  const auto most = [&](const T* x, int64_t token, int64_t head, int heads, int first, int end) {
+    const int chunk = (end - first + a.parts - 1) / a.parts, begin = first + part * chunk;
+    const int count = (min(begin + chunk, end) - begin) * heads;
+    float top = 0.f;
+    if (col >= a.d) return top;
+    for (int i0 = int(threadIdx.x) / kLanes; i0 < count; i0 += kRows * kAhead) {
+      Vec8<T> raw[kAhead] = {};
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        const int i = i0 + u * kRows;
+        if (i < count) raw[u] = *reinterpret_cast<const Vec8<T>*>(x + (begin + i / heads) * token + i % heads * head + col);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        float2 f[4];
+        pairs(raw[u], f);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float m = fabsf(f[k].x), n = fabsf(f[k].y);
+          top = max3(top, m < INFINITY ? m : 0.f, n < INFINITY ? n : 0.f);
+        }
+      }
+    }
+    return top;
+  };
+  const int seeing = keys ? a.causal ? max(0, a.sq - a.sk) : 0 : a.sq;  // first query that sees a key
+  const float g = most(static_cast<const T*>(a.doutPtr) + b * a.doutB + kv * group * a.doutH, a.doutS, a.doutH, group, seeing, a.sq);
+  const float v = most(static_cast<const T*>(a.vPtr) + b * a.vB + kv * a.vH, a.vS, 0, 1, 0, keys);
+  // values above zero are ordered as their bits are
+  __shared__ unsigned tops[2][kWarps];
+  const unsigned x = __reduce_max_sync(0xffffffffu, __float_as_uint(g)), y = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+  if (threadIdx.x % 32 == 0) tops[0][threadIdx.x / 32] = x, tops[1][threadIdx.x / 32] = y;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const unsigned m = __reduce_max_sync(0xffffffffu, tops[0][threadIdx.x]), n = __reduce_max_sync(0xffffffffu, tops[1][threadIdx.x]);
+    if (threadIdx.x == 0) out[((long long)b * a.kvHeads + kv) * kParts + part] = {__uint_as_float(m), __uint_as_float(n)};
+  }
+}
+
+template <class T> constexpr bool kLifted = std::is_same_v<T, __half>;
+// 2^e, for a warp.
+template <class T> __device__ __forceinline__ float liftOf(const Args& a, int b, int kv) {
+  if (!kLifted<T> || !a.bounds) return 1.f;
+  const int part = threadIdx.x % 32;
+  const float2 top = part < a.parts ? a.bounds[((long long)b * a.kvHeads + kv) * kParts + part] : float2{};
+  const unsigned x = __reduce_max_sync(0xffffffffu, __float_as_uint(top.x)), y = __reduce_max_sync(0xffffffffu, __float_as_uint(top.y));
+  const unsigned all = __float_as_uint(__uint_as_float(x) * __uint_as_float(y) * float(a.d));  // 2^-45 to 2^39, or none
+  return all ? __uint_as_float((127 + 13 + 127 - (all >> 23)) << 23) : 1.f;
+}
+// 1 / x of a power of two.
+__device__ __forceinline__ float reciprocal(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+// (y + minus) * lift, where `minus` has been lifted already.
+template <class T> __device__ __forceinline__ float2 lifted(float2 y, float lift, float2 minus) {
+  if constexpr (kLifted<T>) return fma2(y, {lift, lift}, minus);
+  else return add2(y, minus);
+}
+
 // ------------------------------------------------------------------ backward, queries
 // A block owns 128 queries and goes through the key tiles:  S = Q K^T, dP = dout V^T, then
 // dq += dS K.  Two buffers of scores: the next tile's exponentials start while the matrix units
@@ -526,6 +608,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   const uint32_t tmem = begin<P>(warp, tmemAt), dp = tmem + 2 * kCols, dq = tmem + 3 * kCols;
   if (warp == kMmaWarp) dead[1] = 1;
   const int n = uniform(*dead) ? 0 : int((long long)all * (rank + 1) / split) - begun;
+  if constexpr (kLifted<T>) waitForPrevious();  // for the bounds
   letNextStart();  // all blocks have their tensor memory
 
   if (warp == kLoadWarp) {
@@ -611,6 +694,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
       if (live && all != 1 && rank == 0) a.delta[stat] = sum;
       deltas[row] = sum;
     }
+    const float lift = liftOf<T>(a, b, kv);
     asm volatile("bar.sync 1, 256;" ::: "memory");
     float delta = deltas[row];
     // a row that sees nothing, or lies behind the last query, has no probabilities
@@ -652,10 +736,11 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
         asm volatile("bar.sync 1, 256;" ::: "memory");
         delta = deltas[row];
       }
+      const float minus = kLifted<T> ? -delta * lift : -delta;
       const auto gradients = [&](auto masked) {
 #pragma unroll
         for (int k = 0; k < kHalf; k += 2) {
-          float2 g = add2({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, {-delta, -delta});
+          float2 g = lifted<T>({__uint_as_float(y[k]), __uint_as_float(y[k + 1])}, lift, {minus, minus});
           g = mul2({__uint_as_float(x[k]), __uint_as_float(x[k + 1])}, g);
           if (decltype(masked)::value) {
             g.x = k < left ? g.x : 0.f;
@@ -681,7 +766,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
       leaveRow<L::kHeadCols, L::kHeadCols / 2>(kRing, row, dq + lanes, half * L::kHeadCols / 2, n > 0, dead);
     else
       storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dq) + (((long long)b * a.sq + i - lane) * a.heads + h) * a.d, (int64_t)a.heads * a.d, a.sq - (i - lane),
-                                     dq + lanes, half * L::kHeadCols / 2, a.d, factor(seen > 0, a.scale, dead), n > 0, qTile + warp * (F::kQBytes / 8));
+                                     dq + lanes, half * L::kHeadCols / 2, a.d, factor(seen > 0, a.scale * reciprocal(lift), dead), n > 0, qTile + warp * (F::kQBytes / 8));
   } else {
     L::other();
   }
@@ -689,13 +774,14 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
     clusterSync();
     if (warp < kComputeWarps) {
       const int rows = kTile / split, chunks = a.d / 8, count = rows * chunks;
+      const float by = a.scale * reciprocal(liftOf<T>(a, b, kv));
       for (int k = threadIdx.x; k < count; k += kComputeWarps * 32) {
         const int row = rank * rows + k / chunks, chunk = k % chunks, i = q0 + row;
         float sum[8] = {};
         for (int r = 0; r < split; r++) addRow8<L::kHeadCols>(kRing, row, chunk, r, 1.f, sum);
         if (i < a.sq)
           *reinterpret_cast<uint4*>(static_cast<T*>(a.dq) + (((long long)b * a.sq + i) * a.heads + h) * a.d + chunk * 8) =
-              rounded8<T>(reinterpret_cast<const uint32_t*>(sum), seenBy(a, i, keys) > 0 ? a.scale : 0.f);
+              rounded8<T>(reinterpret_cast<const uint32_t*>(sum), seenBy(a, i, keys) > 0 ? by : 0.f);
       }
     }
     clusterSync();  // nobody leaves while its sums are read
@@ -757,6 +843,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
       loadTile<P, kTile>(kTileAt, &a.k, bar(F::kKvFull), j0, kv, b);
       loadTile<P, kTile>(vTileAt, &a.v, bar(F::kKvFull), j0, kv, b);
     }
+    const float lift = kLifted<T> ? liftOf<T>(a, b, kv) * kProbabilityDrop : 1.f;
     for (int it = 0, h = kv * group + (n ? begun / each : 0), qt = n ? begun % each : 0; it < n; it++) {
       const int st = it % F::kStages, turn = it / F::kStages, q0 = (first + qt) * kCols;
       const long long stat = ((long long)b * a.heads + h) * a.sq;
@@ -767,6 +854,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
         l[u] = i < a.sq ? a.lse[stat + i] * -kLog2e : -INFINITY;
         if (l[u] == INFINITY) l[u] = -INFINITY;
         d[u] = i < a.sq ? -a.delta[stat + i] : 0.f;
+        if constexpr (kLifted<T>) l[u] += kProbabilityLift, d[u] *= lift;
       }
       if (turn) barWait(bar(F::kEmpty + st), (turn - 1) & 1, dead);
       if (lane == 0) {
@@ -828,6 +916,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
     // whose statistics it reads from shared memory once for four rows.  (With a row to a thread
     // every statistic went to every thread, and reading them took as long as the exponentials.)
     constexpr int kBlocks8 = kHalf / 8, kRegs = kHalf / 2;
+    const float whole = liftOf<T>(a, b, kv), lift = kLifted<T> ? whole * kProbabilityDrop : 1.f;
     const int row0 = warp % 4 * 32 + lane / 4, col0 = lane % 4 * 2;
     for (int it = 0, qt = n ? begun % each : 0; it < n; it++) {
       const int st = it % F::kStages, q0 = (first + qt) * kCols;
@@ -892,7 +981,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
 #pragma unroll
           for (int u = 0; u < 4; u++) {
             uint32_t *v = x[u / 2] + k * 4 + u % 2 * 2, *w = y[u / 2] + k * 4 + u % 2 * 2;
-            float2 g = add2({__uint_as_float(w[0]), __uint_as_float(w[1])}, ds);
+            float2 g = lifted<T>({__uint_as_float(w[0]), __uint_as_float(w[1])}, lift, ds);
             g = mul2({__uint_as_float(v[0]), __uint_as_float(v[1])}, g);
             if (decltype(masked)::value) {
               g.x = k * 8 >= from(row0 + u * 8) ? g.x : 0.f;
@@ -917,9 +1006,9 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
       const int jw = j - lane;  // the warp's first row
       const long long at = (((long long)b * a.sk + jw) * a.kvHeads + kv) * a.d;
       const int64_t stride = (int64_t)a.kvHeads * a.d;
-      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dv) + at, stride, a.sk - jw, dv + lanes, half * L::kHeadCols / 2, a.d, factor(counts, 1.f, dead), n > 0,
+      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dv) + at, stride, a.sk - jw, dv + lanes, half * L::kHeadCols / 2, a.d, factor(counts, kLifted<T> ? kProbabilityDrop : 1.f, dead), n > 0,
                                      vTileAt + warp * (F::kKBytes / 8));
-      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dk) + at, stride, a.sk - jw, dk + lanes, half * L::kHeadCols / 2, a.d, factor(counts, a.scale, dead), n > 0,
+      storeRows<T, L::kHeadCols / 2>(static_cast<T*>(a.dk) + at, stride, a.sk - jw, dk + lanes, half * L::kHeadCols / 2, a.d, factor(counts, a.scale * reciprocal(whole), dead), n > 0,
                                      kTileAt + warp * (F::kKBytes / 8));
     } else {
       // the tiles of the ring are done with: dv, then dk, in 32 bits
@@ -932,6 +1021,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   if constexpr (kSplit) {
     clusterSync();
     if (warp < kComputeWarps) {
+      const float byV = kLifted<T> ? kProbabilityDrop : 1.f, byK = a.scale * reciprocal(liftOf<T>(a, b, kv));
       const int rows = kTile / split, row0 = rank * rows, chunks = a.d / 8, count = 2 * rows * chunks;
       for (int i = threadIdx.x; i < count; i += kComputeWarps * 32) {
         const int which = i / (rows * chunks), row = row0 + i / chunks % rows, c = i % chunks, j = j0 + row;
@@ -939,7 +1029,7 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
         for (int r = 0; r < split; r++) addRow8<L::kHeadCols>(ring + which * kTile * L::kHeadCols * 4, row, c, r, 1.f, sum);
         if (j >= a.sk) continue;
         T* out = static_cast<T*>(which ? a.dk : a.dv) + (((long long)b * a.sk + j) * a.kvHeads + kv) * a.d + c * 8;
-        *reinterpret_cast<uint4*>(out) = rounded8<T>(reinterpret_cast<const uint32_t*>(sum), j >= keys ? 0.f : which ? a.scale : 1.f);
+        *reinterpret_cast<uint4*>(out) = rounded8<T>(reinterpret_cast<const uint32_t*>(sum), j >= keys ? 0.f : which ? byK : byV);
       }
     }
     clusterSync();  // nobody leaves while its sums are read
@@ -994,6 +1084,8 @@ int check(const tcpxbAttention* a, bool backward) {
     return fail(TCPXB_T_INVALID, "q, out or lse is null, off the 16-byte boundary or broadcast");
   if (keys && (!stridesOk(a->k, a->b, a->sk, a->kv_heads) || !stridesOk(a->v, a->b, a->sk, a->kv_heads)))
     return fail(TCPXB_T_INVALID, "k or v is null, off the 16-byte boundary or broadcast");
+  if (backward && queries && a->dtype == TCPXB_T_F16 && (!a->bounds || reinterpret_cast<uintptr_t>(a->bounds) % 8))
+    return fail(TCPXB_T_INVALID, "fp16 gradients need `bounds`, on an 8-byte boundary");
   if (backward && ((queries && (!stridesOk(a->dout, a->b, a->sq, a->heads) || !a->dq || !a->delta)) || (keys && (!a->dk || !a->dv))))
     return fail(TCPXB_T_INVALID, "dout, dq, dk, dv or delta is null, off the 16-byte boundary or broadcast");
   return TCPXB_T_OK;
@@ -1008,6 +1100,8 @@ int makeArgs(const tcpxbAttention& a, bool backward, int rows, Args* x) {
   x->out = x->o = a.out;
   x->doutPtr = a.dout.ptr;
   x->doutB = a.dout.stride_b, x->doutS = a.dout.stride_s, x->doutH = a.dout.stride_h;
+  x->vPtr = a.v.ptr, x->vB = a.v.stride_b, x->vS = a.v.stride_s, x->vH = a.v.stride_h;
+  x->bounds = nullptr, x->parts = 0;
   x->dq = a.dq, x->dk = a.dk, x->dv = a.dv, x->lse = a.lse, x->delta = a.delta;
   x->keyLengths = a.key_lengths, x->status = a.status;
   x->b = a.b, x->sq = a.sq, x->sk = a.sk, x->heads = a.heads, x->kvHeads = a.kv_heads, x->d = a.d, x->causal = a.causal, x->scale = a.scale;
@@ -1072,8 +1166,15 @@ template <class T, int P> int run(const tcpxbAttention& a, bool backward, cudaSt
                                        "attention forward");
   }
   if (a.b && a.sq) {
+    if constexpr (kLifted<T>) {
+      x.bounds = reinterpret_cast<const float2*>(a.bounds);
+      const long long pairs = (long long)a.kv_heads * a.b;
+      x.parts = int(std::clamp<long long>(2 * 148 / pairs, 1, kParts));
+      boundsKernel<T, P><<<dim3(x.parts, a.kv_heads, a.b), kBoundsThreads, 0, s>>>(x, reinterpret_cast<float2*>(a.bounds));
+      if (const int rc = launched("attention backward, bounds")) return rc;
+    }
     x.split = splitFor(tilesOfQueries * a.heads * a.b, colsOfKeys, 8);
-    if (const int rc = launch<queryKernel<T, P, false>, queryKernel<T, P, true>>(false, dim3(a.heads * x.split, a.b, unsigned(tilesOfQueries)), Tiling<P>::kThreads, Queries<T, P>::kShared, x,
+    if (const int rc = launch<queryKernel<T, P, false>, queryKernel<T, P, true>>(kLifted<T>, dim3(a.heads * x.split, a.b, unsigned(tilesOfQueries)), Tiling<P>::kThreads, Queries<T, P>::kShared, x,
                                                  device, s, "attention backward, queries"))
       return rc;
   }

@@ -401,3 +401,122 @@ def test_long_rows_of_few_queries(b, sq, sk, h, hk, d, dtype):
     check(q, k, v, dout)
     k[:, sk // 2] = math.nan
     assert ops.attention_forward(q, k, v)[0].isnan().all()
+
+
+def gradients_of(q, k, v, dout, out, lse, causal, lengths=None, scale=None):
+    """{name: (value, tolerance)} of dq, dk and dv as functions of what the backward call gets, in 64 bits: the probabilities come
+    from the given lse, and D from the given out, or from the row itself where its keys lie in one tile.  Roundings to the type: probabilities, score gradients and results; the rest
+    is 32-bit, as in train_oracle.  Under float16's normal range an operand would be off by half of its smallest step, 2^-25.
+    Probabilities are lifted by 2^14, score gradients by 2^e with 2^13 <= 2^e X, where X = d max|dout| max|v| over a key head's
+    rows that see a key and keys that are seen: that leaves 2^-39 and 2^-38 X."""
+    (b, sq, h, d), (sk, hk), u, f32 = q.shape, k.shape[1:3], oracle.half(q.dtype), oracle.F32
+    scale = d ** -0.5 if scale is None else scale
+    ok = oracle.visible(b, sq, sk, causal, lengths).cuda()
+    q, out, dout = (t.double().transpose(1, 2) for t in (q, out, dout))
+    seen = ok.expand(b, 1, sq, sk).any(2)[..., None]  # [b, 1, sk, 1]
+    k, v = (torch.where(seen, t.double().transpose(1, 2), 0.0).repeat_interleave(h // hk, 1) for t in (k, v))
+    p = torch.where(ok, (scale * (q @ k.mT) - lse.double()[..., None]).exp(), 0.0)
+    ep = (d + 8) * f32 * scale * (q.abs() @ k.abs().mT) + 8 * f32 * lse.double().abs().nan_to_num(posinf=0.0)[..., None] + 16 * f32
+    sees = ok.expand(b, 1, sq, sk).any(-1, keepdim=True)
+    x = d * (torch.where(sees, dout, 0.0).abs().amax((2, 3)) * v.abs().amax((2, 3))).unflatten(1, (hk, h // hk)).amax(2).repeat_interleave(h // hk, 1)[..., None, None]
+    dp, delta = dout @ v.mT, (dout * out).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    either = ((p * dp).sum(-1, keepdim=True) - delta).abs()
+    eds = ds.abs() * (u + ep) + p * (1 + u) * (either + (d + 8) * f32 * (dout.abs() @ v.abs().mT + (dout * out).abs().sum(-1, keepdim=True)))
+    eds, edp = torch.where(ok, eds + x * 2.0 ** -38, 0.0), torch.where(ok, p * (u + ep) + 2.0 ** -39, 0.0)
+    n, group = max(sq, sk) + 8, h // hk
+    least = torch.finfo(torch.float16).smallest_normal * torch.finfo(torch.float16).eps
+    shared = lambda t: t.unflatten(1, (hk, group)).sum(2)  # noqa: E731
+    dq, dk, dv = scale * (ds @ k), shared(scale * (ds.mT @ q)), shared(p.mT @ dout)
+    edq = u * dq.abs() + scale * ((eds + n * f32 * ds.abs()) @ k.abs())
+    edk = u * dk.abs() + shared(scale * ((eds + group * n * f32 * ds.abs()).mT @ q.abs()))
+    edv = u * dv.abs() + shared((edp + group * n * f32 * p).mT @ dout.abs())
+    return {name: (t.transpose(1, 2), e.transpose(1, 2) * 1.001 + least) for name, t, e in (("dq", dq, edq), ("dk", dk, edk), ("dv", dv, edv))}
+
+
+def check_gradients(q, k, v, dout, causal=False, lengths=None, scale=None):
+    how = {"causal": causal, "key_lengths": lengths, "scale": scale}
+    out, lse = ops.attention_forward(q, k, v, **how)
+    got = dict(zip(("dq", "dk", "dv"), ops.attention_backward(dout, q, k, v, out, lse, **how)))
+    for name, want in gradients_of(q, k, v, dout, out, lse, causal, lengths, scale).items():
+        oracle.close(got[name], want, name)
+    return got
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d", [(1, 2048, 2048, 4, 2, 64), (1, 2048, 2048, 2, 1, 128), (1, 300, 4096, 1, 1, 64), (2, 60, 50, 2, 1, 40), (1, 1500, 1024, 8, 1, 72)])
+def test_small_gradients_in_float16(b, sq, sk, h, hk, d, size, causal):
+    """Probabilities of thousands of keys times gradients of 1e-3 to 1e-5: score gradients under float16's smallest step."""
+    q, k, v, dout = inputs(b, sq, sk, h, hk, d, F16, seed=16)
+    check_gradients(q, k, v, (dout.float() * size).half(), causal)
+
+
+@gpu
+def test_probabilities_of_very_many_keys_in_float16():
+    """At 2^17 keys a probability is 2^-17, which float16 holds with seven bits."""
+    check_gradients(*inputs(1, 64, 1 << 17, 1, 1, 64, F16, seed=17))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_gradients_in_float16(d):
+    """Products of dout and v beyond float16's range, whose gradients are within it; peaked and flat rows."""
+    for spread in (0.1, 3.0):
+        q, k, v, dout = inputs(1, 400, 400, 2, 1, d, F16, seed=18)
+        got = check_gradients((q.float() * 30).half(), (k.float() * 30).half(), (v.float() * 100).half(), (dout.float() * 300).half(), True, scale=spread / (900 * d ** 0.5))
+        assert all(t.isfinite().all() for t in got.values())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_what_no_row_sees_does_not_take_bits(d, dtype):
+    """Large values behind a length, and large gradients of rows that see nothing, leave the others' small ones their bits."""
+    q, k, v, dout = inputs(2, 200, 300, 4, 2, d, dtype, seed=19)
+    dout = (dout.float() * 1e-5).to(dtype)
+    lens = torch.tensor([300, 130], dtype=torch.int32, device="cuda")
+    want = check_gradients(q, k, v, dout, False, lens)
+    v[1, 130:] = 6e4
+    v[1, 200:] = math.nan
+    got = check_gradients(q, k, v, dout, False, lens)
+    assert all(torch.equal(want[n], got[n]) for n in want)
+    q, k, v, dout = inputs(1, 300, 100, 4, 2, d, dtype, seed=20)
+    dout = (dout.float() * 1e-5).to(dtype)
+    want = check_gradients(q, k, v, dout, True)
+    dout[:, :200] = 6e4
+    got = check_gradients(q, k, v, dout, True)
+    assert all(torch.equal(want[n], got[n]) for n in want)
+
+
+@gpu
+def test_infinite_gradients_in_float16_stay_in_their_heads():
+    """A row of infinities (a loss scale that is too large) reaches what it touches and takes no bits from another head's small gradients."""
+    q, k, v, dout = inputs(1, 260, 260, 4, 2, 64, F16, seed=21)
+    dout = (dout.float() * 1e-5).half()
+    want = check_gradients(q, k, v, dout, True)
+    dout[:, 77, 0] = math.inf
+    out, lse = ops.attention_forward(q, k, v, causal=True)
+    got = dict(zip(want, ops.attention_backward(dout, q, k, v, out, lse, causal=True)))
+    assert not got["dq"][:, 77, 0].isfinite().any() and not got["dv"][:, 0, 0].isfinite().any()
+    got["dq"][:, 77, 0] = want["dq"][:, 77, 0]
+    assert torch.equal(got["dq"], want["dq"]) and all(torch.equal(got[n][:, :, 1], want[n][:, :, 1]) for n in want)
+
+
+def test_float16_gradients_need_their_scratch():
+    """The C entry refuses float16 gradients without the scratch for their bounds."""
+    import ctypes
+    import train_abi as A
+    lib = A.library()
+
+    class WithBounds(ctypes.Structure):
+        _fields_ = [("a", A.Attention), ("bounds", ctypes.c_void_p)]
+
+    a = A.Attention(b=1, sq=4, sk=4, heads=4, kv_heads=2, d=64, scale=0.1, dtype=3, **{n: 4096 for n in "out lse dq dk dv delta".split()})
+    for n in ("q", "k", "v", "dout"):
+        for field, x in ((n, 4096), (n + "_b", 1024), (n + "_s", 256), (n + "_h", 64)):
+            setattr(a, field, x)
+    for bounds in (None, 4100):
+        assert lib.tcpxb_attention_backward(ctypes.byref(WithBounds(a, bounds)), None) == -1
+        assert b"bounds" in lib.tcpxb_train_last_error()
