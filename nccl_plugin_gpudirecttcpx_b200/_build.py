@@ -4,7 +4,8 @@ The reference builds one shared library out of per-directory static libraries wi
 CMake (reference: CMakeLists.txt:19-117, src/CMakeLists.txt:15-82).  Here the same
 sources are also buildable without CMake, so that `build()` in the repo root's
 entry file and the test-suite can produce the libraries with nothing but nvcc
-and g++.  Outputs land in `nccl_plugin_gpudirecttcpx_b200/_lib/`:
+and g++; the training operators' Python module, which comes last, also needs torch and
+is left out where there is none.  Outputs land in `nccl_plugin_gpudirecttcpx_b200/_lib/`:
 
   libtcpxb_kernels.so   device kernels behind a C ABI (needs nvcc)
   libtcpxb_train.so     the training step's operators behind a C ABI (needs nvcc)
@@ -16,7 +17,8 @@ and g++.  Outputs land in `nccl_plugin_gpudirecttcpx_b200/_lib/`:
   tcpxb_rxdm            rx buffer manager daemon (host pools; g++ only)
   tcpxb_rxdm_gpu        the same daemon linked against the CUDA build: can own device pools
 
-Objects are rebuilt only when a source or header is newer than the object.
+Objects are rebuilt only when a source or header is newer than the object, the Python module
+also when another torch or Python builds it.
 """
 from __future__ import annotations
 
@@ -129,7 +131,7 @@ def build_cuda(verbose: bool = False) -> list[Path]:
     tlib = OUT / "libtcpxb_train.so"
     if _stale(tlib, tobjs, 0.0):
         _run([nvcc, "-shared", "-o", str(tlib)] + [str(o) for o in tobjs] + ["-cudart", "static"])
-    outs = [klib, tlib, _build_torch_module(nvcc, tlib, hdr, verbose)]
+    outs = [klib, tlib]
     core = _sources("core", ".cc") + _sources("plugin", ".cc") + _sources("engine", ".cc")
     if core:
         cobjs = _compile(core, "full", ["g++"], CXX_FLAGS + ["-I", _cuda_include(nvcc)], hdr, verbose)
@@ -146,24 +148,36 @@ def build_cuda(verbose: bool = False) -> list[Path]:
             _run(["g++"] + CXX_FLAGS + ["-I", _cuda_include(nvcc), str(src), "-o", str(daemon), "-L", str(OUT),
                                         f"-l:{plug.name}", "-Wl,-rpath,$ORIGIN", "-ldl", "-pthread"])
         outs.append(daemon)
-    return outs
+    mod = _build_torch_module(nvcc, tlib, hdr, verbose)
+    return outs + ([mod] if mod else [])
 
 
-def _build_torch_module(nvcc: str, tlib: Path, hdr: float, verbose: bool) -> Path:
-    """The module that ops/train.py calls, against the torch that runs this."""
+def _build_torch_module(nvcc: str, tlib: Path, hdr: float, verbose: bool) -> Path | None:
+    """The module that ops/train.py calls, against the torch that runs this; none without torch."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        if verbose:
+            print("[build] no torch: the training operators' Python module is left out", flush=True)
+        return None
     home = Path(torch.__file__).parent
     inc = [str(home / "include"), str(home / "include/torch/csrc/api/include"), sysconfig.get_paths()["include"], _cuda_include(nvcc)]
     flags = CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=tcpxb_train_torch", "-Wno-unused-parameter"]
     for d in inc:
         flags += ["-isystem", d]
+    # what the objects were built against is in no file's time
+    stamp, against = OBJ / "torch.stamp", f"{torch.__version__}\n{sys.version}\n" + "\n".join(flags)
+    if not stamp.exists() or stamp.read_text() != against:
+        stamp.unlink(missing_ok=True)
+        hdr = float("inf")  # newer than any object
     objs = _compile(_sources("bind", ".cc"), "torch", ["g++"], flags, hdr, verbose)
     mod = OUT / "tcpxb_train_torch.so"
-    if _stale(mod, objs + [tlib], 0.0):
+    if _stale(mod, objs + [tlib], hdr if hdr == float("inf") else 0.0):
         _run(["g++", "-shared", "-o", str(mod)] + [str(o) for o in objs] + ["-L", str(OUT), f"-l:{tlib.name}", "-Wl,-rpath,$ORIGIN", "-L", str(home / "lib"),
              "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
+    stamp.write_text(against)
     return mod
 
 
