@@ -86,8 +86,10 @@ class AdamW(torch.optim.Optimizer):
             lists += [(group, ps, [p.grad.contiguous() for p in ps]) for ps in kinds.values()]
         norm = None
         if self.max_grad_norm is not None and len(lists) > 1:
-            # one norm for lists of several types or groups
-            norm = torch.linalg.vector_norm(torch.stack([grad_norm(grads) for _, _, grads in lists]))
+            # one norm for lists of several types, groups or devices, on the first one's
+            norms = [grad_norm(grads) for _, _, grads in lists]
+            norm = torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]))
+        total = norm
         for group, ps, grads in lists:
             states = [self._state_of(p) for p in ps]
             more = {}
@@ -96,8 +98,11 @@ class AdamW(torch.optim.Optimizer):
             if "master" in states[0]:
                 more["masters"] = [s["master"] for s in states]
             got = adamw_step(ps, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], [s["step"] for s in states], lr=group["lr"],
-                             betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], max_grad_norm=self.max_grad_norm, norm=norm, **more)
-            self.grad_norm = got
+                             betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], max_grad_norm=self.max_grad_norm,
+                             norm=None if norm is None else norm.to(ps[0].device), **more)
+            total = got if total is None else total
+        if lists:
+            self.grad_norm = total
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:

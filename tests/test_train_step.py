@@ -241,6 +241,22 @@ def test_model_with_head_norms_on_the_cpu():
     assert sum(n.endswith(("q_norm.weight", "k_norm.weight")) for n, _ in m.named_parameters()) == 2 * cfg.n_layers
 
 
+def test_optimizer_clips_over_several_devices(monkeypatch):
+    """One norm over all devices, given to each on its own; the kernels' calls are recorded, the second device has no memory."""
+    from nccl_plugin_gpudirecttcpx_b200.ops import optimizer
+    norms, calls = {"cpu": 3.0, "meta": 4.0}, []
+    # a device without memory cannot give its norm away: both come from the first one's
+    monkeypatch.setattr(optimizer, "grad_norm", lambda grads: torch.tensor(norms[grads[0].device.type]))
+    monkeypatch.setattr(optimizer, "adamw_step", lambda ps, *args, norm, **kw: calls.append((ps[0].device, norm)))
+    ps = [torch.nn.Parameter(torch.zeros(3, device=d)) for d in ("cpu", "meta")]
+    for p in ps:
+        p.grad = torch.zeros_like(p)
+    opt = ops.AdamW(ps, max_grad_norm=1.0)
+    opt.step()
+    assert [d.type for d, _ in calls] == [n.device.type for _, n in calls] == ["cpu", "meta"]
+    assert calls[0][1].item() == 5.0 and opt.grad_norm.item() == 5.0
+
+
 def test_optimizer_refusals():
     p = torch.nn.Parameter(torch.zeros(3))
     for kind, kw in ((ValueError, {"lr": -1.0}), (ValueError, {"betas": (1.0, 0.9)}), (ValueError, {"eps": -1.0}), (ValueError, {"weight_decay": -1.0}),
