@@ -39,7 +39,14 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, group: dict) -> None:
         super().add_param_group(group)
-        group = self.param_groups[-1]
+        try:
+            self._check_group(self.param_groups[-1])
+        except (TypeError, ValueError):
+            del self.param_groups[-1]  # a group that is refused is not there
+            raise
+
+    @staticmethod
+    def _check_group(group: dict) -> None:
         if isinstance(group["lr"], torch.Tensor):
             raise TypeError("the learning rate has to be a number")
         (beta1, beta2), numbers = group["betas"], (group["lr"], group["eps"], group["weight_decay"])

@@ -241,6 +241,17 @@ def test_model_with_head_norms_on_the_cpu():
     assert sum(n.endswith(("q_norm.weight", "k_norm.weight")) for n, _ in m.named_parameters()) == 2 * cfg.n_layers
 
 
+def test_a_refused_group_is_not_kept():
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
+    opt = ops.AdamW([p], lr=0.5)
+    for kind, kw in ((ValueError, {"lr": -1.0}), (TypeError, {"lr": torch.tensor(0.1)}), (ValueError, {"betas": (1.0, 0.9)})):
+        with pytest.raises(kind):
+            opt.add_param_group({"params": [q], **kw})
+        assert [g["lr"] for g in opt.param_groups] == [0.5]
+    opt.add_param_group({"params": [q]})
+    assert len(opt.param_groups) == 2
+
+
 def test_optimizer_clips_over_several_devices(monkeypatch):
     """One norm over all devices, given to each on its own; the kernels' calls are recorded, the second device has no memory."""
     from nccl_plugin_gpudirecttcpx_b200.ops import optimizer
