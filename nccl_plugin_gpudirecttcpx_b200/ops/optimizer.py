@@ -121,6 +121,11 @@ class AdamW(torch.optim.Optimizer):
         for p, s in zip(own, states):
             if s and set(s) != names | ({"master"} if self.master_weights and p.dtype is not torch.float32 else set()):
                 raise ValueError(f"the states hold {sorted(s)}: they are of another state_bits or master_weights")
+            for name, t in (s or {}).items():
+                kind = torch.int32 if name == "step" else torch.float32 if self.state_bits == 32 or name not in ("exp_avg", "exp_avg_sq") else torch.float8_e4m3fn
+                size = 1 if name == "step" else -(-p.numel() // STATE_BLOCK) if name.endswith("_scale") else p.numel()
+                if not isinstance(t, torch.Tensor) or t.dtype is not kind or t.numel() != size or not t.is_contiguous():
+                    raise ValueError(f"the state {name} has to be a contiguous {kind} tensor of {size}: these are another optimizer's or of other parameters")
         super().load_state_dict(state_dict)
         for p, s in zip(own, states):
             if s:

@@ -252,6 +252,31 @@ def test_a_refused_group_is_not_kept():
     assert len(opt.param_groups) == 2
 
 
+def test_states_of_another_optimizer_are_refused():
+    """torch.optim.AdamW's have the same names and other types; nothing is loaded of what is refused."""
+    p, q = torch.nn.Parameter(torch.zeros(300)), torch.nn.Parameter(torch.zeros(300))
+    other = torch.optim.AdamW([p])
+    p.grad = torch.ones(300)
+    other.step()
+    good = {"step": torch.ones((), dtype=torch.int32), "exp_avg": torch.ones(300), "exp_avg_sq": torch.ones(300)}
+    opt = ops.AdamW([q])
+    groups = opt.state_dict()["param_groups"]
+    opt.load_state_dict({"state": {0: good}, "param_groups": groups})
+    bad = [other.state_dict()["state"][0]] + [{**good, n: t} for n, t in (
+        ("step", torch.ones(2, dtype=torch.int32)), ("exp_avg", torch.ones(299)), ("exp_avg", torch.ones(300, dtype=BF16)), ("exp_avg_sq", torch.ones(300, 2)[:, 0]))]
+    for state in bad:
+        with pytest.raises(ValueError, match="state"):
+            opt.load_state_dict({"state": {0: state}, "param_groups": groups})
+        assert all(torch.equal(opt.state[q][n], t) and opt.state[q][n].dtype is t.dtype for n, t in good.items())
+    small = {n: torch.ones(1 if n == "step" else 2 if n.endswith("scale") else 300).to(torch.int32 if n == "step" else torch.float32 if n.endswith("scale") else torch.float8_e4m3fn)
+             for n in ("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
+    opt = ops.AdamW([q], state_bits=8)
+    opt.load_state_dict({"state": {0: small}, "param_groups": groups})
+    for n, t in (("exp_avg", torch.ones(300)), ("exp_avg_scale", torch.ones(300))):
+        with pytest.raises(ValueError, match="state"):
+            opt.load_state_dict({"state": {0: {**small, n: t}}, "param_groups": groups})
+
+
 def test_optimizer_clips_over_several_devices(monkeypatch):
     """One norm over all devices, given to each on its own; the kernels' calls are recorded, the second device has no memory."""
     from nccl_plugin_gpudirecttcpx_b200.ops import optimizer
