@@ -108,8 +108,9 @@ class AdamW(torch.optim.Optimizer):
                              betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], max_grad_norm=self.max_grad_norm,
                              norm=None if norm is None else norm.to(ps[0].device), **more)
             total = got if total is None else total
-        if lists:
-            self.grad_norm = total
+        if total is None and self.max_grad_norm is not None:
+            total = torch.zeros((), device=self.param_groups[0]["params"][0].device)  # of no gradients
+        self.grad_norm = total
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:

@@ -277,6 +277,15 @@ def test_states_of_another_optimizer_are_refused():
             opt.load_state_dict({"state": {0: {**small, n: t}}, "param_groups": groups})
 
 
+def test_the_norm_of_a_step_without_gradients_is_zero():
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = ops.AdamW([p], max_grad_norm=1.0)
+    opt.grad_norm = torch.tensor(7.0)  # an earlier step's
+    opt.step()
+    assert opt.grad_norm.item() == 0.0
+    assert not opt.state
+
+
 def test_optimizer_clips_over_several_devices(monkeypatch):
     """One norm over all devices, given to each on its own; the kernels' calls are recorded, the second device has no memory."""
     from nccl_plugin_gpudirecttcpx_b200.ops import optimizer
