@@ -109,7 +109,7 @@ class AdamW(torch.optim.Optimizer):
                              norm=None if norm is None else norm.to(ps[0].device), **more)
             total = got if total is None else total
         if total is None and self.max_grad_norm is not None:
-            total = torch.zeros((), device=self.param_groups[0]["params"][0].device)  # of no gradients
+            total = torch.zeros((), device=next((p.device for g in self.param_groups for p in g["params"]), None))  # of no gradients
         self.grad_norm = total
         return loss
 

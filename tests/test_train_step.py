@@ -279,7 +279,7 @@ def test_states_of_another_optimizer_are_refused():
 
 def test_the_norm_of_a_step_without_gradients_is_zero():
     p = torch.nn.Parameter(torch.zeros(3))
-    opt = ops.AdamW([p], max_grad_norm=1.0)
+    opt = ops.AdamW([{"params": []}, {"params": [p]}], max_grad_norm=1.0)
     opt.grad_norm = torch.tensor(7.0)  # an earlier step's
     opt.step()
     assert opt.grad_norm.item() == 0.0
