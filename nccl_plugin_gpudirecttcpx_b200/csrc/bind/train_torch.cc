@@ -4,12 +4,12 @@
 // and its attention, both ways, 39 us, of which the device needed 11 and 15; here 22 and 19.5 us.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
 #include <cmath>
 #include <optional>
+#include <variant>
 #include <vector>
 
 #include "tcpxb/train.h"
@@ -289,7 +289,7 @@ Tensor gradNorm(const List& grads) {
   return norm;
 }
 
-Maybe adamwStep(const List& params, const List& grads, const List& ms, const List& vs, py::object steps, double lr, double beta1, double beta2, double eps,
+Maybe adamwStep(const List& params, const List& grads, const List& ms, const List& vs, const std::variant<Tensor, List>& steps, double lr, double beta1, double beta2, double eps,
                 double decay, std::optional<double> maxNorm, Maybe norm, std::optional<List> mScales, std::optional<List> vScales, std::optional<List> masters) {
   TORCH_CHECK_VALUE(!params.empty(), "no tensors");
   const Tensor& first = params[0];
@@ -316,15 +316,15 @@ Maybe adamwStep(const List& params, const List& grads, const List& ms, const Lis
   Ranges ranges;
   ranges.reserve(count * 8 + 2);
   const auto write = [&](const Tensor& t) { return ranges.add(t, true); };
-  if (THPVariable_Check(steps.ptr())) {
-    const Tensor& t = THPVariable_Unpack(steps.ptr());
+  if (const auto* whole = std::get_if<Tensor>(&steps)) {
+    const Tensor& t = *whole;
     TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, "steps has to be int32, got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.dim() == 1 && size_t(t.size(0)) == count && t.is_contiguous() && t.device() == first.device(), "steps has to be a contiguous [", count,
                       "] on the same device, got ", t.sizes());
     auto* first = static_cast<int32_t*>(write(t));
     for (size_t i = 0; i < count; i++) table[i].step = first + i;
   } else {
-    const List list = steps.cast<List>();
+    const List& list = std::get<List>(steps);
     checkList("steps", list, count, at::kInt, first, [](size_t) { return 1; });
     for (size_t i = 0; i < count; i++) table[i].step = static_cast<int32_t*>(write(list[i]));
   }
@@ -356,13 +356,21 @@ Maybe adamwStep(const List& params, const List& grads, const List& ms, const Lis
   return norm;
 }
 
+// Other Python threads run meanwhile: an allocation or a launch may wait for the device, and what the
+// device waits for may be another thread's to give.
+struct Release {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Release() { PyEval_RestoreThread(state); }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(tcpxb_train_torch, m) {
-  m.def("attention_forward", &attentionForward);
-  m.def("attention_backward", &attentionBackward);
-  m.def("norm_rope_forward", &normRopeForward);
-  m.def("norm_rope_backward", &normRopeBackward);
-  m.def("grad_norm", &gradNorm);
-  m.def("adamw_step", &adamwStep);
+  using Unlocked = py::call_guard<Release>;
+  m.def("attention_forward", &attentionForward, Unlocked());
+  m.def("attention_backward", &attentionBackward, Unlocked());
+  m.def("norm_rope_forward", &normRopeForward, Unlocked());
+  m.def("norm_rope_backward", &normRopeBackward, Unlocked());
+  m.def("grad_norm", &gradNorm, Unlocked());
+  m.def("adamw_step", &adamwStep, Unlocked());
 }

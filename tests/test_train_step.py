@@ -209,6 +209,41 @@ def test_a_captured_step_of_the_model():
         assert torch.equal(p, q)
 
 
+@gpu
+def test_other_threads_run_while_a_launch_waits():
+    """A full queue of launches makes the next one wait; a second Python thread goes on meanwhile."""
+    import threading
+    import time
+    q = torch.randn(1, 64, 2, 64, device="cuda").to(BF16)
+    p, g, m, v = (torch.zeros(10, device="cuda") for _ in range(4))
+    steps = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cos = sin = torch.zeros(64, 32, device="cuda")
+    for call in (lambda: ops.attention(q, q, q), lambda: ops.qk_norm_rope(q, q, cos, sin), lambda: ops.adamw_step([p], [g], [m], [v], steps, lr=0.0)):
+        call()
+        torch.cuda.synchronize()
+        ticks, done = [], threading.Event()
+
+        def tick():
+            while not done.is_set():
+                ticks.append(time.perf_counter())
+                time.sleep(0.002)
+
+        thread = threading.Thread(target=tick)
+        thread.start()
+        try:
+            torch.cuda._sleep(1_500_000_000)  # most of a second
+            began = time.perf_counter()
+            for _ in range(3000):
+                call()
+            waited = time.perf_counter() - began
+        finally:
+            done.set()
+            thread.join()
+        torch.cuda.synchronize()
+        assert waited > 0.4  # the queue was full
+        assert max(b - a for a, b in zip(ticks, ticks[1:])) < waited / 2
+
+
 def _ddp(args):
     cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=1", "--master-addr", "127.0.0.1", "--master-port", str(free_port()),
            "-m", "nccl_plugin_gpudirecttcpx_b200.parallel.ddp", "--tiny", "--steps", "3", "--warmup", "2", *args]
