@@ -504,6 +504,32 @@ def test_infinite_gradients_in_float16_stay_in_their_heads():
     assert torch.equal(got["dq"], want["dq"]) and all(torch.equal(got[n][:, :, 1], want[n][:, :, 1]) for n in want)
 
 
+@gpu
+def test_float16_in_two_graphs():
+    """The maxima's scratch is each graph's own: two graphs with gradients of very different sizes replay at the same time."""
+    sets = [inputs(2, 260, 700, 4, 2, 64, F16, seed=22 + i) for i in range(2)]
+    sets[0][3].mul_(1e-4), sets[1][3].mul_(1e2)
+    wanted = []
+    for s in sets:
+        out, lse = ops.attention_forward(*s[:3])
+        wanted.append(ops.attention_backward(s[3], *s[:3], out, lse))
+    runs = []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out, lse = ops.attention_forward(*s[:3])
+            runs.append((g, ops.attention_backward(s[3], *s[:3], out, lse)))
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (g, _), st in zip(runs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for want, (_, got) in zip(wanted, runs):
+        assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
 def test_float16_gradients_need_their_scratch():
     """The C entry refuses float16 gradients without the scratch for their bounds."""
     import ctypes
