@@ -251,7 +251,7 @@ __device__ __forceinline__ float warpTop(float x) {
   asm("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
-// About 310 instructions a block, of which 64 are the step itself: at this count issue and memory
+// About 320 instructions a block, of which 64 are the step itself: at this count issue and memory
 // take about the same time, so the rest is kept short (the warp's maximum is one instruction, the four
 // factors of a block are taken by four lanes at once).
 template <bool kVector, bool kWide, class T, class W>

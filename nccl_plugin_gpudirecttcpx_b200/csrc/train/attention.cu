@@ -13,8 +13,9 @@
 //
 // All three kernels work on tiles of scores, 128 rows high.  One warp loads tiles with TMA, one
 // thread issues the matrix instructions, and eight warps turn scores into the operand of the
-// next product, in tensor memory: the score tile is read into registers (a thread has one row, or
-// half of one) and P or dS is written back over it in 16 bits.  A head size under 64 or between
+// next product, in tensor memory: the score tile is read into registers (forward a thread has a row, for
+// the gradients of queries half of one, for those of keys two columns of every eight in four rows) and P or
+// dS is written back over it in 16 bits.  A head size under 64 or between
 // 64 and 128 fills its panel with zeros from the load.
 //
 // Head sizes above 64 take score tiles of 128 columns and one block on an SM: all of its tensor
@@ -609,7 +610,9 @@ template <class T, int P, bool kSplit> __global__ void __launch_bounds__(Tiling<
   if (warp == kMmaWarp) dead[1] = 1;
   const int n = uniform(*dead) ? 0 : int((long long)all * (rank + 1) / split) - begun;
   if constexpr (kLifted<T>) waitForPrevious();  // for the bounds
-  letNextStart();  // all blocks have their tensor memory
+  // The next kernel's blocks may come now, before this one's allocation even: shared memory keeps any that
+  // would need this block's tensor memory off the SM until it has left.
+  letNextStart();
 
   if (warp == kLoadWarp) {
     L::other();

@@ -189,7 +189,8 @@ template <> struct MmaType<__nv_bfloat16> { static constexpr uint32_t code = 1; 
 template <class T> __device__ __forceinline__ constexpr uint32_t mmaShape(int n, bool bRows) {
   return 1u << 4 | MmaType<T>::code << 7 | MmaType<T>::code << 10 | (bRows ? 1u << 16 : 0u) | uint32_t(n / 8) << 17 | 8u << 24;
 }
-// Operand tiles are panels of 64 elements x 128 rows: a row of 128 bytes, groups of eight rows 1024 bytes apart.
+// Operand tiles are panels of 64 elements x 128 rows (a panel of score columns has 64 rows with heads up to 64):
+// a row of 128 bytes, groups of eight rows 1024 bytes apart.
 constexpr uint32_t kPanelBytes = 128 * 128;
 __device__ __forceinline__ uint64_t operandDesc(uint32_t addr, uint32_t panelStride) {
   return uint64_t((addr & 0x3ffff) >> 4) | uint64_t(panelStride >> 4) << 16 | uint64_t(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;

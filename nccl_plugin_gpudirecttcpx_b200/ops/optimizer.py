@@ -1,4 +1,4 @@
-"""AdamW as a torch optimizer, on top of `adamw_step`: the whole parameter list in a few launches."""
+"""AdamW as a torch optimizer, on top of `adamw_step`: a few launches for each 380 parameters of a group and type."""
 from __future__ import annotations
 
 import itertools
@@ -14,7 +14,8 @@ class AdamW(torch.optim.Optimizer):
     """AdamW over bfloat16, float16 or float32 CUDA parameters, with states in 32 or 8 bits.
 
     `state_bits`: 32 keeps float32 states.  8 keeps float8 codes with a scale for each 256 elements: a
-    quarter of the memory and of the states' traffic; a state is off by up to 2^-4 of its value.
+    quarter of the memory and of the states' traffic; a state is off by up to 2^-4 of its value, small ones of a
+    block by up to 2^-10 (a root that is raised to the smallest code: 2^-9) of the block's largest over 448.
     `master_weights`: float32 weights behind 16-bit parameters, which then are their rounded copies: they are
     taken from the parameters at the first step and part of the state, which is loaded with the model's.
     `max_grad_norm`: gradients are scaled, while they are read, by min(1, max_grad_norm / (norm + 1e-6))

@@ -134,7 +134,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                weight_decay: float = 1e-2, max_grad_norm: Optional[float] = None, norm: Optional[torch.Tensor] = None,
                exp_avg_scales: Optional[Sequence[torch.Tensor]] = None, exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
                masters: Optional[Sequence[torch.Tensor]] = None) -> Optional[torch.Tensor]:
-    """One AdamW step over all tensors, in place, in two launches (three with clipping).
+    """One AdamW step over all tensors, in place.  Up to 380 of them take two launches (three with clipping), longer lists as
+    many for each 380.
 
     `params` and `grads`: contiguous tensors of one type (bfloat16, float16, float32) on one device.
     States in 32 bits: `exp_avgs` and `exp_avg_sqs` are float32 tensors of the params' sizes.  In 8 bits:
