@@ -80,7 +80,8 @@ class Attention(nn.Module):
     def _forward_kernels(self, x, cos, sin):
         B, S, _ = x.shape
         q, k, v = (w(x).view(B, S, -1, self.d) for w in (self.wq, self.wk, self.wv))
-        weights = (None, None) if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
+        # under autocast the heads come in 16 bits and the weights in 32: the kernel takes both in one type, which rounds the weights
+        weights = (None, None) if self.q_norm is None else (self.q_norm.weight.to(q.dtype), self.k_norm.weight.to(k.dtype))
         q, k = ops.qk_norm_rope(q, k, cos, sin, *weights, eps=self.eps)
         return self.wo(ops.attention(q, k, v, causal=True).view(B, S, self.h * self.d))
 

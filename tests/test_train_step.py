@@ -177,6 +177,32 @@ def test_model_gradients(qk_norm, heads):
 
 
 @gpu
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_model_under_autocast(qk_norm):
+    """32-bit parameters, heads in 16 bits.  Against the decoder in 64 bits, as in test_model_gradients; the norms' weights are
+    numbers that 16 bits hold, so that their cast takes nothing the plain decoder keeps."""
+    cfg = LlamaConfig(vocab_size=300, d_model=64, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=128, qk_norm=qk_norm)
+    torch.manual_seed(5)
+    plain = LlamaDecoder(cfg).cuda()
+    with torch.no_grad():
+        for n, p in plain.named_parameters():
+            if n.endswith(("q_norm.weight", "k_norm.weight")):
+                p.copy_((1 + 0.2 * torch.randn_like(p)).to(BF16))
+    exact, kernels = copy.deepcopy(plain).double(), LlamaDecoder(LlamaConfig(**{**cfg.__dict__, "kernels": True})).cuda()
+    kernels.load_state_dict(plain.state_dict())
+    tokens = torch.randint(0, 300, (2, 77), device="cuda", generator=torch.Generator("cuda").manual_seed(6))
+    grads = []
+    for model in (exact, plain, kernels):
+        with torch.autocast("cuda", BF16, enabled=model is not exact):
+            loss = model(tokens[:, :-1], tokens[:, 1:])
+        loss.backward()
+        grads.append({n: p.grad.double() for n, p in model.named_parameters()})
+    for n, want in grads[0].items():
+        off = [(g[n] - want).norm() / want.norm() for g in grads[1:]]
+        assert off[1] <= 2 * off[0], (n, off)
+
+
+@gpu
 def test_a_captured_step_of_the_model():
     """Forward, backward and optimizer in one graph give what eager steps give."""
     cfg = LlamaConfig.tiny()
