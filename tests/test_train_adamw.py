@@ -170,6 +170,18 @@ def test_small_roots_stay_above_zero_in_8_bits():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,master", [(BF16, False), (F16, False), (F32, False), (BF16, True), (F16, True)])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset,eps", [(0, 0.0), (1, 0.0), (0, 1e-15), (8, 1e35)])
+def test_eps_of_the_kernels_with_quotients(dtype, master, bits, offset, eps):
+    s = tensors(SIZES, dtype, bits, master, seed=30 + offset, offset=offset)
+    for _ in range(2):
+        step_and_check(s, {**HOW, "eps": eps})
+    many = tensors([300] * 30, dtype, bits, master, seed=31)
+    step_and_check(many, {**HOW, "eps": eps}, max_grad_norm=0.5)
+
+
+@gpu
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("eps", [0.0, 1e-39, 1e-30, 1e-20, 1e-18, 1e-12, 1e-10, 1e33])
 def test_small_second_moments_and_extreme_eps(bits, eps):

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import train_oracle as oracle
-from nccl_plugin_gpudirecttcpx_b200 import ops
+from nccl_plugin_gpudirecttcpx_b200 import _build, ops
 
 gpu = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -233,12 +233,12 @@ extern "C" int run(int blocks, unsigned long long ns, void* stream) {
 
 
 @gpu
+@pytest.mark.skipif(not _build._nvcc(), reason="needs nvcc")
 def test_tensor_memory_that_another_kernel_holds(tmp_path):
     """Blocks that get their tensor memory later than a wait may last: no wait runs out over it."""
     import ctypes
     import subprocess
     import time
-    from nccl_plugin_gpudirecttcpx_b200 import _build
     (tmp_path / "hold.cu").write_text(HOLDER)
     subprocess.run([_build._nvcc(), *_build.NVCC_ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", tmp_path / "hold.so", tmp_path / "hold.cu"], check=True)
     hold = ctypes.CDLL(str(tmp_path / "hold.so")).run
